@@ -20,7 +20,9 @@ OBJDIR = os.path.join(PKG, "build")
 LIB = os.path.join(LIBDIR, "libvo_hip.so")
 ARCH = "gfx950"
 CFLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-Wall", "-Wno-unused-function",
-          "-fno-gpu-rdc", "-DNDEBUG"]
+          "-fno-gpu-rdc", "-DNDEBUG",
+          # no packed float32 arithmetic (v_pk_add/mul/fma_f32): some of its forms have given wrong results now and then
+          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-Wno-unknown-warning-option"]
 
 
 def hipcc() -> str:
