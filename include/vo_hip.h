@@ -85,6 +85,8 @@ int vo_erode3x3_u8(const uint8_t* in, uint8_t* out, int H, int W, void* stream);
  * mixed_precision switch (stereo/raft_args.json:7).  Arithmetic is float32 either way;
  * biases, scales and shifts are always float32. */
 enum { VO_F32 = 0, VO_F16 = 1 };
+/* A third storage type, of the token-major operators (vo_linear, vo_attention) only. */
+enum { VO_BF16 = 2 };
 
 /* ---------------------------------------------------------------------------
  * Fused, in-place normalisation / activation passes of the conv encoders (the
@@ -608,6 +610,28 @@ int vo_ransac_kabsch_batch(const double* P, const double* Q, const uint8_t* weig
                            double threshold, int iterations, uint64_t seed,
                            double* T_out, int32_t* n_inliers_out, uint8_t* inlier_mask_out,
                            int batch, int N, int64_t first_pair, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Token-major matrix product with bias, activation and residual in its store:
+ *     y[m,k] = act( sum_c x[m,c] * weight[k,c] + bias[k] ) + residual[m,k]
+ * It has NO counterpart in the reference; it is vo_conv1x1 for tensors whose rows are pixels or tokens (the layout of
+ * vo_conv1x1_pixel_major's output and of vo_attention below), in three storage types.
+ *   x (M,C), y and residual (M,K): rows of consecutive elements, row strides in ELEMENTS (at least the row's length).
+ *   weight (K,C) dense, bias (K) float32 or NULL, residual NULL or of x's type.  y may be the residual itself (same
+ *   pointer and stride); otherwise it must not overlap any input.
+ *   activation  VO_ACT_*: GELU is 0.5 z (1 + erf(z/sqrt(2))), GELU_TANH its tanh form, SILU z / (1 + exp(-z)).
+ *   dtype       VO_F32, VO_F16 or VO_BF16 of x, weight, residual and y.  Products and sums in float32, one rounding.
+ * Any M >= 0, C >= 1, K >= 1 and any alignment; whole 16-byte pieces per row (C, strides and pointers) are read straight
+ * into LDS, others through registers.  Rows of x and weight must be under 8 MiB (VO_ERR_UNSUPPORTED).
+ * workspace: vo_linear_workspace_bytes(M, C, K, dtype) bytes (often 0), 16-byte aligned, contents irrelevant.  Calls that
+ * share one must be ordered on one stream; two captured graphs that may replay at once need one each.
+ * ------------------------------------------------------------------------- */
+enum { VO_ACT_NONE = 0, VO_ACT_RELU = 1, VO_ACT_GELU = 2, VO_ACT_GELU_TANH = 3, VO_ACT_SILU = 4 };
+int64_t vo_linear_workspace_bytes(int64_t M, int C, int K, int dtype);
+int vo_linear(const void* x, int64_t x_row_stride, const void* weight, const float* bias,
+              const void* residual, int64_t residual_row_stride, void* y, int64_t y_row_stride,
+              int64_t M, int C, int K, int activation, int dtype,
+              void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -15,6 +15,7 @@ LIB_PATH = os.path.join(_PKG, "lib", "libvo_hip.so")
 VO_OK, VO_ERR_INVALID_ARG, VO_ERR_LAUNCH, VO_ERR_UNSUPPORTED = 0, -1, -2, -3
 ABI_VERSION = 301           # the VO_HIP_VERSION of include/vo_hip.h that SIGNATURES below was written for
 VO_PIECES_BF16, VO_PIECES_F16 = 0, 1
+VO_ACT_NONE, VO_ACT_RELU, VO_ACT_GELU, VO_ACT_GELU_TANH, VO_ACT_SILU = range(5)
 
 _P, _I, _L, _D, _F = c_void_p, c_int, c_int64, c_double, c_float
 
@@ -88,9 +89,11 @@ SIGNATURES = {
     "vo_pair_poses": [_P, _L, _P, _P, _P, _P, _D, _D, _D, _P, _I, _P, _P, _P, _L, _I, _I, _I, _I, _P],
     "vo_pair_poses_static": [_P, _L, _P, _P, _P, _P, _D, _D, _D, _P, _I, _P, _P, _I, _I, _I, _I, _P],
     "vo_ransac_kabsch_batch": [_P, _P, _P, _D, _I, c_uint64, _P, _P, _P, _I, _I, _L, _P],
+    "vo_linear": [_P, _L, _P, _P, _P, _L, _P, _L, _L, _I, _I, _I, _I, _P, _L, _P],
 }
 # entry points that return a size instead of a status
-SIZE_QUERIES = {"vo_pair_poses_workspace_bytes": [_I, _I]}
+SIZE_QUERIES = {"vo_pair_poses_workspace_bytes": [_I, _I],
+                "vo_linear_workspace_bytes": [_L, _I, _I, _I]}
 EXPORTS = sorted(list(SIGNATURES) + list(SIZE_QUERIES) + ["vo_version", "vo_last_error"])
 
 _lib = None

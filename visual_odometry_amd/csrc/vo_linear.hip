@@ -1,0 +1,424 @@
+// Token-major matrix product with a fused epilogue: y = act(x W^T + b) + r.
+//   x (M,C) rows, W (K,C) rows, b (K) float32, r and y (M,K) rows; float32, float16 or bfloat16 storage, products and the
+//   sum over C in float32 on the matrix cores, epilogue in float32, one rounding at the store.
+//
+// Three forms, chosen by vo_linear's plan():
+//   tiles   a workgroup forms a BM x BN tile of y; both operands go through LDS in slabs of 128 bytes per row
+//   rows    few rows of x: the read of W is the work.  Waves stream W straight into registers
+//   both can be split over C: partial sums go to a workspace and a second kernel adds them in a fixed order.
+#include "vo_tokens.h"
+
+namespace {
+
+struct LinArgs {
+    const void* x;
+    const void* w;
+    const float* bias;
+    const void* res;
+    void* y;
+    float* part;                     // split over C: partial sums (splits, M, K)
+    int64_t xs, rs, ys;              // row strides in elements
+    int64_t M;
+    int C, K, act;
+    int splits, c_per_split;         // c_per_split: a multiple of the slab
+    unsigned tiles_m, tiles_n;
+    int wide_out;                    // y, r rows allow 16-byte accesses
+};
+
+__device__ __forceinline__ float activate(float z, int act) {
+    switch (act) {
+        case VO_ACT_RELU: return z < 0.f ? 0.f : z;                                          // NaN stays NaN
+        case VO_ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+        case VO_ACT_GELU_TANH: {                                                             // (1 + tanh u) / 2 = 1 / (1 + e^-2u)
+            const float u = 0.79788456080286536f * (z + 0.044715f * z * z * z);
+            return z / (1.f + expf(-2.f * u));
+        }
+        case VO_ACT_SILU: return z / (1.f + expf(-z));
+        default: return z;
+    }
+}
+
+// N consecutive outputs k.. of row m: bias, activation, residual, one rounding.  N = PER (16 bytes) or any number up to it.
+template <typename T> __device__ __forceinline__ void finish(const LinArgs& a, int64_t m, int k, const float* acc) {
+    constexpr int PER = vo_elem<T>::PER;
+    const T* res = static_cast<const T*>(a.res);
+    T* y = static_cast<T*>(a.y) + m * a.ys + k;
+    float v[PER];
+    const int n = a.K - k < PER ? a.K - k : PER;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) v[j] = activate(acc[j] + (a.bias && j < n ? a.bias[k + j] : 0.f), a.act);
+    if (a.wide_out && n == PER) {
+        if (res) {
+            float r[PER];
+            vo_elem<T>::unpack(*reinterpret_cast<const vo_u32x4*>(res + m * a.rs + k), r);
+#pragma unroll
+            for (int j = 0; j < PER; ++j) v[j] += r[j];
+        }
+        *reinterpret_cast<vo_u32x4*>(y) = vo_elem<T>::pack(v);
+    } else {
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+            if (j < n) vo_elem<T>::put(y + j, v[j] + (res ? vo_elem<T>::get(res + m * a.rs + k + j) : 0.f));
+    }
+}
+
+// A wave's PER consecutive sums: into the workspace or through the epilogue.
+template <typename T> __device__ __forceinline__ void emit(const LinArgs& a, int split, int64_t m, int k, const float* acc) {
+    constexpr int PER = vo_elem<T>::PER;
+    if (a.splits > 1) {
+        float* p = a.part + ((int64_t)split * a.M + m) * a.K + k;
+        if ((a.K & 3) == 0 && k + PER <= a.K) {
+#pragma unroll
+            for (int j = 0; j < PER; j += 4) *reinterpret_cast<float4*>(p + j) = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < PER; ++j)
+                if (k + j < a.K) p[j] = acc[j];
+        }
+    } else {
+        finish<T>(a, m, k, acc);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------ tiles
+// WGM x WGN waves; a wave owns TM rows of x times TN outputs as 16x16 products with W as the first operand, so that a lane
+// holds four consecutive outputs of one row.  LDS rows are 128 bytes (eight chunks); chunk c of row r sits at c ^ (r % 8),
+// which spreads the 16-byte reads of eight rows over all banks.  The permutation is applied to the addresses the lanes
+// fetch, because a load into LDS places lane l's bytes at position l.
+template <typename T, int BM, int BN, int WGM, int WGN, bool DIRECT>
+__global__ __launch_bounds__(64 * WGM * WGN) void linear_tiles(const LinArgs a) {
+    constexpr int PER = vo_elem<T>::PER, BK = 8 * PER, NW = WGM * WGN;
+    constexpr int TM = BM / WGM, TN = BN / WGN, MT = TM / 16, NT = TN / 16;
+    constexpr int ROWS = BM + BN, LOADS = ROWS / 8 / NW;             // 1 KiB wave loads (8 rows) per wave and slab
+    constexpr int STRIP = TN + 4;                                    // floats per row of the store's staging strip
+    constexpr int SLAB = ROWS * 128, STAGE = NW * 16 * STRIP * 4;
+    static_assert(ROWS % (8 * NW) == 0 && BM % (8 * NW) == 0, "a wave's loads must not straddle the operands");
+    __shared__ __align__(16) unsigned char lds[2 * SLAB > STAGE ? 2 * SLAB : STAGE];
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // tile order: splits outermost, then bands of 8 row tiles, within a band column by column
+    const unsigned per_split = a.tiles_m * a.tiles_n;
+    unsigned id = vo_xcd_contiguous(blockIdx.x, per_split * a.splits);
+    const int split = id / per_split;
+    id %= per_split;
+    const unsigned band = id / (8 * a.tiles_n), in_band = id % (8 * a.tiles_n);
+    const unsigned band_rows = a.tiles_m - band * 8 < 8 ? a.tiles_m - band * 8 : 8;
+    const int64_t m0 = (int64_t)(band * 8 + in_band % band_rows) * BM;
+    const int n0 = (int)(in_band / band_rows) * BN;
+    const int c_first = split * a.c_per_split;
+    const int c_last = a.C - c_first < a.c_per_split ? a.C : c_first + a.c_per_split;
+    const int slabs = (c_last - c_first + BK - 1) / BK;
+
+    const int64_t xb = (int64_t)sizeof(T) * a.xs, wb = (int64_t)sizeof(T) * a.C;
+    const int rows_x = (int)(a.M - m0 < BM ? a.M - m0 : BM), rows_w = a.K - n0 < BN ? a.K - n0 : BN;
+    const T* xt = static_cast<const T*>(a.x) + m0 * a.xs;
+    const T* wt = static_cast<const T*>(a.w) + (int64_t)n0 * a.C;
+    const __amdgpu_buffer_rsrc_t xrs = vo_buffer(xt, (rows_x - 1) * xb + wb);
+    const __amdgpu_buffer_rsrc_t wrs = vo_buffer(wt, rows_w * wb);
+
+    const int sub = lane >> 3, chunk = (lane & 7) ^ sub;             // this lane's row of eight and the chunk it fetches
+    auto is_x = [&](int i) { return i < LOADS * BM / ROWS; };        // loads 0.. of a wave fetch x, the rest W
+    auto tile_row = [&](int i) {                                     // first of the eight rows of load i, within its operand
+        constexpr int XL = LOADS * BM / ROWS;
+        return is_x(i) ? (wave * XL + i) * 8 : (wave * (LOADS - XL) + i - XL) * 8;
+    };
+    unsigned off[LOADS];
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+        const int r = tile_row(i) + sub;
+        const bool in = r < (is_x(i) ? rows_x : rows_w);
+        off[i] = in ? (unsigned)(r * (is_x(i) ? xb : wb) + chunk * 16) : VO_OUTSIDE;
+    }
+    vo_u32x4 reg[DIRECT ? 1 : LOADS];
+    auto fetch = [&](int s, unsigned char* buf) {
+        const int c0 = c_first + s * BK;
+        if constexpr (DIRECT) {
+            const bool inside = c0 + chunk * PER < c_last;           // whole chunks: C is a multiple of PER
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i)
+                vo_load_to_lds(is_x(i) ? xrs : wrs, buf + (is_x(i) ? 0 : BM * 128) + tile_row(i) * 128,
+                               inside ? off[i] + c0 * (unsigned)sizeof(T) : VO_OUTSIDE);
+        } else {
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) {
+                const int r = tile_row(i) + sub;
+                const bool in = r < (is_x(i) ? rows_x : rows_w);
+                const int c = c0 + chunk * PER;
+                const T* p = (is_x(i) ? xt + r * a.xs : wt + (int64_t)r * a.C) + c;
+                reg[i] = vo_load_unaligned<T>(p, in ? c_last - c : 0);
+            }
+        }
+    };
+    auto put = [&](unsigned char* buf) {
+        if constexpr (!DIRECT) {
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i)
+                *reinterpret_cast<vo_u32x4*>(buf + (is_x(i) ? 0 : BM * 128) + tile_row(i) * 128 + lane * 16) = reg[i];
+        }
+    };
+
+    const int wm = wave / WGN, wn = wave % WGN;
+    vo_f32x4 acc[NT][MT] = {};
+    const int fr = lane & 15, fg = lane >> 4;
+    auto compute = [&](const unsigned char* buf) {
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            const int pos = ((kk * 4 + fg) ^ (fr & 7)) * 16;
+            vo_u32x4 xf[MT], wf[NT];
+#pragma unroll
+            for (int i = 0; i < NT; ++i) wf[i] = *reinterpret_cast<const vo_u32x4*>(buf + (BM + wn * TN + i * 16 + fr) * 128 + pos);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) xf[i] = *reinterpret_cast<const vo_u32x4*>(buf + (wm * TM + i * 16 + fr) * 128 + pos);
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int j = 0; j < MT; ++j) acc[i][j] = vo_elem<T>::mma16(wf[i], xf[j], acc[i][j]);
+        }
+    };
+
+    if (slabs > 0) {
+        fetch(0, lds);
+        put(lds);
+    }
+    for (int s = 0; s < slabs; ++s) {
+        unsigned char* now = lds + (s & 1) * SLAB;
+        unsigned char* next = lds + (1 - (s & 1)) * SLAB;
+        __syncthreads();                                             // slab s has arrived, slab s - 1 has been read
+        if (s + 1 < slabs) fetch(s + 1, next);
+        compute(now);
+        if (s + 1 < slabs) put(next);
+    }
+    __syncthreads();
+
+    // store: sixteen rows at a time through a strip of LDS of the wave's own, so that rows leave in 16-byte pieces
+    float* strip = reinterpret_cast<float*>(lds) + wave * 16 * STRIP;
+    constexpr int ACROSS = TN / PER;                                 // 16-byte pieces per row
+#pragma unroll
+    for (int j = 0; j < MT; ++j) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i) *reinterpret_cast<vo_f32x4*>(strip + fr * STRIP + i * 16 + fg * 4) = acc[i][j];
+        vo_wave_lds_fence();
+#pragma unroll
+        for (int p = 0; p < 16 * ACROSS / 64; ++p) {
+            const int piece = p * 64 + lane, r = piece / ACROSS, k = piece % ACROSS * PER;
+            const int64_t m = m0 + wm * TM + j * 16 + r;
+            const int kg = n0 + wn * TN + k;
+            if (m < a.M && kg < a.K) {
+                float v[PER];
+#pragma unroll
+                for (int q = 0; q < PER; q += 4) {
+                    const vo_f32x4 t = *reinterpret_cast<const vo_f32x4*>(strip + r * STRIP + k + q);
+                    v[q] = t[0]; v[q + 1] = t[1]; v[q + 2] = t[2]; v[q + 3] = t[3];
+                }
+                emit<T>(a, split, m, kg, v);
+            }
+        }
+        vo_wave_lds_fence();
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------- rows
+// At most 16 * XT rows of x: a workgroup forms 16 * WT outputs for all of them, its eight waves each a part of C; W goes
+// from memory to registers once, the rows of x come from the caches.  The waves' sums are added in LDS in wave order.
+template <typename T, int XT, int WT, bool ALIGNED>
+__global__ __launch_bounds__(512) void linear_rows(const LinArgs a) {
+    constexpr int PER = vo_elem<T>::PER, STEP = 4 * PER, NW = 8;     // one product covers STEP elements of C
+    __shared__ __align__(16) float sums[NW][XT * 16][WT * 16 + 4];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int fr = lane & 15, fg = lane >> 4;
+    const unsigned groups = a.tiles_n;
+    const unsigned id = vo_xcd_contiguous(blockIdx.x, groups * a.splits);
+    const int split = id / groups, n0 = (int)(id % groups) * 16 * WT;
+    const int c_first = split * a.c_per_split;
+    const int c_last = a.C - c_first < a.c_per_split ? a.C : c_first + a.c_per_split;
+    // parts of whole pairs of steps: 128 bytes of a row of W
+    const int part = (((c_last - c_first + 2 * STEP - 1) / (2 * STEP) + NW - 1) / NW) * 2 * STEP;
+    const int c_lo = c_first + wave * part < c_last ? c_first + wave * part : c_last;
+    const int c_hi = c_lo + part < c_last ? c_lo + part : c_last;
+
+    const T* x = static_cast<const T*>(a.x);
+    const T* w = static_cast<const T*>(a.w) + (int64_t)n0 * a.C;
+    const int64_t xb = (int64_t)sizeof(T) * a.xs, wb = (int64_t)sizeof(T) * a.C;
+    const int rows_w = a.K - n0 < 16 * WT ? a.K - n0 : 16 * WT;
+    const __amdgpu_buffer_rsrc_t xrs = vo_buffer(x, (a.M - 1) * xb + wb);
+    const __amdgpu_buffer_rsrc_t wrs = vo_buffer(w, rows_w * wb);
+    unsigned xo[XT], wo[WT];
+#pragma unroll
+    for (int i = 0; i < XT; ++i) xo[i] = i * 16 + fr < a.M ? (unsigned)((i * 16 + fr) * xb) + fg * 16 : VO_OUTSIDE;
+#pragma unroll
+    for (int i = 0; i < WT; ++i) wo[i] = i * 16 + fr < rows_w ? (unsigned)((i * 16 + fr) * wb) + fg * 16 : VO_OUTSIDE;
+
+    auto load_x = [&](int i, int c) -> vo_u32x4 {
+        if constexpr (ALIGNED)
+            return __builtin_amdgcn_raw_buffer_load_b128(xrs, c + fg * PER < c_hi ? xo[i] + c * (unsigned)sizeof(T) : VO_OUTSIDE, 0, 0);
+        else
+            return vo_load_unaligned<T>(x + (i * 16 + fr) * a.xs + c + fg * PER, i * 16 + fr < a.M ? c_hi - c - fg * PER : 0);
+    };
+    auto load_w = [&](int i, int c) -> vo_u32x4 {
+        if constexpr (ALIGNED)
+            return __builtin_amdgcn_raw_buffer_load_b128(wrs, c + fg * PER < c_hi ? wo[i] + c * (unsigned)sizeof(T) : VO_OUTSIDE, 0, 0);
+        else
+            return vo_load_unaligned<T>(w + (int64_t)(i * 16 + fr) * a.C + c + fg * PER, i * 16 + fr < rows_w ? c_hi - c - fg * PER : 0);
+    };
+    vo_f32x4 acc[WT][XT] = {};
+    constexpr int DEPTH = WT == 1 ? 8 : 4;                            // steps in flight
+    for (int c = c_lo; c < c_hi; c += DEPTH * STEP) {
+        vo_u32x4 wf[DEPTH][WT], xf[DEPTH][XT];
+#pragma unroll
+        for (int d = 0; d < DEPTH; ++d) {
+#pragma unroll
+            for (int i = 0; i < WT; ++i) wf[d][i] = load_w(i, c + d * STEP);
+#pragma unroll
+            for (int i = 0; i < XT; ++i) xf[d][i] = load_x(i, c + d * STEP);
+        }
+#pragma unroll
+        for (int d = 0; d < DEPTH; ++d)
+#pragma unroll
+            for (int i = 0; i < WT; ++i)
+#pragma unroll
+                for (int j = 0; j < XT; ++j) acc[i][j] = vo_elem<T>::mma16(wf[d][i], xf[d][j], acc[i][j]);
+    }
+#pragma unroll
+    for (int j = 0; j < XT; ++j)
+#pragma unroll
+        for (int i = 0; i < WT; ++i) *reinterpret_cast<vo_f32x4*>(&sums[wave][j * 16 + fr][i * 16 + fg * 4]) = acc[i][j];
+    __syncthreads();
+    constexpr int ACROSS = WT * 16 / PER;
+    for (int piece = threadIdx.x; piece < XT * 16 * ACROSS; piece += 512) {
+        const int r = piece / ACROSS, k = piece % ACROSS * PER;
+        if (r >= a.M || n0 + k >= a.K) continue;
+        float v[PER] = {};
+#pragma unroll
+        for (int s = 0; s < NW; ++s)
+#pragma unroll
+            for (int q = 0; q < PER; ++q) v[q] += sums[s][r][k + q];
+        emit<T>(a, split, r, n0 + k, v);
+    }
+}
+
+// Adds the partial sums of one PER-wide piece in the order of the splits and finishes it.
+template <typename T> __global__ __launch_bounds__(256) void linear_join(const LinArgs a) {
+    constexpr int PER = vo_elem<T>::PER;
+    const int64_t across = (a.K + PER - 1) / PER, piece = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (piece >= a.M * across) return;
+    const int64_t m = piece / across;
+    const int k = (int)(piece % across) * PER;
+    float v[PER] = {};
+    for (int s = 0; s < a.splits; ++s) {
+        const float* p = a.part + ((int64_t)s * a.M + m) * a.K + k;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) v[j] += k + j < a.K ? p[j] : 0.f;
+    }
+    finish<T>(a, m, k, v);
+}
+
+// ------------------------------------------------------------------------------------------------------------- host
+
+struct Plan {
+    int form;                        // 0: rows, 1: 64x64 tiles, 2: 128x128, 3: 256x256
+    int splits, c_per_split;
+    int64_t tiles_m, tiles_n;
+};
+
+Plan plan(int64_t M, int C, int K, int dtype) {
+    const int per = dtype == VO_F32 ? 4 : 8, slab = 8 * per;
+    Plan p{};
+    if (M <= 64) {
+        p.form = 0;
+        p.tiles_m = 1;
+        p.tiles_n = vo_ceil_div(K, M <= 16 ? 16 : 32);
+    } else {
+        const int64_t big = vo_ceil_div(M, 256) * vo_ceil_div(K, 256), mid = vo_ceil_div(M, 128) * vo_ceil_div(K, 128);
+        p.form = big >= 224 && dtype != VO_F32 ? 3 : mid >= 192 ? 2 : 1;
+        const int t = p.form == 3 ? 256 : p.form == 2 ? 128 : 64;
+        p.tiles_m = vo_ceil_div(M, t);
+        p.tiles_n = vo_ceil_div(K, t);
+    }
+    const int64_t tiles = p.tiles_m * p.tiles_n;
+    int64_t splits = 1;
+    const int64_t at_least = p.form == 0 ? 1024 : 512;               // elements of C worth a split
+    if (tiles < 192) {
+        splits = vo_ceil_div(384, tiles);
+        if (splits > C / at_least) splits = C / at_least;
+        if (splits > 16) splits = 16;
+        if (splits < 1) splits = 1;
+    }
+    p.c_per_split = (int)vo_ceil_div(vo_ceil_div(C, slab), splits) * slab;
+    if (p.c_per_split < slab) p.c_per_split = slab;
+    p.splits = (int)vo_ceil_div(C, p.c_per_split);
+    if (p.splits < 1) p.splits = 1;
+    return p;
+}
+
+template <typename T, bool DIRECT> int launch(const LinArgs& a, const Plan& p, hipStream_t st) {
+    const dim3 grid((unsigned)(p.tiles_m * p.tiles_n * p.splits));
+    if (p.form == 0) {
+        const int xt = (int)vo_ceil_div(a.M, 16);
+        if (xt == 1) linear_rows<T, 1, 1, DIRECT><<<grid, 512, 0, st>>>(a);
+        else if (xt == 2) linear_rows<T, 2, 2, DIRECT><<<grid, 512, 0, st>>>(a);
+        else if (xt == 3) linear_rows<T, 3, 2, DIRECT><<<grid, 512, 0, st>>>(a);
+        else linear_rows<T, 4, 2, DIRECT><<<grid, 512, 0, st>>>(a);
+    } else if (p.form == 1) {
+        linear_tiles<T, 64, 64, 2, 2, DIRECT><<<grid, 256, 0, st>>>(a);
+    } else if (p.form == 2) {
+        linear_tiles<T, 128, 128, 2, 2, DIRECT><<<grid, 256, 0, st>>>(a);
+    } else {
+        if constexpr (sizeof(T) == 2) linear_tiles<T, 256, 256, 2, 4, DIRECT><<<grid, 512, 0, st>>>(a);
+    }
+    VO_CHECK_LAUNCH("vo_linear");
+    if (p.splits > 1) {
+        const int64_t pieces = a.M * vo_ceil_div(a.K, vo_elem<T>::PER);
+        linear_join<T><<<dim3((unsigned)vo_ceil_div(pieces, 256)), 256, 0, st>>>(a);
+        VO_CHECK_LAUNCH("vo_linear (join)");
+    }
+    return VO_OK;
+}
+
+template <typename T> int dispatch(const LinArgs& a, const Plan& p, hipStream_t st) {
+    const size_t es = sizeof(T);
+    const bool direct = (a.C * es) % 16 == 0 && (a.xs * es) % 16 == 0 && reinterpret_cast<uintptr_t>(a.x) % 16 == 0 &&
+                        reinterpret_cast<uintptr_t>(a.w) % 16 == 0;
+    return direct ? launch<T, true>(a, p, st) : launch<T, false>(a, p, st);
+}
+
+}  // namespace
+
+extern "C" int64_t vo_linear_workspace_bytes(int64_t M, int C, int K, int dtype) {
+    if (M <= 0 || C <= 0 || K <= 0) return 0;
+    const Plan p = plan(M, C, K, dtype);
+    return p.splits > 1 ? (int64_t)p.splits * M * K * 4 : 0;
+}
+
+extern "C" int vo_linear(const void* x, int64_t x_row_stride, const void* weight, const float* bias, const void* residual,
+                         int64_t residual_row_stride, void* y, int64_t y_row_stride, int64_t M, int C, int K, int activation,
+                         int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+    VO_REQUIRE(dtype == VO_F32 || dtype == VO_F16 || dtype == VO_BF16, "vo_linear: dtype=%d is none of VO_F32, VO_F16, VO_BF16", dtype);
+    VO_REQUIRE(activation >= VO_ACT_NONE && activation <= VO_ACT_SILU, "vo_linear: unknown activation %d", activation);
+    VO_REQUIRE(M >= 0 && C >= 1 && K >= 1, "vo_linear: M=%lld C=%d K=%d (M >= 0, C >= 1, K >= 1 required)", (long long)M, C, K);
+    if (M == 0) return VO_OK;
+    VO_REQUIRE(x && weight && y, "vo_linear: null pointer");
+    VO_REQUIRE(x_row_stride >= C && y_row_stride >= K && (!residual || residual_row_stride >= K),
+               "vo_linear: row strides must be at least the rows' lengths");
+    const int64_t es = dtype == VO_F32 ? 4 : 2;
+    const Plan p = plan(M, C, K, dtype);
+    // a tile's rows are addressed with 32-bit offsets
+    if (x_row_stride * es * 256 >= (1ll << 31) || (int64_t)C * es * 256 >= (1ll << 31))
+        return vo_fail(VO_ERR_UNSUPPORTED, "vo_linear: rows of x and weight must be under 8 MiB");
+    if (p.tiles_m * p.tiles_n * p.splits >= (1ll << 31) || M * vo_ceil_div(K, 4) >= (1ll << 38))
+        return vo_fail(VO_ERR_UNSUPPORTED, "vo_linear: M=%lld K=%d is too large for one launch", (long long)M, K);
+    const int64_t need = p.splits > 1 ? (int64_t)p.splits * M * K * 4 : 0;
+    VO_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
+               "vo_linear: needs a 16-byte aligned workspace of %lld bytes", (long long)need);
+    LinArgs a{};
+    a.x = x; a.w = weight; a.bias = bias; a.res = residual; a.y = y; a.part = static_cast<float*>(workspace);
+    a.xs = x_row_stride; a.rs = residual_row_stride; a.ys = y_row_stride;
+    a.M = M; a.C = C; a.K = K; a.act = activation;
+    a.splits = p.splits; a.c_per_split = p.c_per_split;
+    a.tiles_m = (unsigned)p.tiles_m; a.tiles_n = (unsigned)p.tiles_n;
+    a.wide_out = reinterpret_cast<uintptr_t>(y) % 16 == 0 && y_row_stride * es % 16 == 0 &&
+                 (!residual || (reinterpret_cast<uintptr_t>(residual) % 16 == 0 && residual_row_stride * es % 16 == 0));
+    hipStream_t st = vo_stream(stream);
+    if (dtype == VO_F32) return dispatch<float>(a, p, st);
+    if (dtype == VO_F16) return dispatch<_Float16>(a, p, st);
+    return dispatch<__bf16>(a, p, st);
+}

@@ -118,7 +118,7 @@ def erode3x3(mask: torch.Tensor) -> torch.Tensor:
     return out
 
 
-VO_F32, VO_F16 = 0, 1        # storage codes of the fused conv-net passes (include/vo_hip.h)
+VO_F32, VO_F16, VO_BF16 = 0, 1, 2        # storage codes (include/vo_hip.h); VO_BF16: the token-major operators only
 
 
 def _act(t: torch.Tensor, name: str, like: torch.Tensor | None = None):
@@ -1084,6 +1084,107 @@ def convex_upsample(flow: torch.Tensor, mask: torch.Tensor, factor: int, out_cha
     out = torch.empty((B, Cout, factor * H, factor * W), device=flow.device, dtype=torch.float32)
     _call("vo_convex_upsample", _dev(flow, "flow", torch.float32), _dev(mask, "mask", torch.float32),
               out.data_ptr(), B, Cf, Cout, H, W, factor, float(mask_scale), _stream())
+    return out
+
+
+# ------------------------------------------------------- token-major operators
+# Rows are tokens (or pixels): (M, C) with C consecutive, as conv1x1_pixel_major writes them.
+
+_TOKEN_DTYPES = {torch.float32: VO_F32, torch.float16: VO_F16, torch.bfloat16: VO_BF16}
+ACTIVATIONS = {None: _lib.VO_ACT_NONE, "relu": _lib.VO_ACT_RELU, "gelu": _lib.VO_ACT_GELU,
+               "gelu_tanh": _lib.VO_ACT_GELU_TANH, "silu": _lib.VO_ACT_SILU}
+
+
+def _token_tensor(t, name: str, like: torch.Tensor | None = None) -> torch.Tensor:
+    """A GPU tensor of a token-major type (of ``like``'s type and device)."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise ValueError(f"{name}: expected a GPU tensor (the HIP backend has no CPU path)")
+    if t.dtype not in _TOKEN_DTYPES:
+        raise ValueError(f"{name}: expected float32, float16 or bfloat16, got {t.dtype}")
+    if like is not None and t.dtype != like.dtype:
+        raise ValueError(f"{name}: dtype {t.dtype} differs from {like.dtype}")
+    if like is not None and t.device != like.device:
+        raise ValueError(f"{name}: on {t.device}, the other tensors on {like.device}")
+    return t
+
+
+def _rows(t: torch.Tensor, name: str, width: int):
+    """(..., width) whose leading axes collapse to rows one stride apart -> (ptr, rows, row stride in elements)."""
+    if t.dim() < 1 or t.shape[-1] != width:
+        raise ValueError(f"{name}: expected rows of {width}, got shape {tuple(t.shape)}")
+    m = t.numel() // width
+    if m <= 1:
+        stride = width
+    else:
+        try:
+            flat = t.view(m, width)
+        except RuntimeError:
+            raise ValueError(f"{name}: the leading axes do not collapse to evenly spaced rows (strides {t.stride()})") from None
+        stride = flat.stride(0)
+    if width > 1 and m > 0 and t.stride(-1) != 1:
+        raise ValueError(f"{name}: a row's elements must be consecutive (got strides {t.stride()})")
+    if m > 1 and stride < width:
+        raise ValueError(f"{name}: rows overlap (got strides {t.stride()})")
+    return t.data_ptr(), m, stride
+
+
+def _span(t: torch.Tensor):
+    """First and one-past-last byte a tensor's elements reach."""
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _no_overlap(out: torch.Tensor, t: torch.Tensor | None, name: str) -> None:
+    if t is None or t.numel() == 0 or out.numel() == 0:
+        return
+    (a, b), (c, d) = _span(out), _span(t)
+    if a < d and c < b:
+        raise ValueError(f"out overlaps {name} in memory")
+
+
+def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, activation: str | None = None,
+           residual: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """act(x W^T + bias) + residual for rows x (..., C) and weight (K, C) -> (..., K).
+
+    x, weight, residual and out are float32, float16 or bfloat16 alike, bias (K) is float32; products, sums and the
+    epilogue are float32 with one rounding at the store.  ``activation``: None, "relu", "gelu" (the error function's form),
+    "gelu_tanh" or "silu"; it comes before the residual is added.  Rows of x, residual and out may lie any distance apart
+    (slices of wider tensors), a row's elements are consecutive; weight is contiguous.  ``out`` may be the residual itself;
+    it must not overlap anything else.  Sums are formed in a fixed order: equal inputs give equal bits."""
+    _token_tensor(x, "x")
+    _token_tensor(weight, "weight", x)
+    if weight.dim() != 2 or not weight.is_contiguous() or weight.shape[0] < 1 or weight.shape[1] < 1:
+        raise ValueError("weight must be a contiguous (K,C)")
+    K, C = weight.shape
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation must be one of {list(ACTIVATIONS)}, got {activation!r}")
+    if bias is not None and (bias.numel() != K or bias.device != x.device):
+        raise ValueError("bias must have one entry per output, on x's device")
+    px, M, xs = _rows(x, "x", C)
+    shape = tuple(x.shape[:-1]) + (K,)
+    pr = rs = 0
+    if residual is not None:
+        if tuple(_token_tensor(residual, "residual", x).shape) != shape:
+            raise ValueError(f"residual must be {shape}, got {tuple(residual.shape)}")
+        pr, _, rs = _rows(residual, "residual", K)
+    if out is None:
+        out = torch.empty(shape, device=x.device, dtype=x.dtype)
+        py, ys = out.data_ptr(), K
+    else:
+        if tuple(_token_tensor(out, "out", x).shape) != shape:
+            raise ValueError(f"out must be {shape}, got {tuple(out.shape)}")
+        py, _, ys = _rows(out, "out", K)
+        for t, name in ((x, "x"), (weight, "weight"), (bias, "bias")):
+            _no_overlap(out, t, name)
+        if residual is not None and (py, ys) != (pr, rs):
+            _no_overlap(out, residual, "residual (other than as the same tensor)")
+    dt, es = _TOKEN_DTYPES[x.dtype], x.element_size()
+    with torch.cuda.device(x.device):
+        need = int(_lib.load().vo_linear_workspace_bytes(M, C, K, dt))
+        work = torch.empty((need,), device=x.device, dtype=torch.uint8) if need else None
+        _call("vo_linear", px, xs, weight.data_ptr(), _opt(bias, "bias", torch.float32), pr, rs, py, ys, M, C, K,
+              ACTIVATIONS[activation], dt, 0 if work is None else work.data_ptr(), need, _stream(),
+              nbytes=es * (M * C + K * C + M * K * (1 + (residual is not None))), flops=2 * M * C * K)
     return out
 
 
