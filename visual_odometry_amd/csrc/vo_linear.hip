@@ -190,15 +190,21 @@ __global__ __launch_bounds__(64 * WGM * WGN) void linear_tiles(const LinArgs a) 
     }
     __syncthreads();
 
-    // store: sixteen rows at a time through a strip of LDS of the wave's own, so that rows leave in 16-byte pieces
+    // store: sixteen rows at a time through a strip of LDS of the wave's own, so that rows leave in 16-byte pieces.  The
+    // loop stays rolled (the epilogue's code is long) and the sums move down one place per round, because a register
+    // array with a running index would live in memory.
     float* strip = reinterpret_cast<float*>(lds) + wave * 16 * STRIP;
     constexpr int ACROSS = TN / PER;                                 // 16-byte pieces per row
-#pragma unroll
+#pragma unroll 1
     for (int j = 0; j < MT; ++j) {
 #pragma unroll
-        for (int i = 0; i < NT; ++i) *reinterpret_cast<vo_f32x4*>(strip + fr * STRIP + i * 16 + fg * 4) = acc[i][j];
-        vo_wave_lds_fence();
+        for (int i = 0; i < NT; ++i) *reinterpret_cast<vo_f32x4*>(strip + fr * STRIP + i * 16 + fg * 4) = acc[i][0];
 #pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int q = 0; q + 1 < MT; ++q) acc[i][q] = acc[i][q + 1];
+        vo_wave_lds_fence();
+#pragma unroll 1
         for (int p = 0; p < 16 * ACROSS / 64; ++p) {
             const int piece = p * 64 + lane, r = piece / ACROSS, k = piece % ACROSS * PER;
             const int64_t m = m0 + wm * TM + j * 16 + r;
