@@ -633,6 +633,37 @@ int vo_linear(const void* x, int64_t x_row_stride, const void* weight, const flo
               int64_t M, int C, int K, int activation, int dtype,
               void* workspace, int64_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Attention of packed sequences: row i of a sequence gives
+ *     out[i,h,:] = sum_j p_ij v[j,h',:],   p_ij = softmax_j(scale * q[i,h,:] . k[j,h',:]),   h' = h / (q_heads / k_heads)
+ * over the keys j of its sequence; with causal != 0 over those with j <= i + Lk - Lq (Lq, Lk the sequence's rows and keys:
+ * its last row sees every key).  A row that sees no key gives zeros.  It has NO counterpart in the reference; it is the
+ * all-pairs product of vo_corr_volume_1d / _2d without the volume: along the epipolar lines of a stereo pair (one sequence
+ * a line, causal: a match lies never right of its pixel), among all pixels of a frame, over packed prompts of any lengths,
+ * or for one new token over a long cache.
+ *   q, out (q_tokens, q_heads, D), k, v (k_tokens, k_heads, D): D consecutive elements per token and head, token and head
+ *   strides in ELEMENTS, so slices of one fused projection are fine.  Storage VO_F32, VO_F16 or VO_BF16; products, softmax
+ *   and sums in float32; with 16-bit storage the exponentials are rounded to it (relative to the row's largest) before they
+ *   meet v, and the result is rounded once.  D at most 256; D, strides and pointers whole 16-byte pieces, strides under
+ *   16 MiB (VO_ERR_UNSUPPORTED otherwise).  out overlaps none of the inputs.
+ *   q_offsets, k_offsets: device arrays of sequences + 1 ascending int32: sequence s owns the rows [q_offsets[s],
+ *   q_offsets[s+1]) and the keys [k_offsets[s], k_offsets[s+1]), any length from 0; or both NULL with sequences = 1: all
+ *   rows and keys.  Rows outside every sequence are left as they were.  The offsets are read on the device and clamped to
+ *   the tensors; results for offsets that do not ascend are unspecified.
+ *   A key or value that no row of its sequence sees does not matter whatever it holds; a value (v) that is not finite may
+ *   reach rows of its sequence that do not see it, as a product with a weight of zero.
+ * workspace: vo_attention_workspace_bytes(...) bytes (often 0), 16-byte aligned, contents irrelevant.  Calls that share one
+ * must be ordered on one stream; two captured graphs that may replay at once need one each.
+ * ------------------------------------------------------------------------- */
+int64_t vo_attention_workspace_bytes(int64_t q_tokens, int64_t k_tokens, int sequences, int q_heads, int k_heads, int D);
+int vo_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                 const void* k, int64_t k_token_stride, int64_t k_head_stride,
+                 const void* v, int64_t v_token_stride, int64_t v_head_stride,
+                 void* out, int64_t out_token_stride, int64_t out_head_stride,
+                 const int32_t* q_offsets, const int32_t* k_offsets, int sequences,
+                 int64_t q_tokens, int64_t k_tokens, int q_heads, int k_heads, int D, float scale, int causal, int dtype,
+                 void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

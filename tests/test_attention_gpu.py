@@ -1,0 +1,298 @@
+"""ops.attention against the definition in float64, element by element.
+
+Tolerance, derived.  With A = sum_j p_j |v_j| (p the exact weights):
+  * a score is off by at most 2 (D+2) 2^-24 scale sum |q||k| (any order, doubled for truncating additions inside the matrix
+    instruction), the exponent's argument by a few more roundings of |s| and |m|, the exponential by 2^-21 of itself: the
+    weight's relative error eta, which enters the numerator and the denominator once each;
+  * with 16-bit storage the weight is rounded once, by eps / 2 of itself (float16: by 2^-25 at least, of weights whose
+    largest is at least 1, so 2^-25 sum |v| / l more, l >= 1);
+  * the two sums over n keys are float32: 2 (n + 64) 2^-24 of A each, and one rescaling per key tile;
+  * the store rounds once, by eps / 2 of the value."""
+import numpy as np
+import pytest
+import torch
+
+from visual_odometry_amd import ops
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.float32, torch.float16, torch.bfloat16]
+U32 = 2.0 ** -24
+
+
+def reference(q, k, v, q_len, k_len, causal, scale):
+    """(out, tolerance) in float64 for packed sequences."""
+    dt, D, Hq, Hk = q.dtype, q.shape[2], q.shape[1], k.shape[1]
+    half = torch.finfo(dt).eps / 2
+    out = torch.zeros(sum(q_len), Hq, D, device=q.device, dtype=torch.float64)
+    tol = torch.zeros_like(out)
+    a = b = 0
+    for lq, lk in zip(q_len, k_len):
+        for h in range(Hq):
+            if lq == 0 or lk == 0:
+                continue
+            Q, K, V = q[a:a + lq, h].double(), k[b:b + lk, h // (Hq // Hk)].double(), v[b:b + lk, h // (Hq // Hk)].double()
+            S = Q @ K.t().contiguous() * scale
+            B = Q.abs() @ K.abs().t().contiguous() * scale
+            see = torch.ones(lq, lk, device=q.device, dtype=torch.bool)
+            if causal:
+                see = see.tril(lk - lq)
+            S = S.masked_fill(~see, -torch.inf)
+            some = see.any(1)
+            m = torch.where(some, S.amax(1), torch.zeros_like(S[:, 0]))
+            e = torch.exp(S - m[:, None])
+            l = e.sum(1)
+            p = e / torch.where(some, l, torch.ones_like(l))[:, None]
+            o, A = p @ V, p @ V.abs()
+            x = 2 * (D + 2) * U32 * B + 4 * U32 * (torch.where(see, S, torch.zeros_like(S)).abs() + m.abs()[:, None] + 8)
+            eta = (torch.where(see, torch.expm1(x), torch.zeros_like(x)).amax(1) + 2.0 ** -21)[:, None]
+            rnd = 0.0 if dt == torch.float32 else half
+            t = A * (2 * eta + rnd + 4 * (lk + 64) * U32) * 1.05
+            if dt == torch.float16:
+                t = t + 2.0 ** -25 * (see.double() @ V.abs()) / torch.where(some, l, torch.ones_like(l))[:, None]
+            t = t + half * (o.abs() + t) + {torch.float32: 2.0 ** -120, torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -120}.get(dt, 0.0)
+            out[a:a + lq, h], tol[a:a + lq, h] = o, t
+        a, b = a + lq, b + lk
+    return out, tol
+
+
+def offsets(lengths, first=0):
+    return torch.tensor(np.concatenate([[first], first + np.cumsum(lengths)]).astype(np.int32)).cuda()
+
+
+def make(q_len, k_len, Hq, Hk, D, dtype, seed, spread=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    n = lambda *s: torch.randn(*s, generator=g, device="cuda")
+    return ((n(sum(q_len), Hq, D) * spread).to(dtype), n(sum(k_len), Hk, D).to(dtype), n(sum(k_len), Hk, D).to(dtype))
+
+
+def check(y, want, tol):
+    assert y.shape == want.shape
+    err = (y.double() - want).abs()
+    assert bool((err <= tol).all()), f"error {(err / tol).nan_to_num(0).max().item():.3g} times the bound"
+
+
+def run(q_len, k_len, Hq, Hk, D, dtype, causal, seed=0, scale=None, spread=1.0):
+    q, k, v = make(q_len, k_len, Hq, Hk, D, dtype, seed, spread)
+    y = ops.attention(q, k, v, offsets(q_len), offsets(k_len), causal=causal, scale=scale)
+    assert y.dtype == dtype
+    check(y, *reference(q, k, v, q_len, k_len, causal, D ** -0.5 if scale is None else scale))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("D", [8, 16, 24, 32, 40, 64, 72, 96, 128, 200, 256])
+@pytest.mark.parametrize("form", ["tiles", "rows"])
+def test_head_sizes(vo, dtype, causal, D, form):
+    if form == "tiles":
+        run([130, 1, 0, 67], [130, 1, 5, 200], 4, 2, D, dtype, causal, D)
+    else:
+        run([1, 3, 0, 1], [70, 140, 5, 1], 4, 2, D, dtype, causal, D)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("q_len,k_len", [
+    ([1], [1]), ([1], [31]), ([1], [32]), ([1], [33]), ([2], [64]), ([5], [65]), ([33], [127]), ([127], [128]), ([128], [128]), ([129], [129]),
+    ([255], [257]), ([300], [64]), ([64], [0]), ([0], [64]), ([0, 0, 7], [3, 0, 9]),
+    ([40, 0, 1, 128, 3], [20, 7, 0, 100, 5]),                          # more rows than keys: causal leaves rows empty
+    ([160] * 12, [160] * 12), ([1] * 50, list(range(50))), ([513, 2, 90], [700, 1000, 90])])
+@pytest.mark.parametrize("Hq,Hk", [(3, 3), (8, 2)])
+def test_lengths(vo, dtype, causal, q_len, k_len, Hq, Hk):
+    run(q_len, k_len, Hq, Hk, 64, dtype, causal, len(q_len) + sum(q_len))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("Hq,Hk", [(1, 1), (7, 1), (32, 8), (40, 1), (6, 3)])
+@pytest.mark.parametrize("q_len,k_len", [([1, 1, 1], [700, 3, 90]), ([4, 2, 7], [300, 2, 50]), ([150], [150])])
+def test_groups_of_heads(vo, dtype, Hq, Hk, q_len, k_len):
+    run(q_len, k_len, Hq, Hk, 32, dtype, True, Hq)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("q_len,k_len,Hq,Hk,D", [
+    ([1], [5003], 4, 1, 128), ([1, 2, 1], [4000, 1, 9001], 8, 2, 64), ([3], [2500], 2, 1, 256),       # rows, split over the keys
+    ([100], [6007], 2, 1, 64), ([40, 70], [3000, 2500], 2, 2, 128), ([129], [1500], 1, 1, 256)])      # tiles, split over the keys
+def test_long_axes_are_split_and_joined(vo, dtype, causal, q_len, k_len, Hq, Hk, D):
+    from visual_odometry_amd import _lib
+    assert _lib.load().vo_attention_workspace_bytes(sum(q_len), sum(k_len), len(q_len), Hq, Hk, D) > 0
+    run(q_len, k_len, Hq, Hk, D, dtype, causal, 5)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("q_len,k_len", [([140], [300]), ([2], [300]), ([1], [4000])])
+def test_large_scores_and_other_scales(vo, dtype, q_len, k_len):
+    """Scores of some hundreds: the maximum moves from tile to tile and nearly all weight lies on a few keys."""
+    run(q_len, k_len, 2, 2, 64, dtype, False, 3, spread=12.0)
+    run(q_len, k_len, 2, 2, 64, dtype, True, 4, scale=0.01)
+    run(q_len, k_len, 2, 2, 64, dtype, True, 4, scale=3.0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("q_len", [[130], [2]])
+def test_rising_and_falling_scores(vo, dtype, q_len):
+    """Keys whose scores rise by a little less or more than the rescaling threshold from tile to tile, or only fall."""
+    n, D = 640, 32
+    for slope in (0.02, 0.05, 0.1, 0.5, -0.1):
+        q, k, v = make(q_len, [n], 1, 1, D, dtype, 9)
+        q = torch.zeros_like(q); q[..., 0] = 1
+        k = k * 0.01; k[:, 0, 0] = (torch.arange(n, device="cuda") * slope - 20).to(dtype)
+        y = ops.attention(q, k, v, scale=1.0)
+        check(y, *reference(q, k, v, q_len, [n], False, 1.0))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("lens", [[150, 33, 0, 260], [1, 2, 1]])
+def test_slices_of_one_projection_and_a_strided_result(vo, dtype, causal, lens):
+    Hq, Hk, D = 4, 2, 64
+    g = torch.Generator(device="cuda").manual_seed(2)
+    qkv = torch.randn(sum(lens), (Hq + 2 * Hk + 1) * D, generator=g, device="cuda").to(dtype).view(sum(lens), -1, D)
+    q, k, v = qkv[:, :Hq], qkv[:, Hq:Hq + Hk], qkv[:, Hq + Hk:Hq + 2 * Hk]
+    hold = torch.full((sum(lens), 2 * Hq, 2 * D), 7.0, device="cuda", dtype=dtype)
+    out = hold[:, ::2, D:]
+    y = ops.attention(q, k, v, offsets(lens), causal=causal, out=out)
+    assert y is out
+    check(out, *reference(q, k, v, lens, lens, causal, D ** -0.5))
+    y = y.clone()
+    hold[:, ::2, D:] = 7
+    assert bool((hold == 7).all())
+    # heads ahead of tokens in memory
+    qt, kt, vt = (t.transpose(0, 1).contiguous().transpose(0, 1) for t in (q, k, v))
+    assert torch.equal(ops.attention(qt, kt, vt, offsets(lens), causal=causal), y)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("q_len,k_len", [([140, 3, 60], [200, 70, 60]), ([1, 2, 1], [77, 5, 130]), ([1, 1], [2500, 1300])])
+def test_what_lies_outside_every_sequence_neither_matters_nor_changes(vo, dtype, causal, q_len, k_len):
+    """Rows and keys ahead of the first and behind the last sequence (a padded batch, a cache's unused end) are NaN."""
+    lead, behind, D = 5, 140, 64
+    q, k, v = make(q_len, k_len, 4, 2, D, dtype, 8)
+    pad = lambda t: torch.nn.functional.pad(t.transpose(0, 2), (lead, behind), value=float("nan")).transpose(0, 2).contiguous()
+    out = torch.full((lead + sum(q_len) + behind, 4, D), 7.0, device="cuda", dtype=dtype)
+    ops.attention(pad(q), pad(k), pad(v), offsets(q_len, lead), offsets(k_len, lead), causal=causal, out=out)
+    check(out[lead:lead + sum(q_len)], *reference(q, k, v, q_len, k_len, causal, D ** -0.5))
+    assert bool((out[:lead] == 7).all()) and bool((out[lead + sum(q_len):] == 7).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("q_len,k_len", [([140, 3], [200, 70]), ([1, 2], [77, 50])])
+def test_sequences_do_not_disturb_each_other(vo, dtype, q_len, k_len):
+    """NaN and infinity in one sequence stay in it, whatever shares its tiles of memory."""
+    q, k, v = make(q_len, k_len, 2, 1, 64, dtype, 6)
+    k[k_len[0] - 1] = float("inf"); v[k_len[0] - 2] = float("nan")
+    y = ops.attention(q, k, v, offsets(q_len), offsets(k_len))
+    assert bool(y[:q_len[0]].isnan().all())
+    want, tol = reference(q[q_len[0]:], k[k_len[0]:], v[k_len[0]:], q_len[1:], k_len[1:], False, 0.125)
+    check(y[q_len[0]:], want, tol)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_without_offsets_everything_is_one_sequence(vo, dtype):
+    q, k, v = make([200], [333], 4, 4, 64, dtype, 1)
+    assert torch.equal(ops.attention(q, k, v, causal=True), ops.attention(q, k, v, offsets([200]), offsets([333]), causal=True))
+    assert tuple(ops.attention(q[:0], k, v).shape) == (0, 4, 64)
+    assert bool((ops.attention(q, k[:0], v[:0]) == 0).all())
+
+
+@pytest.mark.parametrize("q_len,k_len", [([200, 40], [200, 40]), ([1, 1], [3000, 40]), ([60], [3000])])
+def test_equal_bits_on_another_stream_and_in_a_graph(vo, q_len, k_len):
+    q, k, v = make(q_len, k_len, 4, 2, 64, torch.bfloat16, 1)
+    qo, ko = offsets(q_len), offsets(k_len)
+    want = ops.attention(q, k, v, qo, ko, causal=True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ys = [ops.attention(q, k, v, qo, ko, causal=True) for _ in range(3)]
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(y, want) for y in ys)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = ops.attention(q, k, v, qo, ko, causal=True)
+    for seed in range(4):                                            # new values and new lengths in the same buffers
+        for t, n in zip((q, k, v), make(q_len, k_len, 4, 2, 64, torch.bfloat16, 20 + seed)):
+            t.copy_(n)
+        if len(k_len) > 1:
+            ko.copy_(offsets([k_len[0] - seed * 17, k_len[1] + seed * 17]))
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, ops.attention(q, k, v, qo, ko, causal=True))
+
+
+def test_a_long_cache_passes_32_bit_offsets(vo):
+    """Keys and values more than 2^31 elements (and 2^32 bytes) apart: a cache of 70000 tokens at a stride of 32768."""
+    n, D, stride = 70000, 64, 32768
+    hold = torch.zeros(n * stride, device="cuda", dtype=torch.float16)
+    kv = hold.view(n, stride // D, D)[:, :2]
+    g = torch.Generator(device="cuda").manual_seed(3)
+    kv.copy_(torch.randn(n, 2, D, generator=g, device="cuda"))
+    for lq in (1, 130):
+        q = torch.randn(lq, 1, D, generator=g, device="cuda").half()
+        y = ops.attention(q, kv[:, :1], kv[:, 1:], causal=True)
+        check(y, *reference(q, kv[:, :1], kv[:, 1:], [lq], [n], True, D ** -0.5))
+
+
+def test_a_block_of_projections_around_attention(vo):
+    """As they are used together: fused projection, attention on its slices, projection back onto the residual, perceptron."""
+    lens, Hq, Hk, D, W = [160, 33, 160, 7], 4, 2, 64, 256
+    T = sum(lens)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    n = lambda *s: torch.randn(*s, generator=g, device="cuda")
+    for dtype, tol in ((torch.float32, 2e-5), (torch.float16, 2e-2), (torch.bfloat16, 1.5e-1)):
+        x = n(T, W).to(dtype)
+        ws = [(n(o, i) * i ** -0.5).to(dtype) for o, i in (((Hq + 2 * Hk) * D, W), (W, Hq * D), (4 * W, W), (W, 4 * W))]
+        bs = [n(w.shape[0]) * 0.1 for w in ws]
+        off = offsets(lens)
+        qkv = ops.linear(x, ws[0], bs[0]).view(T, -1, D)
+        att = ops.attention(qkv[:, :Hq], qkv[:, Hq:Hq + Hk], qkv[:, Hq + Hk:], off, causal=True)
+        h = ops.linear(att.view(T, Hq * D), ws[1], bs[1], residual=x)
+        y = ops.linear(ops.linear(h, ws[2], bs[2], activation="gelu"), ws[3], bs[3], residual=h)
+        X, Ws, Bs = x.double(), [w.double() for w in ws], [b.double() for b in bs]
+        QKV = (X @ Ws[0].t().contiguous() + Bs[0]).view(T, -1, D)
+        A, _ = reference(QKV[:, :Hq], QKV[:, Hq:Hq + Hk], QKV[:, Hq + Hk:], lens, lens, True, D ** -0.5)
+        Hh = X + A.reshape(T, -1) @ Ws[1].t().contiguous() + Bs[1]
+        z = Hh @ Ws[2].t().contiguous() + Bs[2]
+        Y = Hh + (z * torch.special.ndtr(z)) @ Ws[3].t().contiguous() + Bs[3]
+        # values of size 1 to 5 through four roundings of 2^-24 / 2^-11 / 2^-8 whose errors add up over sums of 256 and 1024
+        # terms: some 30 roundings' worth is the largest a correct chain reaches
+        assert float((y.double() - Y).abs().max()) < tol
+
+
+def test_refusals(vo):
+    q, k, v = make([8], [8], 4, 2, 32, torch.float16, 1)
+    o = offsets([8])
+    bad = [
+        (lambda: ops.attention(q.double(), k, v), "float32, float16 or bfloat16"),
+        (lambda: ops.attention(q, k.float(), v), "dtype"),
+        (lambda: ops.attention(q, k, v.cpu()), "GPU tensor"),
+        (lambda: ops.attention(q[0], k, v), "tokens, heads"),
+        (lambda: ops.attention(q, k, v[:4]), "k and v"),
+        (lambda: ops.attention(q, k[..., :16], v[..., :16]), "k and v"),
+        (lambda: ops.attention(q[:, :3], k, v), "multiple"),
+        (lambda: ops.attention(q, k, v, None, o), "needs q_offsets"),
+        (lambda: ops.attention(q[:4], k, v, o), "as many tokens"),
+        (lambda: ops.attention(q, k, v, o.long()), "int32"),
+        (lambda: ops.attention(q, k, v, o, offsets([4, 4])), "as many"),
+        (lambda: ops.attention(q, k, v, o[:1]), "sequences"),
+        (lambda: ops.attention(q, k, v, o.cpu()), "GPU tensor"),
+        (lambda: ops.attention(q, k, v, scale=0.0), "scale"),
+        (lambda: ops.attention(q, k, v, scale=float("nan")), "scale"),
+        (lambda: ops.attention(q, k, v, out=q), "overlaps q"),
+        (lambda: ops.attention(q, k, v, out=q[:4]), "out must be"),
+        (lambda: ops.attention(q, k, v, out=torch.empty_like(q[:1]).expand(8, 4, 32)), "overlap"),
+        (lambda: ops.attention(q.transpose(1, 2).contiguous().transpose(1, 2), k, v), "consecutive"),
+    ]
+    for call, text in bad:
+        with pytest.raises(ValueError, match=text):
+            call()
+    from visual_odometry_amd._lib import VoHipError
+    with pytest.raises(VoHipError, match="16-byte pieces"):
+        ops.attention(q[..., :20], k[..., :20], v[..., :20])
+    with pytest.raises(VoHipError, match="aligned"):
+        ops.attention(q[..., 4:28], k[..., 4:28], v[..., 4:28])
+    w = torch.zeros(8, 4, 300, device="cuda", dtype=torch.float16)
+    with pytest.raises(VoHipError, match="at most 256"):
+        ops.attention(w, w, w)

@@ -90,10 +90,12 @@ SIGNATURES = {
     "vo_pair_poses_static": [_P, _L, _P, _P, _P, _P, _D, _D, _D, _P, _I, _P, _P, _I, _I, _I, _I, _P],
     "vo_ransac_kabsch_batch": [_P, _P, _P, _D, _I, c_uint64, _P, _P, _P, _I, _I, _L, _P],
     "vo_linear": [_P, _L, _P, _P, _P, _L, _P, _L, _L, _I, _I, _I, _I, _P, _L, _P],
+    "vo_attention": [_P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _P, _I, _L, _L, _I, _I, _I, _F, _I, _I, _P, _L, _P],
 }
 # entry points that return a size instead of a status
 SIZE_QUERIES = {"vo_pair_poses_workspace_bytes": [_I, _I],
-                "vo_linear_workspace_bytes": [_L, _I, _I, _I]}
+                "vo_linear_workspace_bytes": [_L, _I, _I, _I],
+                "vo_attention_workspace_bytes": [_L, _L, _I, _I, _I, _I]}
 EXPORTS = sorted(list(SIGNATURES) + list(SIZE_QUERIES) + ["vo_version", "vo_last_error"])
 
 _lib = None

@@ -1,0 +1,544 @@
+// Attention of packed sequences: o_i = sum_j softmax_j(scale q_i . k_j) v_j over the keys a row sees.
+//   q, out (Tq,Hq,D), k, v (Tk,Hk,D) in float32, float16 or bfloat16; head h reads key head h / (Hq/Hk); sequence s owns
+//   the rows [q_offsets[s], q_offsets[s+1]) and the keys [k_offsets[s], k_offsets[s+1]); causal: row i of Lq sees the
+//   keys j <= i + Lk - Lq.  A row that sees nothing gives 0.
+//
+// One pass over the keys with a running maximum m and sum l per row.  Both products run on the matrix cores, transposed:
+//   S^T = K Q^T   lane l holds column q = l % 32 and the keys 8 b + 4 (l / 32) + i of a block of 32 (b, i = 0..3)
+//   O^T = V^T P^T wants column q = l % 32 and, from lane half l / 32, half of the keys of each step: whichever half of the
+//                 keys that is, the sum over keys is the same as long as V^T is read in the same order.  So the exponentials
+//                 are already where the second product needs them: they are rounded to the 16-bit type in place (float32: not
+//                 at all) and no value crosses lanes.  m, l and the rescaling factor are one number per lane.
+// V^T in 16 bits comes out of LDS by the transposing read: four keys of one feature per lane.
+//
+// The exponent's argument is (s - m) * scale * log2(e), formed in one fused multiply-add; m follows the true maximum only
+// when it has grown by more than 2^8 in the exponentials, so most tiles need no rescaling of the sums (the exponentials are
+// then at most 256, which costs no bits in a floating-point format).
+//
+// Two forms:
+//   tiles  a workgroup of four waves takes 128 rows of one head; key tiles are shared in LDS, loaded while the previous
+//          tile is multiplied
+//   rows   few rows per sequence (single tokens above all): the rows of all heads that share a key head are one tile of 32,
+//          every wave streams key tiles of its own into its own part of LDS, the waves' results are joined at the end
+// Either can be split over the keys; the parts (m, l, unnormalised sums) go to a workspace and are joined in a fixed order.
+#include "vo_packed.h"
+#include "vo_tokens.h"
+
+namespace {
+
+constexpr float LOG2E = 1.44269504088896341f;
+
+struct AttArgs {
+    const void* q;
+    const void* k;
+    const void* v;
+    void* out;
+    float* part;                                  // splits > 1: sums (splits, Tq, Hq, D), then m and l (splits, Tq, Hq, 2)
+    const int* q_off;
+    const int* k_off;
+    int64_t qs, qh, ks, kh, vs, vh, os, oh;       // token and head strides in elements
+    int64_t Tq, Tk;
+    int sequences, Hq, Hk, group, D, causal, splits;
+    unsigned tiles;                               // row tiles over all sequences (an upper bound)
+    float c;                                      // scale * log2(e)
+};
+
+// Key tiles in LDS: rows of DT elements in 16-byte chunks, chunk c of row r at c ^ swizzle(r).  K is read 16 rows of one
+// chunk at a time, V (16 bits) four rows of 64 bytes, V (float32) two rows of 128 bytes four rows apart: each permutation
+// spreads its reader's bytes over all 64 banks.
+template <typename T, int DT> struct Tile {
+    static constexpr int ES = sizeof(T), PER = vo_elem<T>::PER, CH = DT / PER, ROW = DT * ES;
+    static constexpr int PER_LINE = ROW >= 256 ? 1 : 256 / ROW;      // rows in 256 bytes
+    static constexpr int KMASK = CH < 16 ? CH - 1 : 15;
+    static __device__ __forceinline__ int k_swz(int r) { return (r / PER_LINE) & KMASK; }
+    static __device__ __forceinline__ int v_swz(int r) {
+        if constexpr (ES == 4) return CH > 8 ? ((r >> 2) & 1) << 3 : 0;
+        return CH <= 4 ? 0 : CH == 8 ? ((r >> 1) & 1) << 2 : (r & 3) << 2;
+    }
+};
+
+// 32 rows of one wave against key tiles.
+template <typename T, int DT, int KEYS> struct Core {
+    using E = vo_elem<T>;
+    using L = Tile<T, DT>;
+    static constexpr int QS = DT / (2 * E::PER), KB = KEYS / 32, DB = DT / 32;
+    vo_u32x4 q[QS];
+    vo_f32x16 o[DB];
+    float m, l;                                   // m: the maximum of the scores s = q.k (not scaled) that the sums refer to
+
+    __device__ __forceinline__ void reset() {
+#pragma unroll
+        for (int i = 0; i < DB; ++i)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) o[i][j] = 0.f;
+        m = -INFINITY;
+        l = 0.f;
+    }
+    // p: this lane's row (null: no row), chunks of D elements
+    __device__ __forceinline__ void load_q(const T* p, int D, int lane) {
+#pragma unroll
+        for (int s = 0; s < QS; ++s) {
+            const int c = s * 2 + (lane >> 5);
+            q[s] = p && c * E::PER < D ? *reinterpret_cast<const vo_u32x4*>(p + c * E::PER) : vo_u32x4{0, 0, 0, 0};
+        }
+    }
+    // One tile; `limit`: the lane's row sees the tile's keys below it (used when masked)
+    __device__ __forceinline__ void step(const unsigned char* kt, const unsigned char* vt, float c, bool masked, int limit, int lane) {
+        const int col = lane & 31, half = lane >> 5;
+        vo_f32x16 s[KB];
+#pragma unroll
+        for (int b = 0; b < KB; ++b) {
+            const int r = b * 32 + col;
+            vo_f32x16 acc = {};
+#pragma unroll
+            for (int i = 0; i < QS; ++i) {
+                const vo_u32x4 kf = *reinterpret_cast<const vo_u32x4*>(kt + r * L::ROW + (((i * 2 + half) ^ L::k_swz(r)) * 16));
+                acc = E::mma32(kf, q[i], acc);
+            }
+            s[b] = acc;
+        }
+        if (masked) {
+#pragma unroll
+            for (int b = 0; b < KB; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (b * 32 + 8 * (i >> 2) + 4 * half + (i & 3) >= limit) s[b][i] = -INFINITY;
+        }
+        float top = s[0][0];
+#pragma unroll
+        for (int b = 0; b < KB; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
+        top = fmaxf(top, __shfl_xor(top, 32));
+        if (__any(top * c > m * c + 8.f || (m == -INFINITY && top > m))) {
+            const float next = fmaxf(m, top);
+            const float f = next == -INFINITY ? 0.f : exp2f((m - next) * c);
+            l *= f;
+#pragma unroll
+            for (int i = 0; i < DB; ++i)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) o[i][j] *= f;
+            m = next;
+        }
+        const float base = m == -INFINITY ? 0.f : -m * c;
+        float sum = 0.f;
+#pragma unroll
+        for (int b = 0; b < KB; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], c, base));
+                sum += s[b][i];
+            }
+        l += sum;
+#pragma unroll
+        for (int b = 0; b < KB; ++b) {
+            if constexpr (sizeof(T) == 2) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float p[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) p[i] = s[b][8 * h + i];
+                    const vo_u32x4 pf = E::pack(p);
+#pragma unroll
+                    for (int d = 0; d < DB; ++d) {
+                        // keys r.. and r + 8.. : the lane supplies 8 bytes of row r + (lane % 16) / 4 and receives four rows of
+                        // feature d * 32 + lane % 32
+                        const int r = b * 32 + 16 * h + 4 * half + ((lane & 15) >> 2);
+                        const int chunk = d * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
+                        const int at = (lane & 1) * 8;
+                        const vo_u32x2 lo = transposed(vt + r * L::ROW + ((chunk ^ L::v_swz(r)) * 16) + at);
+                        const vo_u32x2 hi = transposed(vt + (r + 8) * L::ROW + ((chunk ^ L::v_swz(r + 8)) * 16) + at);
+                        o[d] = E::mma32(vo_u32x4{lo[0], lo[1], hi[0], hi[1]}, pf, o[d]);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int r = b * 32 + 8 * (i >> 2) + 4 * half + (i & 3);
+#pragma unroll
+                    for (int d = 0; d < DB; ++d) {
+                        const int chunk = d * 8 + (col >> 2);
+                        const float vf = *reinterpret_cast<const float*>(vt + r * L::ROW + ((chunk ^ L::v_swz(r)) * 16) + (col & 3) * 4);
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf, s[b][i], o[d], 0, 0, 0);
+                    }
+                }
+            }
+        }
+    }
+    static __device__ __forceinline__ vo_u32x2 transposed(const unsigned char* p) {
+        typedef short s16x4 __attribute__((ext_vector_type(4)));
+        return __builtin_bit_cast(vo_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
+    }
+};
+
+// A wave's share of the 16-byte pieces of one operand's key tile: N loads of 64 pieces.
+template <typename T, int DT, int KEYS, int WAVES> struct Loader {
+    using L = Tile<T, DT>;
+    static constexpr int N = KEYS * L::CH / 64 / WAVES;
+    static_assert(N >= 1 && KEYS * L::CH % (64 * WAVES) == 0, "a key tile must be whole wave loads");
+    unsigned off[N];
+    __device__ __forceinline__ void init(int64_t stride, int D, bool is_v, int wave, int lane) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int piece = (wave * N + i) * 64 + lane, r = piece / L::CH;
+            const int chunk = (piece % L::CH) ^ (is_v ? L::v_swz(r) : L::k_swz(r));
+            off[i] = chunk * L::PER < D ? (unsigned)(r * stride * L::ES) + chunk * 16 : VO_OUTSIDE;
+        }
+    }
+    // base: the tile's first key; keys: how many there are (the rest of the tile becomes zero)
+    __device__ __forceinline__ void load(const T* base, int64_t stride, int64_t keys, int D, unsigned char* lds, int wave) const {
+        const int64_t n = keys < KEYS ? keys : KEYS;
+        const __amdgpu_buffer_rsrc_t rs = vo_buffer(base, n > 0 ? ((n - 1) * stride + D) * L::ES : 0);
+#pragma unroll
+        for (int i = 0; i < N; ++i) vo_load_to_lds(rs, lds + (wave * N + i) * 1024, off[i]);
+    }
+};
+
+// A lane's column of O^T: row `row` of the output, or (split) of the workspace.
+template <typename T, int DT> __device__ __forceinline__ void store_part(const AttArgs& a, int split, int64_t token, int head,
+                                                                         const vo_f32x16* o, float m, float l, int lane) {
+    const int64_t row = ((int64_t)split * a.Tq + token) * a.Hq + head;
+    float* p = a.part + row * a.D;
+#pragma unroll
+    for (int d = 0; d < DT / 32; ++d)
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const int f = d * 32 + 8 * b + 4 * (lane >> 5);
+            if (f < a.D) *reinterpret_cast<float4*>(p + f) = make_float4(o[d][4 * b], o[d][4 * b + 1], o[d][4 * b + 2], o[d][4 * b + 3]);
+        }
+    if (lane < 32) {
+        float* ml = a.part + (int64_t)a.splits * a.Tq * a.Hq * a.D + row * 2;
+        ml[0] = m * a.c;
+        ml[1] = l;
+    }
+}
+
+template <typename T, int DT> __device__ __forceinline__ void store_out(const AttArgs& a, int64_t token, int head, const vo_f32x16* o,
+                                                                        float inv, int lane) {
+    T* p = static_cast<T*>(a.out) + token * a.os + head * a.oh;
+#pragma unroll
+    for (int d = 0; d < DT / 32; ++d)
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const int f = d * 32 + 8 * b + 4 * (lane >> 5);
+            if (f >= a.D) continue;
+            const float v0 = o[d][4 * b] * inv, v1 = o[d][4 * b + 1] * inv, v2 = o[d][4 * b + 2] * inv, v3 = o[d][4 * b + 3] * inv;
+            if constexpr (sizeof(T) == 2)
+                *reinterpret_cast<vo_u32x2*>(p + f) = vo_u32x2{vo_elem<T>::pack2(v0, v1), vo_elem<T>::pack2(v2, v3)};
+            else
+                *reinterpret_cast<float4*>(p + f) = make_float4(v0, v1, v2, v3);
+        }
+}
+
+__device__ __forceinline__ float inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }      // 0: the row saw nothing
+
+// ------------------------------------------------------------------------------------------------------------ tiles
+template <typename T, int DT, int KEYS, int MIN_BLOCKS>
+__global__ __launch_bounds__(256, MIN_BLOCKS) void attention_tiles(const AttArgs a) {
+    using L = Tile<T, DT>;
+    constexpr int ROWS = 128, HALF = KEYS * L::ROW;
+    __shared__ __align__(16) unsigned char lds[4 * HALF];            // two stages of K and V
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+
+    // numbers: key head outermost (an XCD keeps to few of them: their keys stay in its L2), then split, then row tiles from
+    // the last (the longest ones of a causal sequence come first), then the heads of the group
+    const unsigned id = vo_xcd_contiguous(blockIdx.x, gridDim.x);
+    const int g = id % a.group;
+    unsigned rest = id / a.group;
+    const unsigned tile = a.tiles - 1 - rest % a.tiles;
+    rest /= a.tiles;
+    const int split = rest % a.splits, kh = rest / a.splits, head = kh * a.group + g;
+    const vo_place p = vo_find_tile(a.q_off, a.k_off, a.sequences, a.Tq, a.Tk, tile, 1, ROWS);
+    if (!p.any) return;
+
+    const int64_t shift = p.Lk - p.Lq;
+    const int64_t last_row = p.row + ROWS < p.Lq ? p.row + ROWS : p.Lq;                      // one past the tile's rows
+    int64_t seen = a.causal ? last_row + shift : p.Lk;                                       // keys that some row sees
+    seen = vo_clamp64(seen, 0, p.Lk);
+    const int64_t key_tiles = (seen + KEYS - 1) / KEYS, per = (key_tiles + a.splits - 1) / a.splits;
+    const int64_t t0 = split * per < key_tiles ? split * per : key_tiles, t1 = t0 + per < key_tiles ? t0 + per : key_tiles;
+
+    const int64_t row = p.row + wave * 32 + (lane & 31);
+    const bool have = row < p.Lq;
+    Core<T, DT, KEYS> core;
+    core.reset();
+    core.load_q(have ? static_cast<const T*>(a.q) + (p.q0 + row) * a.qs + head * a.qh : nullptr, a.D, lane);
+    // keys below `limit` are seen by this lane's row; tiles wholly below wave_all need no mask, from wave_any on no work
+    const int64_t limit = a.causal ? vo_clamp64(row + shift + 1, 0, p.Lk) : p.Lk;
+    const int64_t wave_all = a.causal ? vo_clamp64(p.row + wave * 32 + shift + 1, 0, p.Lk) : p.Lk;
+    const int64_t wave_any = a.causal ? vo_clamp64(p.row + wave * 32 + 32 + shift, 0, p.Lk) : p.Lk;
+
+    const T* kb = static_cast<const T*>(a.k) + p.k0 * a.ks + kh * a.kh;
+    const T* vb = static_cast<const T*>(a.v) + p.k0 * a.vs + kh * a.vh;
+    Loader<T, DT, KEYS, 4> lk, lv;
+    lk.init(a.ks, a.D, false, wave, lane);
+    lv.init(a.vs, a.D, true, wave, lane);
+    auto fetch = [&](int64_t t, unsigned char* buf) {
+        lk.load(kb + t * KEYS * a.ks, a.ks, p.Lk - t * KEYS, a.D, buf, wave);
+        lv.load(vb + t * KEYS * a.vs, a.vs, p.Lk - t * KEYS, a.D, buf + HALF, wave);
+    };
+    if (t0 < t1) fetch(t0, lds);
+    for (int64_t t = t0; t < t1; ++t) {
+        unsigned char* now = lds + ((t - t0) & 1) * 2 * HALF;
+        __syncthreads();                                             // tile t has arrived, tile t - 1 has been read
+        if (t + 1 < t1) fetch(t + 1, lds + (1 - ((t - t0) & 1)) * 2 * HALF);
+        const int64_t key = t * KEYS;
+        if (key < wave_any) core.step(now, now + HALF, a.c, key + KEYS > wave_all, (int)vo_clamp64(limit - key, 0, KEYS), lane);
+    }
+    const float l = core.l + __shfl_xor(core.l, 32);
+    if (!have) return;
+    if (a.splits > 1) store_part<T, DT>(a, split, p.q0 + row, head, core.o, core.m, l, lane);
+    else store_out<T, DT>(a, p.q0 + row, head, core.o, inverse(l), lane);
+}
+
+// ------------------------------------------------------------------------------------------------------------- rows
+template <typename T, int DT, int KEYS, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void attention_rows(const AttArgs a) {
+    using L = Tile<T, DT>;
+    constexpr int HALF = KEYS * L::ROW, MINE = 4 * HALF;             // a wave's two stages of K and V
+    __shared__ __align__(16) unsigned char lds[WAVES * MINE];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const unsigned id = vo_xcd_contiguous(blockIdx.x, gridDim.x);
+    const int split = id % a.splits;
+    unsigned rest = id / a.splits;
+    const unsigned tile = rest % a.tiles;
+    const int kh = rest / a.tiles;
+    const vo_place p = vo_find_tile(a.q_off, a.k_off, a.sequences, a.Tq, a.Tk, tile, a.group, 32);
+    if (!p.any) return;
+
+    const int64_t shift = p.Lk - p.Lq, rows = p.Lq * a.group;
+    const int64_t last_row = p.row + 32 < rows ? p.row + 32 : rows;
+    int64_t seen = a.causal ? (last_row - 1) / a.group + 1 + shift : p.Lk;
+    seen = vo_clamp64(seen, 0, p.Lk);
+    const int64_t key_tiles = (seen + KEYS - 1) / KEYS, per = (key_tiles + a.splits - 1) / a.splits;
+    const int64_t t0 = split * per < key_tiles ? split * per : key_tiles, t1 = t0 + per < key_tiles ? t0 + per : key_tiles;
+
+    const int64_t row = p.row + (lane & 31);
+    const bool have = row < rows;
+    const int64_t token = have ? row / a.group : 0;
+    const int head = kh * a.group + (int)(have ? row % a.group : 0);
+    Core<T, DT, KEYS> core;
+    core.reset();
+    core.load_q(have ? static_cast<const T*>(a.q) + (p.q0 + token) * a.qs + head * a.qh : nullptr, a.D, lane);
+    const int64_t limit = a.causal ? vo_clamp64(token + shift + 1, 0, p.Lk) : p.Lk;
+    const int64_t all = a.causal ? vo_clamp64(p.row / a.group + shift + 1, 0, p.Lk) : p.Lk;
+
+    const T* kb = static_cast<const T*>(a.k) + p.k0 * a.ks + kh * a.kh;
+    const T* vb = static_cast<const T*>(a.v) + p.k0 * a.vs + kh * a.vh;
+    unsigned char* mine = lds + wave * MINE;
+    Loader<T, DT, KEYS, 1> lk, lv;
+    lk.init(a.ks, a.D, false, 0, lane);
+    lv.init(a.vs, a.D, true, 0, lane);
+    auto fetch = [&](int64_t t, unsigned char* buf) {                // 2 * N loads into the wave's own LDS
+        lk.load(kb + t * KEYS * a.ks, a.ks, p.Lk - t * KEYS, a.D, buf, 0);
+        lv.load(vb + t * KEYS * a.vs, a.vs, p.Lk - t * KEYS, a.D, buf + HALF, 0);
+    };
+    if (t0 + wave < t1) fetch(t0 + wave, mine);
+    int stage = 0;
+    for (int64_t t = t0 + wave; t < t1; t += WAVES, stage ^= 1) {
+        unsigned char* now = mine + stage * 2 * HALF;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");             // tile t has arrived
+        if (t + WAVES < t1) fetch(t + WAVES, mine + (stage ^ 1) * 2 * HALF);
+        const int64_t key = t * KEYS;
+        core.step(now, now + HALF, a.c, key + KEYS > all, (int)vo_clamp64(limit - key, 0, KEYS), lane);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");           // its reads are done before it is loaded over
+    }
+    core.l += __shfl_xor(core.l, 32);
+
+    // join the waves in order: sums as (feature, row) planes of LDS, m and l behind them
+    constexpr int PLANE = DT * 33 * 4;                               // 33: lanes of one row apart in banks
+    static_assert(PLANE + 256 <= MINE || WAVES == 1, "the join must fit the wave's stages");
+    float* ml = reinterpret_cast<float*>(lds + wave * MINE + PLANE);
+    float m = core.m, l = core.l;
+    if constexpr (WAVES > 1) {
+        float* sums = reinterpret_cast<float*>(mine);
+        // every wave's own stages are free here: its loads have landed and its reads are done
+#pragma unroll
+        for (int d = 0; d < DT / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sums[(d * 32 + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3)) * 33 + (lane & 31)] = core.o[d][i];
+        if (lane < 32) { ml[lane] = core.m; ml[32 + lane] = core.l; }
+        __syncthreads();
+        float w[WAVES];
+        m = -INFINITY;
+        l = 0.f;
+#pragma unroll
+        for (int i = 0; i < WAVES; ++i) m = fmaxf(m, reinterpret_cast<const float*>(lds + i * MINE + PLANE)[lane & 31]);
+#pragma unroll
+        for (int i = 0; i < WAVES; ++i) {
+            const float* x = reinterpret_cast<const float*>(lds + i * MINE + PLANE);
+            w[i] = m == -INFINITY ? 0.f : exp2f((x[lane & 31] - m) * a.c);
+            l += w[i] * x[32 + (lane & 31)];
+        }
+        // wave w finishes the feature blocks w, w + WAVES, ..
+        const int64_t prow = ((int64_t)split * a.Tq + p.q0 + token) * a.Hq + head;
+        const float inv = inverse(l);
+        for (int d = wave; d < DT / 32; d += WAVES) {
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const int f = d * 32 + 8 * b + 4 * (lane >> 5);
+                float v[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    v[j] = 0.f;
+#pragma unroll
+                    for (int i = 0; i < WAVES; ++i) v[j] += w[i] * reinterpret_cast<const float*>(lds + i * MINE)[(f + j) * 33 + (lane & 31)];
+                }
+                if (!have || f >= a.D) continue;
+                if (a.splits > 1) {
+                    *reinterpret_cast<float4*>(a.part + prow * a.D + f) = make_float4(v[0], v[1], v[2], v[3]);
+                } else {
+                    T* y = static_cast<T*>(a.out) + (p.q0 + token) * a.os + head * a.oh + f;
+                    if constexpr (sizeof(T) == 2)
+                        *reinterpret_cast<vo_u32x2*>(y) = vo_u32x2{vo_elem<T>::pack2(v[0] * inv, v[1] * inv), vo_elem<T>::pack2(v[2] * inv, v[3] * inv)};
+                    else
+                        *reinterpret_cast<float4*>(y) = make_float4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+                }
+            }
+        }
+        if (a.splits > 1 && wave == 0 && lane < 32 && have) {
+            float* x = a.part + (int64_t)a.splits * a.Tq * a.Hq * a.D + prow * 2;
+            x[0] = m * a.c;
+            x[1] = l;
+        }
+    } else {
+        if (!have) return;
+        if (a.splits > 1) store_part<T, DT>(a, split, p.q0 + token, head, core.o, m, l, lane);
+        else store_out<T, DT>(a, p.q0 + token, head, core.o, inverse(l), lane);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------- join
+// One wave per (token, head); the parts are added in their order.  Rows outside every sequence stay as they are.
+template <typename T> __global__ __launch_bounds__(256) void attention_join(const AttArgs a) {
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    const int64_t token = row / a.Hq;
+    if (token >= a.Tq) return;
+    if (a.q_off && (token < a.q_off[0] || token >= a.q_off[a.sequences])) return;
+    const int head = (int)(row % a.Hq);
+    const int64_t step = a.Tq * a.Hq;
+    const float* ml = a.part + (int64_t)a.splits * step * a.D;
+    float m = -INFINITY;
+    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, ml[(s * step + row) * 2]);
+    float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < a.splits; ++s) {
+        const float ms = ml[(s * step + row) * 2], w = ms == -INFINITY ? 0.f : exp2f(ms - m);
+        if (ms == -INFINITY) continue;                               // that part saw no key of this row
+        l += w * ml[(s * step + row) * 2 + 1];
+        if (lane * 4 < a.D) {
+            const float4 x = *reinterpret_cast<const float4*>(a.part + (s * step + row) * a.D + lane * 4);
+            o[0] += w * x.x; o[1] += w * x.y; o[2] += w * x.z; o[3] += w * x.w;
+        }
+    }
+    if (lane * 4 >= a.D) return;
+    const float inv = inverse(l);
+    T* p = static_cast<T*>(a.out) + token * a.os + head * a.oh + lane * 4;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) vo_elem<T>::put(p + j, o[j] * inv);
+}
+
+// ------------------------------------------------------------------------------------------------------------- host
+
+struct Plan {
+    bool rows;
+    int splits;
+    int64_t tiles, blocks;
+};
+
+Plan plan(int64_t Tq, int64_t Tk, int sequences, int Hq, int Hk) {
+    const int group = Hq / Hk;
+    Plan p{};
+    const int64_t rows = vo_ceil_div(Tq * group, sequences);         // a sequence's rows per key head, on average
+    const int64_t keys = vo_ceil_div(Tk, sequences);
+    p.rows = rows <= 32;
+    p.tiles = p.rows ? vo_tiles_bound(Tq, sequences, group, 32) : vo_tiles_bound(Tq, sequences, 1, 128);
+    const int64_t base = p.tiles * (p.rows ? Hk : Hq);
+    int64_t want = vo_ceil_div(p.rows ? 2048 : 768, base), most = keys / (p.rows ? 128 : 256);
+    if (want > most) want = most;
+    if (want > 64) want = 64;
+    if (want < 1) want = 1;
+    p.splits = (int)want;
+    p.blocks = base * want;
+    return p;
+}
+
+int64_t workspace(const Plan& p, int64_t Tq, int Hq, int D) { return p.splits > 1 ? (int64_t)p.splits * Tq * Hq * (D + 2) * 4 : 0; }
+
+template <typename T, int DT> int launch(const AttArgs& a, const Plan& p, hipStream_t st) {
+    constexpr int BYTES = DT * (int)sizeof(T);                       // of a row
+    const dim3 grid((unsigned)p.blocks);
+    if (p.rows) {
+        constexpr int KEYS = BYTES <= 128 ? 64 : 32, WAVES = BYTES <= 256 ? 4 : BYTES <= 512 ? 2 : 1;
+        attention_rows<T, DT, KEYS, WAVES><<<grid, 64 * WAVES, 0, st>>>(a);
+    } else {
+        constexpr int KEYS = BYTES <= 512 ? 64 : 32;
+        attention_tiles<T, DT, KEYS, BYTES <= 256 ? 2 : 1><<<grid, 256, 0, st>>>(a);
+    }
+    VO_CHECK_LAUNCH("vo_attention");
+    if (p.splits > 1) {
+        attention_join<T><<<dim3((unsigned)vo_ceil_div(a.Tq * a.Hq, 4)), 256, 0, st>>>(a);
+        VO_CHECK_LAUNCH("vo_attention (join)");
+    }
+    return VO_OK;
+}
+
+template <typename T> int dispatch(const AttArgs& a, const Plan& p, hipStream_t st) {
+    if (a.D <= 32) return launch<T, 32>(a, p, st);
+    if (a.D <= 64) return launch<T, 64>(a, p, st);
+    if (a.D <= 128) return launch<T, 128>(a, p, st);
+    return launch<T, 256>(a, p, st);
+}
+
+}  // namespace
+
+extern "C" int64_t vo_attention_workspace_bytes(int64_t q_tokens, int64_t k_tokens, int sequences, int q_heads, int k_heads, int D) {
+    if (q_tokens <= 0 || k_tokens < 0 || sequences <= 0 || q_heads <= 0 || k_heads <= 0 || q_heads % k_heads || D <= 0) return 0;
+    return workspace(plan(q_tokens, k_tokens, sequences, q_heads, k_heads), q_tokens, q_heads, D);
+}
+
+extern "C" int vo_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k, int64_t k_token_stride,
+                            int64_t k_head_stride, const void* v, int64_t v_token_stride, int64_t v_head_stride, void* out,
+                            int64_t out_token_stride, int64_t out_head_stride, const int32_t* q_offsets, const int32_t* k_offsets,
+                            int sequences, int64_t q_tokens, int64_t k_tokens, int q_heads, int k_heads, int D, float scale, int causal,
+                            int dtype, void* workspace_ptr, int64_t workspace_bytes, void* stream) {
+    VO_REQUIRE(dtype == VO_F32 || dtype == VO_F16 || dtype == VO_BF16, "vo_attention: dtype=%d is none of VO_F32, VO_F16, VO_BF16", dtype);
+    VO_REQUIRE(sequences >= 1 && q_tokens >= 0 && k_tokens >= 0 && q_heads >= 1 && k_heads >= 1 && q_heads % k_heads == 0,
+               "vo_attention: sequences=%d q_tokens=%lld k_tokens=%lld heads %d / %d (heads a multiple of the key heads)", sequences,
+               (long long)q_tokens, (long long)k_tokens, q_heads, k_heads);
+    VO_REQUIRE(scale > 0.f && scale < INFINITY, "vo_attention: scale must be positive and finite");
+    VO_REQUIRE((q_offsets && k_offsets) || (!q_offsets && !k_offsets && sequences == 1),
+               "vo_attention: both offset arrays, or none and one sequence");
+    const int64_t es = dtype == VO_F32 ? 4 : 2;
+    if (D < 1 || D > 256 || D * es % 16) return vo_fail(VO_ERR_UNSUPPORTED, "vo_attention: D=%d must be at most 256 and whole 16-byte pieces", D);
+    if (q_tokens == 0) return VO_OK;
+    VO_REQUIRE(q && out && (k_tokens == 0 || (k && v)), "vo_attention: null pointer");
+    const int64_t strides[] = {q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride, out_token_stride, out_head_stride};
+    for (int64_t s : strides)
+        if (s < 0 || s * es % 16 || s * es >= (1ll << 24))
+            return vo_fail(VO_ERR_UNSUPPORTED, "vo_attention: strides must be whole 16-byte pieces under 16 MiB (got %lld elements)", (long long)s);
+    if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(out)) % 16)
+        return vo_fail(VO_ERR_UNSUPPORTED, "vo_attention: tensors must be 16-byte aligned");
+    if (q_tokens >= (1ll << 31) || k_tokens >= (1ll << 31))
+        return vo_fail(VO_ERR_UNSUPPORTED, "vo_attention: offsets are 32-bit: fewer than 2^31 tokens");
+    const Plan p = plan(q_tokens, k_tokens, sequences, q_heads, k_heads);
+    if (p.blocks >= (1ll << 31) || q_tokens * q_heads >= (1ll << 32))
+        return vo_fail(VO_ERR_UNSUPPORTED, "vo_attention: %lld tokens of %d heads are too many for one launch", (long long)q_tokens, q_heads);
+    const int64_t need = workspace(p, q_tokens, q_heads, D);
+    VO_REQUIRE(need == 0 || (workspace_ptr && workspace_bytes >= need && reinterpret_cast<uintptr_t>(workspace_ptr) % 16 == 0),
+               "vo_attention: needs a 16-byte aligned workspace of %lld bytes", (long long)need);
+    AttArgs a{};
+    a.q = q; a.k = k; a.v = v; a.out = out; a.part = static_cast<float*>(workspace_ptr);
+    a.q_off = q_offsets; a.k_off = k_offsets;
+    a.qs = q_token_stride; a.qh = q_head_stride; a.ks = k_token_stride; a.kh = k_head_stride;
+    a.vs = v_token_stride; a.vh = v_head_stride; a.os = out_token_stride; a.oh = out_head_stride;
+    a.Tq = q_tokens; a.Tk = k_tokens;
+    a.sequences = sequences; a.Hq = q_heads; a.Hk = k_heads; a.group = q_heads / k_heads;
+    a.D = D; a.causal = causal != 0; a.splits = p.splits;
+    a.tiles = (unsigned)p.tiles;
+    a.c = scale * LOG2E;
+    hipStream_t st = vo_stream(stream);
+    if (dtype == VO_F32) return dispatch<float>(a, p, st);
+    if (dtype == VO_F16) return dispatch<_Float16>(a, p, st);
+    return dispatch<__bf16>(a, p, st);
+}

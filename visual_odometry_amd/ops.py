@@ -1188,6 +1188,76 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     return out
 
 
+def _heads(t: torch.Tensor, name: str):
+    """(tokens, heads, D) with D consecutive -> (ptr, token stride, head stride) in elements."""
+    if t.dim() != 3 or t.shape[1] < 1 or t.shape[2] < 1:
+        raise ValueError(f"{name} must be (tokens, heads, D), got {tuple(t.shape)}")
+    st = t.stride()
+    if t.shape[2] > 1 and st[2] != 1:
+        raise ValueError(f"{name}: a head's elements must be consecutive (got strides {st})")
+    D = t.shape[2]
+    return t.data_ptr(), (st[0] if t.shape[0] > 1 else t.shape[1] * D), (st[1] if t.shape[1] > 1 else D)
+
+
+def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: torch.Tensor | None = None,
+              k_offsets: torch.Tensor | None = None, causal: bool = False, scale: float | None = None,
+              out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of packed sequences: q (Tq,Hq,D), k and v (Tk,Hk,D), Hq a multiple of Hk -> (Tq,Hq,D).
+
+    Sequence s owns the rows q_offsets[s] .. q_offsets[s+1]-1 and the keys k_offsets[s] .. k_offsets[s+1]-1 (ascending int32
+    GPU tensors of sequences + 1 entries, any length from 0; without offsets everything is one sequence; q_offsets alone
+    serves for both when Tq = Tk).  Every row takes softmax(scale * q.k) over its sequence's keys, ``causal``: over the keys
+    j <= i + Lk - Lq (aligned at the ends, so a single new row sees the whole history); a row that sees no key gives zeros.
+    ``scale`` defaults to 1/sqrt(D).  float32, float16 or bfloat16; scores, softmax and sums in float32.  Tokens and heads may
+    lie any whole number of 16-byte pieces apart (slices of a fused projection); D is at most 256 and a multiple of 8 (4 in
+    float32).  Rows outside every sequence are not written (give ``out`` to say what they hold).  The lengths stay on the
+    device: nothing synchronises, and the call can be captured.  Equal inputs give equal bits."""
+    _token_tensor(q, "q")
+    _token_tensor(k, "k", q)
+    _token_tensor(v, "v", q)
+    pq, qs, qh = _heads(q, "q")
+    pk, ks, kh = _heads(k, "k")
+    pv, vs, vh = _heads(v, "v")
+    Tq, Hq, D = q.shape
+    Tk, Hk, _ = k.shape
+    if v.shape != k.shape or k.shape[2] != D:
+        raise ValueError(f"k and v must be (Tk,Hk,{D}), got {tuple(k.shape)} and {tuple(v.shape)}")
+    if Hq % Hk:
+        raise ValueError(f"{Hq} heads are no multiple of {Hk} key heads")
+    if k_offsets is None and q_offsets is not None:
+        if Tq != Tk:
+            raise ValueError("q_offsets alone serves for both only when q and k have as many tokens")
+        k_offsets = q_offsets
+    if (q_offsets is None) != (k_offsets is None):
+        raise ValueError("k_offsets needs q_offsets")
+    sequences = 1
+    if q_offsets is not None:
+        for t, n in ((q_offsets, "q_offsets"), (k_offsets, "k_offsets")):
+            _dev(t, n, torch.int32)
+            if t.dim() != 1 or t.numel() < 2 or t.numel() != q_offsets.numel() or t.device != q.device:
+                raise ValueError(f"{n} must be (sequences + 1) on q's device, as many as q_offsets")
+        sequences = q_offsets.numel() - 1
+    scale = D ** -0.5 if scale is None else float(scale)
+    if out is None:
+        out = torch.empty((Tq, Hq, D), device=q.device, dtype=q.dtype)
+    elif tuple(_token_tensor(out, "out", q).shape) != (Tq, Hq, D):
+        raise ValueError(f"out must be {(Tq, Hq, D)}, got {tuple(out.shape)}")
+    else:
+        if any(s <= 0 for n, s in zip(out.shape, out.stride()) if n > 1):
+            raise ValueError(f"out: elements overlap (got strides {out.stride()})")
+        for t, n in ((q, "q"), (k, "k"), (v, "v")):
+            _no_overlap(out, t, n)
+    po, os_, oh = _heads(out, "out")
+    with torch.cuda.device(q.device):
+        need = int(_lib.load().vo_attention_workspace_bytes(Tq, Tk, sequences, Hq, Hk, D))
+        work = torch.empty((need,), device=q.device, dtype=torch.uint8) if need else None
+        _call("vo_attention", pq, qs, qh, pk, ks, kh, pv, vs, vh, po, os_, oh,
+              0 if q_offsets is None else q_offsets.data_ptr(), 0 if k_offsets is None else k_offsets.data_ptr(), sequences, Tq, Tk,
+              Hq, Hk, D, scale, int(bool(causal)), _TOKEN_DTYPES[q.dtype], 0 if work is None else work.data_ptr(), need, _stream(),
+              nbytes=q.element_size() * D * (2 * Tq * Hq + 2 * Tk * Hk))
+    return out
+
+
 # -------------------------------------------------------------- geometry ops
 
 def disparity_to_depth(disparity: torch.Tensor, fxB: float, divide_in_f64: bool = True) -> torch.Tensor:
