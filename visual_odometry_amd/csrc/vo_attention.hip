@@ -280,7 +280,7 @@ __global__ __launch_bounds__(256, MIN_BLOCKS) void attention_tiles(const AttArgs
     if (t0 < t1) fetch(t0, lds);
     for (int64_t t = t0; t < t1; ++t) {
         unsigned char* now = lds + ((t - t0) & 1) * 2 * HALF;
-        __syncthreads();                                             // tile t has arrived, tile t - 1 has been read
+        vo_lds_barrier();                                            // tile t has arrived, tile t - 1 has been read
         if (t + 1 < t1) fetch(t + 1, lds + (1 - ((t - t0) & 1)) * 2 * HALF);
         const int64_t key = t * KEYS;
         if (key < wave_any) core.step(now, now + HALF, a.c, key + KEYS > wave_all, (int)vo_clamp64(limit - key, 0, KEYS), lane);

@@ -38,47 +38,59 @@ __device__ __forceinline__ float activate(float z, int act) {
     }
 }
 
-// N consecutive outputs k.. of row m: bias, activation, residual, one rounding.  N = PER (16 bytes) or any number up to it.
-template <typename T> __device__ __forceinline__ void finish(const LinArgs& a, int64_t m, int k, const float* acc) {
-    constexpr int PER = vo_elem<T>::PER;
-    const T* res = static_cast<const T*>(a.res);
-    T* y = static_cast<T*>(a.y) + m * a.ys + k;
-    float v[PER];
-    const int n = a.K - k < PER ? a.K - k : PER;
-#pragma unroll
-    for (int j = 0; j < PER; ++j) v[j] = activate(acc[j] + (a.bias && j < n ? a.bias[k + j] : 0.f), a.act);
-    if (a.wide_out && n == PER) {
-        if (res) {
-            float r[PER];
-            vo_elem<T>::unpack(*reinterpret_cast<const vo_u32x4*>(res + m * a.rs + k), r);
-#pragma unroll
-            for (int j = 0; j < PER; ++j) v[j] += r[j];
-        }
-        *reinterpret_cast<vo_u32x4*>(y) = vo_elem<T>::pack(v);
-    } else {
-#pragma unroll
-        for (int j = 0; j < PER; ++j)
-            if (j < n) vo_elem<T>::put(y + j, v[j] + (res ? vo_elem<T>::get(res + m * a.rs + k + j) : 0.f));
-    }
-}
+// PER consecutive outputs k.. of one row (`n` of them exist): the bias and, where rows allow wide accesses, the residual are
+// fetched ahead of their use.
+template <typename T> struct Piece {
+    static constexpr int PER = vo_elem<T>::PER;
+    vo_u32x4 res;
 
-// A wave's PER consecutive sums: into the workspace or through the epilogue.
-template <typename T> __device__ __forceinline__ void emit(const LinArgs& a, int split, int64_t m, int k, const float* acc) {
-    constexpr int PER = vo_elem<T>::PER;
-    if (a.splits > 1) {
-        float* p = a.part + ((int64_t)split * a.M + m) * a.K + k;
-        if ((a.K & 3) == 0 && k + PER <= a.K) {
+    static __device__ __forceinline__ void load_bias(const LinArgs& a, int k, float* bias) {
 #pragma unroll
-            for (int j = 0; j < PER; j += 4) *reinterpret_cast<float4*>(p + j) = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+        for (int j = 0; j < PER; ++j) bias[j] = a.bias && k + j < a.K ? a.bias[k + j] : 0.f;
+    }
+    __device__ __forceinline__ void load_residual(const LinArgs& a, int64_t m, int k) {
+        res = vo_u32x4{0, 0, 0, 0};
+        if (a.res && a.wide_out && m < a.M && k + PER <= a.K)
+            res = *reinterpret_cast<const vo_u32x4*>(static_cast<const T*>(a.res) + m * a.rs + k);
+    }
+    // bias, activation, residual, one rounding
+    __device__ __forceinline__ void finish(const LinArgs& a, int64_t m, int k, const float* acc, const float* bias) const {
+        T* y = static_cast<T*>(a.y) + m * a.ys + k;
+        float v[PER];
+#pragma unroll
+        for (int j = 0; j < PER; ++j) v[j] = activate(acc[j] + bias[j], a.act);
+        if (a.wide_out && k + PER <= a.K) {
+            if (a.res) {
+                float r[PER];
+                vo_elem<T>::unpack(res, r);
+#pragma unroll
+                for (int j = 0; j < PER; ++j) v[j] += r[j];
+            }
+            *reinterpret_cast<vo_u32x4*>(y) = vo_elem<T>::pack(v);
         } else {
+            const T* r = static_cast<const T*>(a.res) + m * a.rs + k;
 #pragma unroll
             for (int j = 0; j < PER; ++j)
-                if (k + j < a.K) p[j] = acc[j];
+                if (k + j < a.K) vo_elem<T>::put(y + j, v[j] + (a.res ? vo_elem<T>::get(r + j) : 0.f));
         }
-    } else {
-        finish<T>(a, m, k, acc);
     }
-}
+    // into the workspace or through the epilogue
+    __device__ __forceinline__ void emit(const LinArgs& a, int split, int64_t m, int k, const float* acc, const float* bias) const {
+        if (a.splits > 1) {
+            float* p = a.part + ((int64_t)split * a.M + m) * a.K + k;
+            if ((a.K & 3) == 0 && k + PER <= a.K) {
+#pragma unroll
+                for (int j = 0; j < PER; j += 4) *reinterpret_cast<float4*>(p + j) = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < PER; ++j)
+                    if (k + j < a.K) p[j] = acc[j];
+            }
+        } else {
+            finish(a, m, k, acc, bias);
+        }
+    }
+};
 
 // ------------------------------------------------------------------------------------------------------------ tiles
 // WGM x WGN waves; a wave owns TM rows of x times TN outputs as 16x16 products with W as the first operand, so that a lane
@@ -160,41 +172,83 @@ __global__ __launch_bounds__(64 * WGM * WGN) void linear_tiles(const LinArgs a) 
     const int wm = wave / WGN, wn = wave % WGN;
     vo_f32x4 acc[NT][MT] = {};
     const int fr = lane & 15, fg = lane >> 4;
-    auto compute = [&](const unsigned char* buf) {
+    struct Frags { vo_u32x4 w[NT], x[MT]; } f0, f1;                  // operands of a slab's two halves
+    auto read = [&](Frags& f, const unsigned char* buf, int kk) {
+        const int pos = ((kk * 4 + fg) ^ (fr & 7)) * 16;
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            const int pos = ((kk * 4 + fg) ^ (fr & 7)) * 16;
-            vo_u32x4 xf[MT], wf[NT];
+        for (int i = 0; i < NT; ++i) f.w[i] = *reinterpret_cast<const vo_u32x4*>(buf + (BM + wn * TN + i * 16 + fr) * 128 + pos);
 #pragma unroll
-            for (int i = 0; i < NT; ++i) wf[i] = *reinterpret_cast<const vo_u32x4*>(buf + (BM + wn * TN + i * 16 + fr) * 128 + pos);
+        for (int i = 0; i < MT; ++i) f.x[i] = *reinterpret_cast<const vo_u32x4*>(buf + (wm * TM + i * 16 + fr) * 128 + pos);
+    };
+    auto multiply = [&](const Frags& f) {
 #pragma unroll
-            for (int i = 0; i < MT; ++i) xf[i] = *reinterpret_cast<const vo_u32x4*>(buf + (wm * TM + i * 16 + fr) * 128 + pos);
+        for (int i = 0; i < NT; ++i)
 #pragma unroll
-            for (int i = 0; i < NT; ++i)
+            for (int j = 0; j < MT; ++j) acc[i][j] = vo_elem<T>::mma16(f.w[i], f.x[j], acc[i][j]);
+    };
+    // one LDS read per few products, so that neither pipe waits for the other
+    auto interleave = [&]() {
+        constexpr int PRODUCTS = NT * MT * (sizeof(T) == 4 ? 4 : 1), READS = NT + MT, EACH = PRODUCTS / READS;
 #pragma unroll
-                for (int j = 0; j < MT; ++j) acc[i][j] = vo_elem<T>::mma16(wf[i], xf[j], acc[i][j]);
+        for (int i = 0; i < READS; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, EACH, 0);
         }
+        __builtin_amdgcn_sched_group_barrier(0x008, PRODUCTS - READS * EACH, 0);
     };
 
-    if (slabs > 0) {
-        fetch(0, lds);
-        put(lds);
+    auto barrier = [&]() {
+        if constexpr (DIRECT) vo_lds_barrier();
+        else __syncthreads();
+    };
+    // While one half of a slab is multiplied the operands of the next half are read from LDS.  The barrier sits between the
+    // halves: there slab s has been read to its end by all waves (its buffer takes slab s + 2) and slab s + 1 has arrived.
+    fetch(0, lds);
+    put(lds);
+    if (slabs > 1) {
+        fetch(1, lds + SLAB);
+        put(lds + SLAB);
     }
-    for (int s = 0; s < slabs; ++s) {
+    if (!DIRECT && slabs > 2) fetch(2, nullptr);
+    barrier();
+    read(f0, lds, 0);
+    for (int s = 0; s + 1 < slabs; ++s) {
         unsigned char* now = lds + (s & 1) * SLAB;
         unsigned char* next = lds + (1 - (s & 1)) * SLAB;
-        __syncthreads();                                             // slab s has arrived, slab s - 1 has been read
-        if (s + 1 < slabs) fetch(s + 1, next);
-        compute(now);
-        if (s + 1 < slabs) put(next);
+        read(f1, now, 1);
+        multiply(f0);
+        interleave();
+        barrier();
+        if constexpr (DIRECT) {
+            if (s + 2 < slabs) fetch(s + 2, now);
+        } else {
+            if (s + 2 < slabs) put(now);
+            if (s + 3 < slabs) fetch(s + 3, nullptr);
+        }
+        read(f0, next, 0);
+        multiply(f1);
+        interleave();
     }
-    __syncthreads();
+    read(f1, lds + ((slabs - 1) & 1) * SLAB, 1);
+    multiply(f0);
+    interleave();
+    multiply(f1);
 
     // store: sixteen rows at a time through a strip of LDS of the wave's own, so that rows leave in 16-byte pieces.  The
     // loop stays rolled (the epilogue's code is long) and the sums move down one place per round, because a register
-    // array with a running index would live in memory.
+    // array with a running index would live in memory.  The residual's pieces are fetched a round ahead.
     float* strip = reinterpret_cast<float*>(lds) + wave * 16 * STRIP;
-    constexpr int ACROSS = TN / PER;                                 // 16-byte pieces per row
+    constexpr int ACROSS = TN / PER, PIECES = 16 * ACROSS / 64;      // 16-byte pieces per row, and per lane and round
+    static_assert(64 % ACROSS == 0, "a lane keeps to its columns");
+    const int col = lane % ACROSS * PER, k = n0 + wn * TN + col;
+    const int64_t m_first = m0 + wm * TM + lane / ACROSS;
+    constexpr int STEP = 64 / ACROSS;                                // rows between a lane's pieces
+    float bias[PER];
+    Piece<T> ahead[PIECES];
+    Piece<T>::load_bias(a, k, bias);
+#pragma unroll
+    for (int p = 0; p < PIECES; ++p) ahead[p].load_residual(a, m_first + p * STEP, k);
+    __syncthreads();
 #pragma unroll 1
     for (int j = 0; j < MT; ++j) {
 #pragma unroll
@@ -203,20 +257,24 @@ __global__ __launch_bounds__(64 * WGM * WGN) void linear_tiles(const LinArgs a) 
         for (int i = 0; i < NT; ++i)
 #pragma unroll
             for (int q = 0; q + 1 < MT; ++q) acc[i][q] = acc[i][q + 1];
+        Piece<T> now[PIECES];
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p) {
+            now[p] = ahead[p];
+            if (j + 1 < MT) ahead[p].load_residual(a, m_first + (j + 1) * 16 + p * STEP, k);
+        }
         vo_wave_lds_fence();
-#pragma unroll 1
-        for (int p = 0; p < 16 * ACROSS / 64; ++p) {
-            const int piece = p * 64 + lane, r = piece / ACROSS, k = piece % ACROSS * PER;
-            const int64_t m = m0 + wm * TM + j * 16 + r;
-            const int kg = n0 + wn * TN + k;
-            if (m < a.M && kg < a.K) {
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p) {
+            const int64_t m = m_first + j * 16 + p * STEP;
+            if (m < a.M && k < a.K) {
                 float v[PER];
 #pragma unroll
                 for (int q = 0; q < PER; q += 4) {
-                    const vo_f32x4 t = *reinterpret_cast<const vo_f32x4*>(strip + r * STRIP + k + q);
+                    const vo_f32x4 t = *reinterpret_cast<const vo_f32x4*>(strip + (lane / ACROSS + p * STEP) * STRIP + col + q);
                     v[q] = t[0]; v[q + 1] = t[1]; v[q + 2] = t[2]; v[q + 3] = t[3];
                 }
-                emit<T>(a, split, m, kg, v);
+                now[p].emit(a, split, m, k, v, bias);
             }
         }
         vo_wave_lds_fence();
@@ -267,38 +325,56 @@ __global__ __launch_bounds__(512) void linear_rows(const LinArgs a) {
             return vo_load_unaligned<T>(w + (int64_t)(i * 16 + fr) * a.C + c + fg * PER, i * 16 + fr < rows_w ? c_hi - c - fg * PER : 0);
     };
     vo_f32x4 acc[WT][XT] = {};
-    constexpr int DEPTH = WT == 1 ? 8 : 4;                            // steps in flight
-    for (int c = c_lo; c < c_hi; c += DEPTH * STEP) {
-        vo_u32x4 wf[DEPTH][WT], xf[DEPTH][XT];
+    // DEPTH steps of loads are issued together, the next ones before this batch is multiplied
+    constexpr int DEPTH = XT == 1 ? 8 : XT == 2 ? 4 : 3;
+    struct Batch { vo_u32x4 w[DEPTH][WT], x[DEPTH][XT]; };
+    auto load = [&](Batch& b, int c) {
 #pragma unroll
         for (int d = 0; d < DEPTH; ++d) {
 #pragma unroll
-            for (int i = 0; i < WT; ++i) wf[d][i] = load_w(i, c + d * STEP);
+            for (int i = 0; i < WT; ++i) b.w[d][i] = load_w(i, c + d * STEP);
 #pragma unroll
-            for (int i = 0; i < XT; ++i) xf[d][i] = load_x(i, c + d * STEP);
+            for (int i = 0; i < XT; ++i) b.x[d][i] = load_x(i, c + d * STEP);
         }
+    };
+    auto multiply = [&](const Batch& b) {
 #pragma unroll
         for (int d = 0; d < DEPTH; ++d)
 #pragma unroll
             for (int i = 0; i < WT; ++i)
 #pragma unroll
-                for (int j = 0; j < XT; ++j) acc[i][j] = vo_elem<T>::mma16(wf[d][i], xf[d][j], acc[i][j]);
+                for (int j = 0; j < XT; ++j) acc[i][j] = vo_elem<T>::mma16(b.w[d][i], b.x[d][j], acc[i][j]);
+    };
+    Batch b0, b1;
+    load(b0, c_lo);
+    for (int c = c_lo; c < c_hi; c += 2 * DEPTH * STEP) {
+        load(b1, c + DEPTH * STEP);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(b0);
+        __builtin_amdgcn_sched_barrier(0);
+        if (c + 2 * DEPTH * STEP < c_hi) load(b0, c + 2 * DEPTH * STEP);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(b1);
+        __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
     for (int j = 0; j < XT; ++j)
 #pragma unroll
         for (int i = 0; i < WT; ++i) *reinterpret_cast<vo_f32x4*>(&sums[wave][j * 16 + fr][i * 16 + fg * 4]) = acc[i][j];
-    __syncthreads();
     constexpr int ACROSS = WT * 16 / PER;
+    __syncthreads();
     for (int piece = threadIdx.x; piece < XT * 16 * ACROSS; piece += 512) {
         const int r = piece / ACROSS, k = piece % ACROSS * PER;
         if (r >= a.M || n0 + k >= a.K) continue;
-        float v[PER] = {};
+        Piece<T> p;
+        float v[PER] = {}, bias[PER];
+        p.load_residual(a, r, n0 + k);
+        Piece<T>::load_bias(a, n0 + k, bias);
 #pragma unroll
         for (int s = 0; s < NW; ++s)
 #pragma unroll
             for (int q = 0; q < PER; ++q) v[q] += sums[s][r][k + q];
-        emit<T>(a, split, r, n0 + k, v);
+        p.emit(a, split, r, n0 + k, v, bias);
     }
 }
 
@@ -309,13 +385,25 @@ template <typename T> __global__ __launch_bounds__(256) void linear_join(const L
     if (piece >= a.M * across) return;
     const int64_t m = piece / across;
     const int k = (int)(piece % across) * PER;
-    float v[PER] = {};
+    Piece<T> piece_of;
+    float v[PER] = {}, bias[PER];
+    piece_of.load_residual(a, m, k);
+    Piece<T>::load_bias(a, k, bias);
+    const bool wide = (a.K & 3) == 0 && k + PER <= a.K;
     for (int s = 0; s < a.splits; ++s) {
         const float* p = a.part + ((int64_t)s * a.M + m) * a.K + k;
+        if (wide) {
 #pragma unroll
-        for (int j = 0; j < PER; ++j) v[j] += k + j < a.K ? p[j] : 0.f;
+            for (int j = 0; j < PER; j += 4) {
+                const vo_f32x4 t = *reinterpret_cast<const vo_f32x4*>(p + j);
+                v[j] += t[0]; v[j + 1] += t[1]; v[j + 2] += t[2]; v[j + 3] += t[3];
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < PER; ++j) v[j] += k + j < a.K ? p[j] : 0.f;
+        }
     }
-    finish<T>(a, m, k, v);
+    piece_of.finish(a, m, k, v, bias);
 }
 
 // ------------------------------------------------------------------------------------------------------------- host
@@ -369,7 +457,7 @@ template <typename T, bool DIRECT> int launch(const LinArgs& a, const Plan& p, h
     } else if (p.form == 2) {
         linear_tiles<T, 128, 128, 2, 2, DIRECT><<<grid, 256, 0, st>>>(a);
     } else {
-        if constexpr (sizeof(T) == 2) linear_tiles<T, 256, 256, 2, 4, DIRECT><<<grid, 512, 0, st>>>(a);
+        if constexpr (sizeof(T) == 2 && DIRECT) linear_tiles<T, 256, 256, 2, 4, DIRECT><<<grid, 512, 0, st>>>(a);
     }
     VO_CHECK_LAUNCH("vo_linear");
     if (p.splits > 1) {
@@ -380,10 +468,15 @@ template <typename T, bool DIRECT> int launch(const LinArgs& a, const Plan& p, h
     return VO_OK;
 }
 
-template <typename T> int dispatch(const LinArgs& a, const Plan& p, hipStream_t st) {
+template <typename T> int dispatch(LinArgs a, Plan p, hipStream_t st) {
     const size_t es = sizeof(T);
     const bool direct = (a.C * es) % 16 == 0 && (a.xs * es) % 16 == 0 && reinterpret_cast<uintptr_t>(a.x) % 16 == 0 &&
                         reinterpret_cast<uintptr_t>(a.w) % 16 == 0;
+    if (!direct && p.form == 3) {                                    // registers for staging leave room for half the tile
+        p.form = 2;
+        a.tiles_m = (unsigned)(p.tiles_m = vo_ceil_div(a.M, 128));
+        a.tiles_n = (unsigned)(p.tiles_n = vo_ceil_div(a.K, 128));
+    }
     return direct ? launch<T, true>(a, p, st) : launch<T, false>(a, p, st);
 }
 
@@ -410,7 +503,7 @@ extern "C" int vo_linear(const void* x, int64_t x_row_stride, const void* weight
     // a tile's rows are addressed with 32-bit offsets
     if (x_row_stride * es * 256 >= (1ll << 31) || (int64_t)C * es * 256 >= (1ll << 31))
         return vo_fail(VO_ERR_UNSUPPORTED, "vo_linear: rows of x and weight must be under 8 MiB");
-    if (p.tiles_m * p.tiles_n * p.splits >= (1ll << 31) || M * vo_ceil_div(K, 4) >= (1ll << 38))
+    if (p.tiles_m * p.tiles_n * p.splits * 4 >= (1ll << 31) || M * vo_ceil_div(K, 4) >= (1ll << 38))
         return vo_fail(VO_ERR_UNSUPPORTED, "vo_linear: M=%lld K=%d is too large for one launch", (long long)M, K);
     const int64_t need = p.splits > 1 ? (int64_t)p.splits * M * K * 4 : 0;
     VO_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && reinterpret_cast<uintptr_t>(workspace) % 16 == 0),

@@ -113,6 +113,13 @@ static __device__ __forceinline__ void vo_load_to_lds(__amdgpu_buffer_rsrc_t rs,
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)lds, 16, offset, 0, 0, 0);
 }
 
+// Waits for this wave's loads into LDS, then for the workgroup.  The wait is spelled out because the compiler's own barrier
+// does not count loads into LDS in every loop (results of another wave's load were read too early without it).
+static __device__ __forceinline__ void vo_lds_barrier() {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+}
+
 // `n` (< PER) or all PER elements of a row from any address: a wide load that needs no alignment, or element by element at
 // a row's end.  Missing elements are zero.
 template <typename T> static __device__ __forceinline__ vo_u32x4 vo_load_unaligned(const T* p, int64_t n) {

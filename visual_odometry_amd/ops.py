@@ -9,6 +9,7 @@ CPU tensor: there is deliberately no fallback path.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import numpy as np
 import torch
@@ -1099,33 +1100,37 @@ def _token_tensor(t, name: str, like: torch.Tensor | None = None) -> torch.Tenso
     """A GPU tensor of a token-major type (of ``like``'s type and device)."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError(f"{name}: expected a GPU tensor (the HIP backend has no CPU path)")
-    if t.dtype not in _TOKEN_DTYPES:
-        raise ValueError(f"{name}: expected float32, float16 or bfloat16, got {t.dtype}")
-    if like is not None and t.dtype != like.dtype:
+    if like is None:
+        if t.dtype not in _TOKEN_DTYPES:
+            raise ValueError(f"{name}: expected float32, float16 or bfloat16, got {t.dtype}")
+    elif t.dtype != like.dtype:
         raise ValueError(f"{name}: dtype {t.dtype} differs from {like.dtype}")
-    if like is not None and t.device != like.device:
+    elif t.device != like.device:
         raise ValueError(f"{name}: on {t.device}, the other tensors on {like.device}")
     return t
 
 
 def _rows(t: torch.Tensor, name: str, width: int):
     """(..., width) whose leading axes collapse to rows one stride apart -> (ptr, rows, row stride in elements)."""
-    if t.dim() < 1 or t.shape[-1] != width:
-        raise ValueError(f"{name}: expected rows of {width}, got shape {tuple(t.shape)}")
-    m = t.numel() // width
-    if m <= 1:
-        stride = width
-    else:
+    shape, st = t.shape, t.stride()
+    if not shape or shape[-1] != width:
+        raise ValueError(f"{name}: expected rows of {width}, got shape {tuple(shape)}")
+    if len(shape) != 2 and t.numel() > width:
         try:
-            flat = t.view(m, width)
+            flat = t.view(-1, width)
         except RuntimeError:
-            raise ValueError(f"{name}: the leading axes do not collapse to evenly spaced rows (strides {t.stride()})") from None
-        stride = flat.stride(0)
-    if width > 1 and m > 0 and t.stride(-1) != 1:
-        raise ValueError(f"{name}: a row's elements must be consecutive (got strides {t.stride()})")
-    if m > 1 and stride < width:
-        raise ValueError(f"{name}: rows overlap (got strides {t.stride()})")
-    return t.data_ptr(), m, stride
+            raise ValueError(f"{name}: the leading axes do not collapse to evenly spaced rows (strides {st})") from None
+        shape, st = flat.shape, flat.stride()
+    m = shape[0] if len(shape) == 2 else t.numel() // width
+    if m == 0:
+        return 0, 0, width
+    if width > 1 and st[-1] != 1:
+        raise ValueError(f"{name}: a row's elements must be consecutive (got strides {st})")
+    if m == 1:
+        return t.data_ptr(), 1, width
+    if st[0] < width:
+        raise ValueError(f"{name}: rows overlap (got strides {st})")
+    return t.data_ptr(), m, st[0]
 
 
 def _span(t: torch.Tensor):
@@ -1142,6 +1147,23 @@ def _no_overlap(out: torch.Tensor, t: torch.Tensor | None, name: str) -> None:
         raise ValueError(f"out overlaps {name} in memory")
 
 
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(query: str, *sizes) -> int:
+    """What a size query of the library answers; it depends on its arguments alone."""
+    return int(getattr(_lib.load(), query)(*sizes))
+
+
+def _call_on(device: torch.device, name: str, args, need: int, nbytes: int, flops: int = 0) -> None:
+    """_call on ``device`` (which need not be the current one) and its current stream, with ``need`` bytes of workspace
+    from the caching allocator; the entry point's last three arguments are workspace, its size and the stream."""
+    index = device.index
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _call_on(device, name, args, need, nbytes, flops)
+    work = torch.empty((need,), device=device, dtype=torch.uint8) if need else None
+    _call(name, *args, 0 if work is None else work.data_ptr(), need, torch._C._cuda_getCurrentRawStream(index), nbytes=nbytes, flops=flops)
+
+
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, activation: str | None = None,
            residual: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """act(x W^T + bias) + residual for rows x (..., C) and weight (K, C) -> (..., K).
@@ -1153,7 +1175,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     it must not overlap anything else.  Sums are formed in a fixed order: equal inputs give equal bits."""
     _token_tensor(x, "x")
     _token_tensor(weight, "weight", x)
-    if weight.dim() != 2 or not weight.is_contiguous() or weight.shape[0] < 1 or weight.shape[1] < 1:
+    if weight.dim() != 2 or not weight.is_contiguous() or weight.numel() == 0:
         raise ValueError("weight must be a contiguous (K,C)")
     K, C = weight.shape
     if activation not in ACTIVATIONS:
@@ -1161,42 +1183,42 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     if bias is not None and (bias.numel() != K or bias.device != x.device):
         raise ValueError("bias must have one entry per output, on x's device")
     px, M, xs = _rows(x, "x", C)
-    shape = tuple(x.shape[:-1]) + (K,)
+    shape = x.shape[:-1] + (K,)
     pr = rs = 0
     if residual is not None:
-        if tuple(_token_tensor(residual, "residual", x).shape) != shape:
-            raise ValueError(f"residual must be {shape}, got {tuple(residual.shape)}")
+        if _token_tensor(residual, "residual", x).shape != shape:
+            raise ValueError(f"residual must be {tuple(shape)}, got {tuple(residual.shape)}")
         pr, _, rs = _rows(residual, "residual", K)
     if out is None:
         out = torch.empty(shape, device=x.device, dtype=x.dtype)
         py, ys = out.data_ptr(), K
     else:
-        if tuple(_token_tensor(out, "out", x).shape) != shape:
-            raise ValueError(f"out must be {shape}, got {tuple(out.shape)}")
+        if _token_tensor(out, "out", x).shape != shape:
+            raise ValueError(f"out must be {tuple(shape)}, got {tuple(out.shape)}")
         py, _, ys = _rows(out, "out", K)
         for t, name in ((x, "x"), (weight, "weight"), (bias, "bias")):
             _no_overlap(out, t, name)
         if residual is not None and (py, ys) != (pr, rs):
             _no_overlap(out, residual, "residual (other than as the same tensor)")
     dt, es = _TOKEN_DTYPES[x.dtype], x.element_size()
-    with torch.cuda.device(x.device):
-        need = int(_lib.load().vo_linear_workspace_bytes(M, C, K, dt))
-        work = torch.empty((need,), device=x.device, dtype=torch.uint8) if need else None
-        _call("vo_linear", px, xs, weight.data_ptr(), _opt(bias, "bias", torch.float32), pr, rs, py, ys, M, C, K,
-              ACTIVATIONS[activation], dt, 0 if work is None else work.data_ptr(), need, _stream(),
-              nbytes=es * (M * C + K * C + M * K * (1 + (residual is not None))), flops=2 * M * C * K)
+    _call_on(x.device, "vo_linear",
+             (px, xs, weight.data_ptr(), _opt(bias, "bias", torch.float32), pr, rs, py, ys, M, C, K, ACTIVATIONS[activation], dt),
+             _workspace_bytes("vo_linear_workspace_bytes", M, C, K, dt),
+             es * (M * C + K * C + M * K * (1 + (residual is not None))), 2 * M * C * K)
     return out
 
 
 def _heads(t: torch.Tensor, name: str):
-    """(tokens, heads, D) with D consecutive -> (ptr, token stride, head stride) in elements."""
-    if t.dim() != 3 or t.shape[1] < 1 or t.shape[2] < 1:
+    """(tokens, heads, D) with D consecutive -> (token stride, head stride) in elements."""
+    if t.dim() != 3:
         raise ValueError(f"{name} must be (tokens, heads, D), got {tuple(t.shape)}")
+    n, h, d = t.shape
     st = t.stride()
-    if t.shape[2] > 1 and st[2] != 1:
+    if h < 1 or d < 1:
+        raise ValueError(f"{name} must be (tokens, heads, D), got {tuple(t.shape)}")
+    if d > 1 and st[2] != 1:
         raise ValueError(f"{name}: a head's elements must be consecutive (got strides {st})")
-    D = t.shape[2]
-    return t.data_ptr(), (st[0] if t.shape[0] > 1 else t.shape[1] * D), (st[1] if t.shape[1] > 1 else D)
+    return (st[0] if n > 1 else h * d), (st[1] if h > 1 else d)
 
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: torch.Tensor | None = None,
@@ -1215,12 +1237,12 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: torc
     _token_tensor(q, "q")
     _token_tensor(k, "k", q)
     _token_tensor(v, "v", q)
-    pq, qs, qh = _heads(q, "q")
-    pk, ks, kh = _heads(k, "k")
-    pv, vs, vh = _heads(v, "v")
+    qs, qh = _heads(q, "q")
+    ks, kh = _heads(k, "k")
+    vs, vh = _heads(v, "v")
     Tq, Hq, D = q.shape
-    Tk, Hk, _ = k.shape
-    if v.shape != k.shape or k.shape[2] != D:
+    Tk, Hk, Dk = k.shape
+    if v.shape != k.shape or Dk != D:
         raise ValueError(f"k and v must be (Tk,Hk,{D}), got {tuple(k.shape)} and {tuple(v.shape)}")
     if Hq % Hk:
         raise ValueError(f"{Hq} heads are no multiple of {Hk} key heads")
@@ -1228,33 +1250,31 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: torc
         if Tq != Tk:
             raise ValueError("q_offsets alone serves for both only when q and k have as many tokens")
         k_offsets = q_offsets
-    if (q_offsets is None) != (k_offsets is None):
-        raise ValueError("k_offsets needs q_offsets")
-    sequences = 1
-    if q_offsets is not None:
-        for t, n in ((q_offsets, "q_offsets"), (k_offsets, "k_offsets")):
-            _dev(t, n, torch.int32)
-            if t.dim() != 1 or t.numel() < 2 or t.numel() != q_offsets.numel() or t.device != q.device:
-                raise ValueError(f"{n} must be (sequences + 1) on q's device, as many as q_offsets")
+    sequences, pqo, pko = 1, 0, 0
+    if k_offsets is not None:
+        if q_offsets is None:
+            raise ValueError("k_offsets needs q_offsets")
+        pqo, pko = _dev(q_offsets, "q_offsets", torch.int32), _dev(k_offsets, "k_offsets", torch.int32)
         sequences = q_offsets.numel() - 1
-    scale = D ** -0.5 if scale is None else float(scale)
+        if (sequences < 1 or q_offsets.dim() != 1 or k_offsets.shape != q_offsets.shape or q_offsets.device != q.device
+                or k_offsets.device != q.device):
+            raise ValueError("q_offsets and k_offsets must both be (sequences + 1), as many as each other, on q's device")
     if out is None:
         out = torch.empty((Tq, Hq, D), device=q.device, dtype=q.dtype)
-    elif tuple(_token_tensor(out, "out", q).shape) != (Tq, Hq, D):
+        os_, oh = Hq * D, D
+    elif _token_tensor(out, "out", q).shape != q.shape:
         raise ValueError(f"out must be {(Tq, Hq, D)}, got {tuple(out.shape)}")
     else:
-        if any(s <= 0 for n, s in zip(out.shape, out.stride()) if n > 1):
-            raise ValueError(f"out: elements overlap (got strides {out.stride()})")
+        os_, oh = _heads(out, "out")
+        if (Tq > 1 and os_ < D) or (Hq > 1 and oh < D) or (Tq > 1 and Hq > 1 and os_ < Hq * oh and oh < Tq * os_):
+            raise ValueError(f"out: elements overlap or interleave (got strides {out.stride()})")
         for t, n in ((q, "q"), (k, "k"), (v, "v")):
             _no_overlap(out, t, n)
-    po, os_, oh = _heads(out, "out")
-    with torch.cuda.device(q.device):
-        need = int(_lib.load().vo_attention_workspace_bytes(Tq, Tk, sequences, Hq, Hk, D))
-        work = torch.empty((need,), device=q.device, dtype=torch.uint8) if need else None
-        _call("vo_attention", pq, qs, qh, pk, ks, kh, pv, vs, vh, po, os_, oh,
-              0 if q_offsets is None else q_offsets.data_ptr(), 0 if k_offsets is None else k_offsets.data_ptr(), sequences, Tq, Tk,
-              Hq, Hk, D, scale, int(bool(causal)), _TOKEN_DTYPES[q.dtype], 0 if work is None else work.data_ptr(), need, _stream(),
-              nbytes=q.element_size() * D * (2 * Tq * Hq + 2 * Tk * Hk))
+    _call_on(q.device, "vo_attention",
+             (q.data_ptr(), qs, qh, k.data_ptr(), ks, kh, v.data_ptr(), vs, vh, out.data_ptr(), os_, oh, pqo, pko, sequences, Tq, Tk, Hq, Hk,
+              D, D ** -0.5 if scale is None else float(scale), 1 if causal else 0, _TOKEN_DTYPES[q.dtype]),
+             _workspace_bytes("vo_attention_workspace_bytes", Tq, Tk, sequences, Hq, Hk, D),
+             q.element_size() * D * (2 * Tq * Hq + 2 * Tk * Hk))
     return out
 
 
