@@ -93,7 +93,8 @@ template <typename T, int DT, int KEYS> struct Core {
 #pragma unroll
             for (int i = 0; i < QS; ++i) {
                 const vo_u32x4 kf = *reinterpret_cast<const vo_u32x4*>(kt + r * L::ROW + (((i * 2 + half) ^ L::k_swz(r)) * 16));
-                acc = E::mma32(kf, q[i], acc);
+#pragma unroll
+                for (int part = 0; part < E::PARTS; ++part) acc = E::mma32(kf, q[i], acc, part);
             }
             s[b] = acc;
         }
@@ -148,7 +149,7 @@ template <typename T, int DT, int KEYS> struct Core {
                         const int at = (lane & 1) * 8;
                         const vo_u32x2 lo = transposed(vt + r * L::ROW + ((chunk ^ L::v_swz(r)) * 16) + at);
                         const vo_u32x2 hi = transposed(vt + (r + 8) * L::ROW + ((chunk ^ L::v_swz(r + 8)) * 16) + at);
-                        o[d] = E::mma32(vo_u32x4{lo[0], lo[1], hi[0], hi[1]}, pf, o[d]);
+                        o[d] = E::mma32(vo_u32x4{lo[0], lo[1], hi[0], hi[1]}, pf, o[d], 0);
                     }
                 }
             } else {

@@ -93,19 +93,26 @@ template <typename T> struct Piece {
 };
 
 // ------------------------------------------------------------------------------------------------------------ tiles
+__device__ __forceinline__ int swizzle(int row) { return (row >> 1) & 7; }
+template <int SIDE> struct Sums { using type = vo_f32x4; };
+template <> struct Sums<32> { using type = vo_f32x16; };
+
 // WGM x WGN waves; a wave owns TM rows of x times TN outputs as 16x16 products with W as the first operand, so that a lane
-// holds four consecutive outputs of one row.  LDS rows are 128 bytes (eight chunks); chunk c of row r sits at c ^ (r % 8),
-// which spreads the 16-byte reads of eight rows over all banks.  The permutation is applied to the addresses the lanes
+// holds four consecutive outputs of one row.  LDS rows are 128 bytes (eight chunks); chunk c of row r sits at
+// c ^ (r / 2 % 8), which spreads the 16-byte reads of sixteen rows over all 64 banks (r % 8 in its place: half of the LDS cycles
+// were conflicts).  The permutation is applied to the addresses the lanes
 // fetch, because a load into LDS places lane l's bytes at position l.
-template <typename T, int BM, int BN, int WGM, int WGN, bool DIRECT>
+template <typename T, int BM, int BN, int WGM, int WGN, int SIDE, int STAGES, bool DIRECT>
 __global__ __launch_bounds__(64 * WGM * WGN) void linear_tiles(const LinArgs a) {
     constexpr int PER = vo_elem<T>::PER, BK = 8 * PER, NW = WGM * WGN;
-    constexpr int TM = BM / WGM, TN = BN / WGN, MT = TM / 16, NT = TN / 16;
+    constexpr int TM = BM / WGM, TN = BN / WGN, MT = TM / SIDE, NT = TN / SIDE;
+    constexpr int GROUPS = 64 / SIDE, KK = 4 / GROUPS;               // lane groups; products along half a slab
     constexpr int ROWS = BM + BN, LOADS = ROWS / 8 / NW;             // 1 KiB wave loads (8 rows) per wave and slab
     constexpr int STRIP = TN + 4;                                    // floats per row of the store's staging strip
-    constexpr int SLAB = ROWS * 128, STAGE = NW * 16 * STRIP * 4;
+    constexpr int SLAB = ROWS * 128, STAGE = NW * SIDE * STRIP * 4;
     static_assert(ROWS % (8 * NW) == 0 && BM % (8 * NW) == 0, "a wave's loads must not straddle the operands");
-    __shared__ __align__(16) unsigned char lds[2 * SLAB > STAGE ? 2 * SLAB : STAGE];
+    static_assert(DIRECT || STAGES == 2, "registers hold one more slab");
+    __shared__ __align__(16) unsigned char lds[STAGES * SLAB > STAGE ? STAGES * SLAB : STAGE];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // tile order: splits outermost, then bands of 8 row tiles, within a band column by column
@@ -128,34 +135,34 @@ __global__ __launch_bounds__(64 * WGM * WGN) void linear_tiles(const LinArgs a) 
     const __amdgpu_buffer_rsrc_t xrs = vo_buffer(xt, (rows_x - 1) * xb + wb);
     const __amdgpu_buffer_rsrc_t wrs = vo_buffer(wt, rows_w * wb);
 
-    const int sub = lane >> 3, chunk = (lane & 7) ^ sub;             // this lane's row of eight and the chunk it fetches
+    const int sub = lane >> 3;                                       // this lane's row of a load's eight
     auto is_x = [&](int i) { return i < LOADS * BM / ROWS; };        // loads 0.. of a wave fetch x, the rest W
     auto tile_row = [&](int i) {                                     // first of the eight rows of load i, within its operand
         constexpr int XL = LOADS * BM / ROWS;
         return is_x(i) ? (wave * XL + i) * 8 : (wave * (LOADS - XL) + i - XL) * 8;
     };
+    auto chunk = [&](int i) { return (lane & 7) ^ swizzle(tile_row(i) + sub); };             // the chunk it fetches
     unsigned off[LOADS];
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
         const int r = tile_row(i) + sub;
         const bool in = r < (is_x(i) ? rows_x : rows_w);
-        off[i] = in ? (unsigned)(r * (is_x(i) ? xb : wb) + chunk * 16) : VO_OUTSIDE;
+        off[i] = in ? (unsigned)(r * (is_x(i) ? xb : wb) + chunk(i) * 16) : VO_OUTSIDE;
     }
     vo_u32x4 reg[DIRECT ? 1 : LOADS];
     auto fetch = [&](int s, unsigned char* buf) {
         const int c0 = c_first + s * BK;
         if constexpr (DIRECT) {
-            const bool inside = c0 + chunk * PER < c_last;           // whole chunks: C is a multiple of PER
 #pragma unroll
-            for (int i = 0; i < LOADS; ++i)
+            for (int i = 0; i < LOADS; ++i)                          // whole chunks: C is a multiple of PER
                 vo_load_to_lds(is_x(i) ? xrs : wrs, buf + (is_x(i) ? 0 : BM * 128) + tile_row(i) * 128,
-                               inside ? off[i] + c0 * (unsigned)sizeof(T) : VO_OUTSIDE);
+                               c0 + chunk(i) * PER < c_last ? off[i] + c0 * (unsigned)sizeof(T) : VO_OUTSIDE);
         } else {
 #pragma unroll
             for (int i = 0; i < LOADS; ++i) {
                 const int r = tile_row(i) + sub;
                 const bool in = r < (is_x(i) ? rows_x : rows_w);
-                const int c = c0 + chunk * PER;
+                const int c = c0 + chunk(i) * PER;
                 const T* p = (is_x(i) ? xt + r * a.xs : wt + (int64_t)r * a.C) + c;
                 reg[i] = vo_load_unaligned<T>(p, in ? c_last - c : 0);
             }
@@ -170,75 +177,91 @@ __global__ __launch_bounds__(64 * WGM * WGN) void linear_tiles(const LinArgs a) 
     };
 
     const int wm = wave / WGN, wn = wave % WGN;
-    vo_f32x4 acc[NT][MT] = {};
-    const int fr = lane & 15, fg = lane >> 4;
-    struct Frags { vo_u32x4 w[NT], x[MT]; } f0, f1;                  // operands of a slab's two halves
-    auto read = [&](Frags& f, const unsigned char* buf, int kk) {
-        const int pos = ((kk * 4 + fg) ^ (fr & 7)) * 16;
+    typename Sums<SIDE>::type acc[NT][MT] = {};
+    const int fr = lane % SIDE, fg = lane / SIDE;
+    struct Frags { vo_u32x4 w[NT][KK], x[MT][KK]; } f0, f1;          // operands of a slab's two halves
+    auto read = [&](Frags& f, const unsigned char* buf, int half) {
 #pragma unroll
-        for (int i = 0; i < NT; ++i) f.w[i] = *reinterpret_cast<const vo_u32x4*>(buf + (BM + wn * TN + i * 16 + fr) * 128 + pos);
+        for (int q = 0; q < KK; ++q) {
+            const int pos = ((half * 4 + q * GROUPS + fg) ^ swizzle(fr)) * 16;
 #pragma unroll
-        for (int i = 0; i < MT; ++i) f.x[i] = *reinterpret_cast<const vo_u32x4*>(buf + (wm * TM + i * 16 + fr) * 128 + pos);
+            for (int i = 0; i < NT; ++i) f.w[i][q] = *reinterpret_cast<const vo_u32x4*>(buf + (BM + wn * TN + i * SIDE + fr) * 128 + pos);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) f.x[i][q] = *reinterpret_cast<const vo_u32x4*>(buf + (wm * TM + i * SIDE + fr) * 128 + pos);
+        }
     };
     auto multiply = [&](const Frags& f) {
 #pragma unroll
-        for (int i = 0; i < NT; ++i)
+        for (int q = 0; q < KK; ++q)
 #pragma unroll
-            for (int j = 0; j < MT; ++j) acc[i][j] = vo_elem<T>::mma16(f.w[i], f.x[j], acc[i][j]);
+            for (int part = 0; part < vo_elem<T>::PARTS; ++part)
+#pragma unroll
+                for (int i = 0; i < NT; ++i)
+#pragma unroll
+                    for (int j = 0; j < MT; ++j) {
+                        if constexpr (SIDE == 32) acc[i][j] = vo_elem<T>::mma32(f.w[i][q], f.x[j][q], acc[i][j], part);
+                        else acc[i][j] = vo_elem<T>::mma16(f.w[i][q], f.x[j][q], acc[i][j], part);
+                    }
     };
     // one LDS read per few products, so that neither pipe waits for the other
     auto interleave = [&]() {
-        constexpr int PRODUCTS = NT * MT * (sizeof(T) == 4 ? 4 : 1), READS = NT + MT, EACH = PRODUCTS / READS;
+        constexpr int PRODUCTS = NT * MT * KK * vo_elem<T>::PARTS, READS = (NT + MT) * KK, EACH = PRODUCTS / READS > 0 ? PRODUCTS / READS : 1;
 #pragma unroll
         for (int i = 0; i < READS; ++i) {
             __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
             __builtin_amdgcn_sched_group_barrier(0x008, EACH, 0);
         }
-        __builtin_amdgcn_sched_group_barrier(0x008, PRODUCTS - READS * EACH, 0);
+        if constexpr (PRODUCTS > READS * EACH) __builtin_amdgcn_sched_group_barrier(0x008, PRODUCTS - READS * EACH, 0);
     };
 
-    auto barrier = [&]() {
-        if constexpr (DIRECT) vo_lds_barrier();
-        else __syncthreads();
-    };
     // While one half of a slab is multiplied the operands of the next half are read from LDS.  The barrier sits between the
-    // halves: there slab s has been read to its end by all waves (its buffer takes slab s + 2) and slab s + 1 has arrived.
-    fetch(0, lds);
-    put(lds);
-    if (slabs > 1) {
-        fetch(1, lds + SLAB);
-        put(lds + SLAB);
+    // halves: there slab s has been read to its end by all waves (its buffer takes slab s + STAGES) and slab s + 1 has
+    // arrived; the loads of the slabs behind that stay under way.  Slabs past the end are fetched too (as zeros, without
+    // any traffic), so that the number of loads under way is always the same.
+    unsigned char* buf = lds;                                        // of slab s
+    auto after = [&](unsigned char* p) { return p + SLAB == lds + STAGES * SLAB ? lds : p + SLAB; };
+    if constexpr (DIRECT) {
+#pragma unroll
+        for (int i = 0; i < STAGES; ++i) fetch(i, lds + i * SLAB);
+        vo_lds_barrier<(STAGES - 1) * LOADS>();
+    } else {
+        fetch(0, nullptr);
+        put(lds);
+        if (slabs > 1) {
+            fetch(1, nullptr);
+            put(lds + SLAB);
+        }
+        if (slabs > 2) fetch(2, nullptr);
+        __syncthreads();
     }
-    if (!DIRECT && slabs > 2) fetch(2, nullptr);
-    barrier();
-    read(f0, lds, 0);
+    read(f0, buf, 0);
     for (int s = 0; s + 1 < slabs; ++s) {
-        unsigned char* now = lds + (s & 1) * SLAB;
-        unsigned char* next = lds + (1 - (s & 1)) * SLAB;
-        read(f1, now, 1);
+        read(f1, buf, 1);
         multiply(f0);
         interleave();
-        barrier();
         if constexpr (DIRECT) {
-            if (s + 2 < slabs) fetch(s + 2, now);
+            vo_lds_barrier<(STAGES - 2) * LOADS>();
+            fetch(s + STAGES, buf);
         } else {
-            if (s + 2 < slabs) put(now);
+            __syncthreads();
+            if (s + 2 < slabs) put(buf);
             if (s + 3 < slabs) fetch(s + 3, nullptr);
         }
-        read(f0, next, 0);
+        buf = after(buf);
+        read(f0, buf, 0);
         multiply(f1);
         interleave();
     }
-    read(f1, lds + ((slabs - 1) & 1) * SLAB, 1);
+    read(f1, buf, 1);
     multiply(f0);
     interleave();
     multiply(f1);
 
-    // store: sixteen rows at a time through a strip of LDS of the wave's own, so that rows leave in 16-byte pieces.  The
+    // store: SIDE rows at a time through a strip of LDS of the wave's own, so that rows leave in 16-byte pieces.  The
     // loop stays rolled (the epilogue's code is long) and the sums move down one place per round, because a register
     // array with a running index would live in memory.  The residual's pieces are fetched a round ahead.
-    float* strip = reinterpret_cast<float*>(lds) + wave * 16 * STRIP;
-    constexpr int ACROSS = TN / PER, PIECES = 16 * ACROSS / 64;      // 16-byte pieces per row, and per lane and round
+    float* strip = reinterpret_cast<float*>(lds) + wave * SIDE * STRIP;
+    constexpr int ACROSS = TN / PER, PIECES = SIDE * ACROSS >= 64 ? SIDE * ACROSS / 64 : 1;   // 16-byte pieces per row; per lane and round
     static_assert(64 % ACROSS == 0, "a lane keeps to its columns");
     const int col = lane % ACROSS * PER, k = n0 + wn * TN + col;
     const int64_t m_first = m0 + wm * TM + lane / ACROSS;
@@ -248,11 +271,20 @@ __global__ __launch_bounds__(64 * WGM * WGN) void linear_tiles(const LinArgs a) 
     Piece<T>::load_bias(a, k, bias);
 #pragma unroll
     for (int p = 0; p < PIECES; ++p) ahead[p].load_residual(a, m_first + p * STEP, k);
-    __syncthreads();
+    vo_lds_barrier();
 #pragma unroll 1
     for (int j = 0; j < MT; ++j) {
 #pragma unroll
-        for (int i = 0; i < NT; ++i) *reinterpret_cast<vo_f32x4*>(strip + fr * STRIP + i * 16 + fg * 4) = acc[i][0];
+        for (int i = 0; i < NT; ++i) {
+            if constexpr (SIDE == 32) {
+#pragma unroll
+                for (int b = 0; b < 4; ++b)
+                    *reinterpret_cast<vo_f32x4*>(strip + fr * STRIP + i * 32 + b * 8 + fg * 4) =
+                        vo_f32x4{acc[i][0][4 * b], acc[i][0][4 * b + 1], acc[i][0][4 * b + 2], acc[i][0][4 * b + 3]};
+            } else {
+                *reinterpret_cast<vo_f32x4*>(strip + fr * STRIP + i * 16 + fg * 4) = acc[i][0];
+            }
+        }
 #pragma unroll
         for (int i = 0; i < NT; ++i)
 #pragma unroll
@@ -261,13 +293,13 @@ __global__ __launch_bounds__(64 * WGM * WGN) void linear_tiles(const LinArgs a) 
 #pragma unroll
         for (int p = 0; p < PIECES; ++p) {
             now[p] = ahead[p];
-            if (j + 1 < MT) ahead[p].load_residual(a, m_first + (j + 1) * 16 + p * STEP, k);
+            if (j + 1 < MT) ahead[p].load_residual(a, m_first + (j + 1) * SIDE + p * STEP, k);
         }
         vo_wave_lds_fence();
 #pragma unroll
         for (int p = 0; p < PIECES; ++p) {
-            const int64_t m = m_first + j * 16 + p * STEP;
-            if (m < a.M && k < a.K) {
+            const int64_t m = m_first + j * SIDE + p * STEP;
+            if (m < a.M && k < a.K && lane / ACROSS + p * STEP < SIDE) {
                 float v[PER];
 #pragma unroll
                 for (int q = 0; q < PER; q += 4) {
@@ -282,100 +314,67 @@ __global__ __launch_bounds__(64 * WGM * WGN) void linear_tiles(const LinArgs a) 
 }
 
 // ------------------------------------------------------------------------------------------------------------- rows
-// At most 16 * XT rows of x: a workgroup forms 16 * WT outputs for all of them, its eight waves each a part of C; W goes
-// from memory to registers once, the rows of x come from the caches.  The waves' sums are added in LDS in wave order.
-template <typename T, int XT, int WT, bool ALIGNED>
+// At most 16 rows of x: a workgroup forms 16 outputs for all of them, its eight waves each a part of C; W goes from memory
+// to registers once, the rows of x come from the caches.  The waves' sums are added in LDS in wave order.
+template <typename T, bool ALIGNED>
 __global__ __launch_bounds__(512) void linear_rows(const LinArgs a) {
     constexpr int PER = vo_elem<T>::PER, STEP = 4 * PER, NW = 8;     // one product covers STEP elements of C
-    __shared__ __align__(16) float sums[NW][XT * 16][WT * 16 + 4];
+    __shared__ __align__(16) float sums[NW][16][20];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int fr = lane & 15, fg = lane >> 4;
-    const unsigned groups = a.tiles_n;
-    const unsigned id = vo_xcd_contiguous(blockIdx.x, groups * a.splits);
-    const int split = id / groups, n0 = (int)(id % groups) * 16 * WT;
+    const unsigned id = vo_xcd_contiguous(blockIdx.x, a.tiles_n * a.splits);
+    const int split = id / a.tiles_n, n0 = (int)(id % a.tiles_n) * 16;
     const int c_first = split * a.c_per_split;
     const int c_last = a.C - c_first < a.c_per_split ? a.C : c_first + a.c_per_split;
     // parts of whole pairs of steps: 128 bytes of a row of W
-    const int part = (((c_last - c_first + 2 * STEP - 1) / (2 * STEP) + NW - 1) / NW) * 2 * STEP;
+    const int part = ((c_last - c_first + 2 * STEP - 1) / (2 * STEP) + NW - 1) / NW * 2 * STEP;
     const int c_lo = c_first + wave * part < c_last ? c_first + wave * part : c_last;
     const int c_hi = c_lo + part < c_last ? c_lo + part : c_last;
 
     const T* x = static_cast<const T*>(a.x);
     const T* w = static_cast<const T*>(a.w) + (int64_t)n0 * a.C;
     const int64_t xb = (int64_t)sizeof(T) * a.xs, wb = (int64_t)sizeof(T) * a.C;
-    const int rows_w = a.K - n0 < 16 * WT ? a.K - n0 : 16 * WT;
+    const int rows_w = a.K - n0 < 16 ? a.K - n0 : 16;
     const __amdgpu_buffer_rsrc_t xrs = vo_buffer(x, (a.M - 1) * xb + wb);
     const __amdgpu_buffer_rsrc_t wrs = vo_buffer(w, rows_w * wb);
-    unsigned xo[XT], wo[WT];
-#pragma unroll
-    for (int i = 0; i < XT; ++i) xo[i] = i * 16 + fr < a.M ? (unsigned)((i * 16 + fr) * xb) + fg * 16 : VO_OUTSIDE;
-#pragma unroll
-    for (int i = 0; i < WT; ++i) wo[i] = i * 16 + fr < rows_w ? (unsigned)((i * 16 + fr) * wb) + fg * 16 : VO_OUTSIDE;
+    const unsigned xo = fr < a.M ? (unsigned)(fr * xb) + fg * 16 : VO_OUTSIDE;
+    const unsigned wo = fr < rows_w ? (unsigned)(fr * wb) + fg * 16 : VO_OUTSIDE;
 
-    auto load_x = [&](int i, int c) -> vo_u32x4 {
-        if constexpr (ALIGNED)
-            return __builtin_amdgcn_raw_buffer_load_b128(xrs, c + fg * PER < c_hi ? xo[i] + c * (unsigned)sizeof(T) : VO_OUTSIDE, 0, 0);
-        else
-            return vo_load_unaligned<T>(x + (i * 16 + fr) * a.xs + c + fg * PER, i * 16 + fr < a.M ? c_hi - c - fg * PER : 0);
-    };
-    auto load_w = [&](int i, int c) -> vo_u32x4 {
-        if constexpr (ALIGNED)
-            return __builtin_amdgcn_raw_buffer_load_b128(wrs, c + fg * PER < c_hi ? wo[i] + c * (unsigned)sizeof(T) : VO_OUTSIDE, 0, 0);
-        else
-            return vo_load_unaligned<T>(w + (int64_t)(i * 16 + fr) * a.C + c + fg * PER, i * 16 + fr < rows_w ? c_hi - c - fg * PER : 0);
-    };
-    vo_f32x4 acc[WT][XT] = {};
-    // DEPTH steps of loads are issued together, the next ones before this batch is multiplied
-    constexpr int DEPTH = XT == 1 ? 8 : XT == 2 ? 4 : 3;
-    struct Batch { vo_u32x4 w[DEPTH][WT], x[DEPTH][XT]; };
-    auto load = [&](Batch& b, int c) {
+    constexpr int DEPTH = 8;                                         // steps whose loads are issued together
+    vo_f32x4 acc = {};
+    for (int first = c_lo; first < c_hi; first += DEPTH * STEP) {
+        vo_u32x4 wf[DEPTH], xf[DEPTH];
 #pragma unroll
         for (int d = 0; d < DEPTH; ++d) {
-#pragma unroll
-            for (int i = 0; i < WT; ++i) b.w[d][i] = load_w(i, c + d * STEP);
-#pragma unroll
-            for (int i = 0; i < XT; ++i) b.x[d][i] = load_x(i, c + d * STEP);
+            const int c = first + d * STEP + fg * PER;
+            if constexpr (ALIGNED) {
+                const unsigned at = (first + d * STEP) * (unsigned)sizeof(T);
+                wf[d] = __builtin_amdgcn_raw_buffer_load_b128(wrs, c < c_hi ? wo + at : VO_OUTSIDE, 0, 0);
+                xf[d] = __builtin_amdgcn_raw_buffer_load_b128(xrs, c < c_hi ? xo + at : VO_OUTSIDE, 0, 0);
+            } else {
+                wf[d] = vo_load_unaligned<T>(w + (int64_t)fr * a.C + c, fr < rows_w ? c_hi - c : 0);
+                xf[d] = vo_load_unaligned<T>(x + fr * a.xs + c, fr < a.M ? c_hi - c : 0);
+            }
         }
-    };
-    auto multiply = [&](const Batch& b) {
 #pragma unroll
         for (int d = 0; d < DEPTH; ++d)
 #pragma unroll
-            for (int i = 0; i < WT; ++i)
-#pragma unroll
-                for (int j = 0; j < XT; ++j) acc[i][j] = vo_elem<T>::mma16(b.w[d][i], b.x[d][j], acc[i][j]);
-    };
-    Batch b0, b1;
-    load(b0, c_lo);
-    for (int c = c_lo; c < c_hi; c += 2 * DEPTH * STEP) {
-        load(b1, c + DEPTH * STEP);
-        __builtin_amdgcn_sched_barrier(0);
-        multiply(b0);
-        __builtin_amdgcn_sched_barrier(0);
-        if (c + 2 * DEPTH * STEP < c_hi) load(b0, c + 2 * DEPTH * STEP);
-        __builtin_amdgcn_sched_barrier(0);
-        multiply(b1);
-        __builtin_amdgcn_sched_barrier(0);
+            for (int part = 0; part < vo_elem<T>::PARTS; ++part) acc = vo_elem<T>::mma16(wf[d], xf[d], acc, part);
     }
-#pragma unroll
-    for (int j = 0; j < XT; ++j)
-#pragma unroll
-        for (int i = 0; i < WT; ++i) *reinterpret_cast<vo_f32x4*>(&sums[wave][j * 16 + fr][i * 16 + fg * 4]) = acc[i][j];
-    constexpr int ACROSS = WT * 16 / PER;
+    *reinterpret_cast<vo_f32x4*>(&sums[wave][fr][fg * 4]) = acc;
     __syncthreads();
-    for (int piece = threadIdx.x; piece < XT * 16 * ACROSS; piece += 512) {
-        const int r = piece / ACROSS, k = piece % ACROSS * PER;
-        if (r >= a.M || n0 + k >= a.K) continue;
-        Piece<T> p;
-        float v[PER] = {}, bias[PER];
-        p.load_residual(a, r, n0 + k);
-        Piece<T>::load_bias(a, n0 + k, bias);
+    constexpr int ACROSS = 16 / PER;
+    const int r = threadIdx.x / ACROSS, k = threadIdx.x % ACROSS * PER;
+    if (r >= 16 || r >= a.M || n0 + k >= a.K) return;
+    Piece<T> p;
+    float v[PER] = {}, bias[PER];
+    p.load_residual(a, r, n0 + k);
+    Piece<T>::load_bias(a, n0 + k, bias);
 #pragma unroll
-        for (int s = 0; s < NW; ++s)
+    for (int s = 0; s < NW; ++s)
 #pragma unroll
-            for (int q = 0; q < PER; ++q) v[q] += sums[s][r][k + q];
-        p.emit(a, split, r, n0 + k, v, bias);
-    }
+        for (int q = 0; q < PER; ++q) v[q] += sums[s][r][k + q];
+    p.emit(a, split, r, n0 + k, v, bias);
 }
 
 // Adds the partial sums of one PER-wide piece in the order of the splits and finishes it.
@@ -408,57 +407,59 @@ template <typename T> __global__ __launch_bounds__(256) void linear_join(const L
 
 // ------------------------------------------------------------------------------------------------------------- host
 
+// Tiles: rows of x, outputs, and the rate at which a full machine works on them relative to the largest (16-bit, float32).
+struct Form { int bm, bn; float rate16, rate32; };
+constexpr Form FORMS[] = {{16, 16, 0, 0}, {32, 64, 0, 0}, {64, 64, 0.5f, 1.f}, {128, 128, 0.75f, 1.f}, {256, 256, 1.f, 0.f}};
+
 struct Plan {
-    int form;                        // 0: rows, 1: 64x64 tiles, 2: 128x128, 3: 256x256
+    int form;                        // of FORMS; 0: linear_rows
     int splits, c_per_split;
     int64_t tiles_m, tiles_n;
 };
 
 Plan plan(int64_t M, int C, int K, int dtype) {
-    const int per = dtype == VO_F32 ? 4 : 8, slab = 8 * per;
+    const int slab = dtype == VO_F32 ? 32 : 64;
     Plan p{};
-    if (M <= 64) {
-        p.form = 0;
-        p.tiles_m = 1;
-        p.tiles_n = vo_ceil_div(K, M <= 16 ? 16 : 32);
-    } else {
-        const int64_t big = vo_ceil_div(M, 256) * vo_ceil_div(K, 256), mid = vo_ceil_div(M, 128) * vo_ceil_div(K, 128);
-        p.form = big >= 224 && dtype != VO_F32 ? 3 : mid >= 192 ? 2 : 1;
-        const int t = p.form == 3 ? 256 : p.form == 2 ? 128 : 64;
-        p.tiles_m = vo_ceil_div(M, t);
-        p.tiles_n = vo_ceil_div(K, t);
+    if (M <= 16) p.form = 0;
+    else if (M <= 32) p.form = 1;
+    else {
+        // the tile whose rounds over the 256 CUs take least
+        float best = 0.f;
+        for (int f = 2; f <= 4; ++f) {
+            const float rate = dtype == VO_F32 ? FORMS[f].rate32 : FORMS[f].rate16;
+            if (rate == 0.f) continue;
+            const int64_t tiles = vo_ceil_div(M, FORMS[f].bm) * vo_ceil_div(K, FORMS[f].bn);
+            const float cost = (float)vo_ceil_div(tiles, 256) * FORMS[f].bm * FORMS[f].bn / rate;
+            if (p.form == 0 || cost < best) {
+                p.form = f;
+                best = cost;
+            }
+        }
     }
+    p.tiles_m = vo_ceil_div(M, FORMS[p.form].bm);
+    p.tiles_n = vo_ceil_div(K, FORMS[p.form].bn);
     const int64_t tiles = p.tiles_m * p.tiles_n;
     int64_t splits = 1;
     const int64_t at_least = p.form == 0 ? 1024 : 512;               // elements of C worth a split
     if (tiles < 192) {
-        splits = vo_ceil_div(384, tiles);
+        splits = vo_ceil_div(256, tiles);
         if (splits > C / at_least) splits = C / at_least;
         if (splits > 16) splits = 16;
         if (splits < 1) splits = 1;
     }
     p.c_per_split = (int)vo_ceil_div(vo_ceil_div(C, slab), splits) * slab;
-    if (p.c_per_split < slab) p.c_per_split = slab;
     p.splits = (int)vo_ceil_div(C, p.c_per_split);
-    if (p.splits < 1) p.splits = 1;
     return p;
 }
 
 template <typename T, bool DIRECT> int launch(const LinArgs& a, const Plan& p, hipStream_t st) {
     const dim3 grid((unsigned)(p.tiles_m * p.tiles_n * p.splits));
-    if (p.form == 0) {
-        const int xt = (int)vo_ceil_div(a.M, 16);
-        if (xt == 1) linear_rows<T, 1, 1, DIRECT><<<grid, 512, 0, st>>>(a);
-        else if (xt == 2) linear_rows<T, 2, 2, DIRECT><<<grid, 512, 0, st>>>(a);
-        else if (xt == 3) linear_rows<T, 3, 2, DIRECT><<<grid, 512, 0, st>>>(a);
-        else linear_rows<T, 4, 2, DIRECT><<<grid, 512, 0, st>>>(a);
-    } else if (p.form == 1) {
-        linear_tiles<T, 64, 64, 2, 2, DIRECT><<<grid, 256, 0, st>>>(a);
-    } else if (p.form == 2) {
-        linear_tiles<T, 128, 128, 2, 2, DIRECT><<<grid, 256, 0, st>>>(a);
-    } else {
-        if constexpr (sizeof(T) == 2 && DIRECT) linear_tiles<T, 256, 256, 2, 4, DIRECT><<<grid, 512, 0, st>>>(a);
-    }
+    constexpr int S32 = DIRECT ? 6 : 2, S64 = DIRECT ? 4 : 2;
+    if (p.form == 0) linear_rows<T, DIRECT><<<grid, 512, 0, st>>>(a);
+    else if (p.form == 1) linear_tiles<T, 32, 64, 1, 4, 16, S32, DIRECT><<<grid, 256, 0, st>>>(a);
+    else if (p.form == 2) linear_tiles<T, 64, 64, 2, 2, 16, S64, DIRECT><<<grid, 256, 0, st>>>(a);
+    else if (p.form == 3) linear_tiles<T, 128, 128, 2, 2, 16, 2, DIRECT><<<grid, 256, 0, st>>>(a);
+    else if constexpr (sizeof(T) == 2 && DIRECT) linear_tiles<T, 256, 256, 2, 4, 32, 2, DIRECT><<<grid, 512, 0, st>>>(a);
     VO_CHECK_LAUNCH("vo_linear");
     if (p.splits > 1) {
         const int64_t pieces = a.M * vo_ceil_div(a.K, vo_elem<T>::PER);
@@ -472,8 +473,8 @@ template <typename T> int dispatch(LinArgs a, Plan p, hipStream_t st) {
     const size_t es = sizeof(T);
     const bool direct = (a.C * es) % 16 == 0 && (a.xs * es) % 16 == 0 && reinterpret_cast<uintptr_t>(a.x) % 16 == 0 &&
                         reinterpret_cast<uintptr_t>(a.w) % 16 == 0;
-    if (!direct && p.form == 3) {                                    // registers for staging leave room for half the tile
-        p.form = 2;
+    if (!direct && p.form == 4) {                                    // registers for staging leave no room for the largest tile
+        p.form = 3;
         a.tiles_m = (unsigned)(p.tiles_m = vo_ceil_div(a.M, 128));
         a.tiles_n = (unsigned)(p.tiles_n = vo_ceil_div(a.K, 128));
     }

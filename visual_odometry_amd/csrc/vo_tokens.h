@@ -23,17 +23,14 @@ template <typename T> struct vo_elem;
 
 template <> struct vo_elem<float> {
     static constexpr int PER = 4;
-    static __device__ __forceinline__ vo_f32x4 mma16(vo_u32x4 a, vo_u32x4 b, vo_f32x4 c) {
+    static constexpr int PARTS = 4;                                  // instructions per chunk: callers put other sums between them
+    static __device__ __forceinline__ vo_f32x4 mma16(vo_u32x4 a, vo_u32x4 b, vo_f32x4 c, int part) {
         const vo_f32x4 x = __builtin_bit_cast(vo_f32x4, a), y = __builtin_bit_cast(vo_f32x4, b);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], y[j], c, 0, 0, 0);
-        return c;
+        return __builtin_amdgcn_mfma_f32_16x16x4f32(x[part], y[part], c, 0, 0, 0);
     }
-    static __device__ __forceinline__ vo_f32x16 mma32(vo_u32x4 a, vo_u32x4 b, vo_f32x16 c) {
+    static __device__ __forceinline__ vo_f32x16 mma32(vo_u32x4 a, vo_u32x4 b, vo_f32x16 c, int part) {
         const vo_f32x4 x = __builtin_bit_cast(vo_f32x4, a), y = __builtin_bit_cast(vo_f32x4, b);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[j], y[j], c, 0, 0, 0);
-        return c;
+        return __builtin_amdgcn_mfma_f32_32x32x2f32(x[part], y[part], c, 0, 0, 0);
     }
     static __device__ __forceinline__ float get(const float* p) { return *p; }
     static __device__ __forceinline__ void put(float* p, float v) { *p = v; }
@@ -51,10 +48,11 @@ template <> struct vo_elem<float> {
 // result leaves in the tensor's type.
 template <> struct vo_elem<_Float16> {
     static constexpr int PER = 8;
-    static __device__ __forceinline__ vo_f32x4 mma16(vo_u32x4 a, vo_u32x4 b, vo_f32x4 c) {
+    static constexpr int PARTS = 1;
+    static __device__ __forceinline__ vo_f32x4 mma16(vo_u32x4 a, vo_u32x4 b, vo_f32x4 c, int) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(vo_f16x8, a), __builtin_bit_cast(vo_f16x8, b), c, 0, 0, 0);
     }
-    static __device__ __forceinline__ vo_f32x16 mma32(vo_u32x4 a, vo_u32x4 b, vo_f32x16 c) {
+    static __device__ __forceinline__ vo_f32x16 mma32(vo_u32x4 a, vo_u32x4 b, vo_f32x16 c, int) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(vo_f16x8, a), __builtin_bit_cast(vo_f16x8, b), c, 0, 0, 0);
     }
     static __device__ __forceinline__ float get(const _Float16* p) { return (float)*p; }
@@ -75,10 +73,11 @@ template <> struct vo_elem<_Float16> {
 
 template <> struct vo_elem<__bf16> {
     static constexpr int PER = 8;
-    static __device__ __forceinline__ vo_f32x4 mma16(vo_u32x4 a, vo_u32x4 b, vo_f32x4 c) {
+    static constexpr int PARTS = 1;
+    static __device__ __forceinline__ vo_f32x4 mma16(vo_u32x4 a, vo_u32x4 b, vo_f32x4 c, int) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(vo_bf16x8, a), __builtin_bit_cast(vo_bf16x8, b), c, 0, 0, 0);
     }
-    static __device__ __forceinline__ vo_f32x16 mma32(vo_u32x4 a, vo_u32x4 b, vo_f32x16 c) {
+    static __device__ __forceinline__ vo_f32x16 mma32(vo_u32x4 a, vo_u32x4 b, vo_f32x16 c, int) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(vo_bf16x8, a), __builtin_bit_cast(vo_bf16x8, b), c, 0, 0, 0);
     }
     static __device__ __forceinline__ float get(const __bf16* p) { return (float)*p; }
@@ -113,11 +112,13 @@ static __device__ __forceinline__ void vo_load_to_lds(__amdgpu_buffer_rsrc_t rs,
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)lds, 16, offset, 0, 0, 0);
 }
 
-// Waits for this wave's loads into LDS, then for the workgroup.  The wait is spelled out because the compiler's own barrier
-// does not count loads into LDS in every loop (results of another wave's load were read too early without it).
-static __device__ __forceinline__ void vo_lds_barrier() {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
+// Waits for this wave's loads into LDS and its LDS reads, then for the workgroup.  Spelled out because the compiler's own
+// barrier does not count loads into LDS in every loop (another wave's load was read too early without it), and would not
+// leave any pending.
+// PENDING: how many of this wave's youngest loads may still be under way.
+template <int PENDING = 0> static __device__ __forceinline__ void vo_lds_barrier() {
+    static_assert(PENDING >= 0 && PENDING < 64, "the counter has six bits");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(PENDING) : "memory");
 }
 
 // `n` (< PER) or all PER elements of a row from any address: a wide load that needs no alignment, or element by element at
