@@ -25,15 +25,28 @@ struct LinArgs {
     int wide_out;                    // y, r rows allow 16-byte accesses
 };
 
-__device__ __forceinline__ float activate(float z, int act) {
+// z / (1 + e^-u): the exponential is exp2 of u log2(e), rounded once, so its relative error grows like |u| 2^-24; where |u| is
+// large the sum is 1 or the quotient has vanished from 16 bits.  float32 storage takes the library's functions.
+template <bool EXACT> __device__ __forceinline__ float over_sigmoid(float z, float u) {
+    if constexpr (EXACT) return z / (1.f + expf(-u));
+    return z * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504088896341f * u));
+}
+
+// erf for results of 16 bits: Abramowitz and Stegun 7.1.26, |error| <= 1.5e-7.  The library's erff takes both of its branches in
+// most waves: its share of a 16384 x 4096 x 16384 product was 150 us of 1883.
+__device__ __forceinline__ float erf_short(float x) {
+    const float y = fabsf(x), t = __builtin_amdgcn_rcpf(1.f + 0.3275911f * y);
+    const float p = t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+    return copysignf(1.f - p * __builtin_amdgcn_exp2f(-1.44269504088896341f * y * y), x);
+}
+
+template <bool EXACT> __device__ __forceinline__ float activate(float z, int act) {
     switch (act) {
         case VO_ACT_RELU: return z < 0.f ? 0.f : z;                                          // NaN stays NaN
-        case VO_ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
-        case VO_ACT_GELU_TANH: {                                                             // (1 + tanh u) / 2 = 1 / (1 + e^-2u)
-            const float u = 0.79788456080286536f * (z + 0.044715f * z * z * z);
-            return z / (1.f + expf(-2.f * u));
-        }
-        case VO_ACT_SILU: return z / (1.f + expf(-z));
+        case VO_ACT_GELU: return 0.5f * z * (1.f + (EXACT ? erff(z * 0.70710678118654752f) : erf_short(z * 0.70710678118654752f)));
+        case VO_ACT_GELU_TANH:                                                               // (1 + tanh u) / 2 = 1 / (1 + e^-2u)
+            return over_sigmoid<EXACT>(z, 1.5957691216057308f * (z + 0.044715f * z * z * z));
+        case VO_ACT_SILU: return over_sigmoid<EXACT>(z, z);
         default: return z;
     }
 }
@@ -58,7 +71,7 @@ template <typename T> struct Piece {
         T* y = static_cast<T*>(a.y) + m * a.ys + k;
         float v[PER];
 #pragma unroll
-        for (int j = 0; j < PER; ++j) v[j] = activate(acc[j] + bias[j], a.act);
+        for (int j = 0; j < PER; ++j) v[j] = activate<sizeof(T) == 4>(acc[j] + bias[j], a.act);
         if (a.wide_out && k + PER <= a.K) {
             if (a.res) {
                 float r[PER];
@@ -93,25 +106,23 @@ template <typename T> struct Piece {
 };
 
 // ------------------------------------------------------------------------------------------------------------ tiles
-__device__ __forceinline__ int swizzle(int row) { return (row >> 1) & 7; }
-template <int SIDE> struct Sums { using type = vo_f32x4; };
-template <> struct Sums<32> { using type = vo_f32x16; };
+template <int CH> __device__ __forceinline__ int swizzle(int row) { return (row / (16 / CH)) & (CH - 1); }
 
 // WGM x WGN waves; a wave owns TM rows of x times TN outputs as 16x16 products with W as the first operand, so that a lane
 // holds four consecutive outputs of one row.  LDS rows are 128 bytes (eight chunks); chunk c of row r sits at
 // c ^ (r / 2 % 8), which spreads the 16-byte reads of sixteen rows over all 64 banks (r % 8 in its place: half of the LDS cycles
 // were conflicts).  The permutation is applied to the addresses the lanes
 // fetch, because a load into LDS places lane l's bytes at position l.
-template <typename T, int BM, int BN, int WGM, int WGN, int SIDE, int STAGES, bool DIRECT>
+template <typename T, int BM, int BN, int WGM, int WGN, int ROWB, int STAGES, bool DIRECT>
 __global__ __launch_bounds__(64 * WGM * WGN) void linear_tiles(const LinArgs a) {
-    constexpr int PER = vo_elem<T>::PER, BK = 8 * PER, NW = WGM * WGN;
-    constexpr int TM = BM / WGM, TN = BN / WGN, MT = TM / SIDE, NT = TN / SIDE;
-    constexpr int GROUPS = 64 / SIDE, KK = 4 / GROUPS;               // lane groups; products along half a slab
-    constexpr int ROWS = BM + BN, LOADS = ROWS / 8 / NW;             // 1 KiB wave loads (8 rows) per wave and slab
+    constexpr int PER = vo_elem<T>::PER, CH = ROWB / 16, BK = CH * PER, NW = WGM * WGN;
+    constexpr int TM = BM / WGM, TN = BN / WGN, MT = TM / 16, NT = TN / 16;
+    constexpr int LR = 1024 / ROWB;                                  // rows per wave load of 1 KiB
+    constexpr int ROWS = BM + BN, LOADS = ROWS / LR / NW;            // wave loads per wave and slab
     constexpr int STRIP = TN + 4;                                    // floats per row of the store's staging strip
-    constexpr int SLAB = ROWS * 128, STAGE = NW * SIDE * STRIP * 4;
-    static_assert(ROWS % (8 * NW) == 0 && BM % (8 * NW) == 0, "a wave's loads must not straddle the operands");
-    static_assert(DIRECT || STAGES == 2, "registers hold one more slab");
+    constexpr int SLAB = ROWS * ROWB, STAGE = NW * 16 * STRIP * 4;
+    static_assert(ROWS % (LR * NW) == 0 && BM % (LR * NW) == 0 && (ROWB == 64 || ROWB == 128), "a wave's loads must not straddle the operands");
+    static_assert(DIRECT || (STAGES == 2 && ROWB == 128), "registers hold one more slab");
     __shared__ __align__(16) unsigned char lds[STAGES * SLAB > STAGE ? STAGES * SLAB : STAGE];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -135,28 +146,36 @@ __global__ __launch_bounds__(64 * WGM * WGN) void linear_tiles(const LinArgs a) 
     const __amdgpu_buffer_rsrc_t xrs = vo_buffer(xt, (rows_x - 1) * xb + wb);
     const __amdgpu_buffer_rsrc_t wrs = vo_buffer(wt, rows_w * wb);
 
-    const int sub = lane >> 3;                                       // this lane's row of a load's eight
-    auto is_x = [&](int i) { return i < LOADS * BM / ROWS; };        // loads 0.. of a wave fetch x, the rest W
-    auto tile_row = [&](int i) {                                     // first of the eight rows of load i, within its operand
-        constexpr int XL = LOADS * BM / ROWS;
-        return is_x(i) ? (wave * XL + i) * 8 : (wave * (LOADS - XL) + i - XL) * 8;
+    constexpr int XL = LOADS * BM / ROWS;                            // loads 0 .. XL - 1 of a wave fetch x, the rest W
+    const int sub = lane / CH;                                       // this lane's row of a load's
+    auto is_x = [&](int i) { return i < XL; };
+    auto tile_row = [&](int i) {                                     // first of the rows of load i, within its operand
+        return (is_x(i) ? wave * XL + i : wave * (LOADS - XL) + i - XL) * LR;
     };
-    auto chunk = [&](int i) { return (lane & 7) ^ swizzle(tile_row(i) + sub); };             // the chunk it fetches
-    unsigned off[LOADS];
+    auto chunk = [&](int i) { return (lane % CH) ^ swizzle<CH>(tile_row(i) + sub); };        // the chunk it fetches
+    // Offsets of an operand's first two loads (the chunk order repeats every 16 rows); load i lies i whole loads further.  Rows
+    // behind the operand's last lie behind its descriptor and become zero by themselves.
+    unsigned first[2][2];
+    int ahead_of[2][2];                                              // elements of C ahead of the chunk within the slab
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-        const int r = tile_row(i) + sub;
-        const bool in = r < (is_x(i) ? rows_x : rows_w);
-        off[i] = in ? (unsigned)(r * (is_x(i) ? xb : wb) + chunk(i) * 16) : VO_OUTSIDE;
-    }
+    for (int o = 0; o < 2; ++o)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            const int i = o == 0 ? q : XL + q;
+            first[o][q] = (unsigned)((tile_row(i) - q * LR + sub) * (o == 0 ? xb : wb)) + chunk(i) * 16;
+            ahead_of[o][q] = chunk(i) * PER;
+        }
     vo_u32x4 reg[DIRECT ? 1 : LOADS];
     auto fetch = [&](int s, unsigned char* buf) {
         const int c0 = c_first + s * BK;
         if constexpr (DIRECT) {
 #pragma unroll
-            for (int i = 0; i < LOADS; ++i)                          // whole chunks: C is a multiple of PER
-                vo_load_to_lds(is_x(i) ? xrs : wrs, buf + (is_x(i) ? 0 : BM * 128) + tile_row(i) * 128,
-                               c0 + chunk(i) * PER < c_last ? off[i] + c0 * (unsigned)sizeof(T) : VO_OUTSIDE);
+            for (int i = 0; i < LOADS; ++i) {                        // whole chunks: C is a multiple of PER
+                const int o = is_x(i) ? 0 : 1, j = is_x(i) ? i : i - XL;
+                const unsigned at = first[o][j & 1] + (unsigned)(c0 * (int)sizeof(T) + j * LR * (int)(o == 0 ? xb : wb));
+                vo_load_to_lds(o == 0 ? xrs : wrs, buf + (o == 0 ? 0 : BM * ROWB) + tile_row(i) * ROWB,
+                               ahead_of[o][j & 1] < c_last - c0 ? at : VO_OUTSIDE);
+            }
         } else {
 #pragma unroll
             for (int i = 0; i < LOADS; ++i) {
@@ -172,40 +191,32 @@ __global__ __launch_bounds__(64 * WGM * WGN) void linear_tiles(const LinArgs a) 
         if constexpr (!DIRECT) {
 #pragma unroll
             for (int i = 0; i < LOADS; ++i)
-                *reinterpret_cast<vo_u32x4*>(buf + (is_x(i) ? 0 : BM * 128) + tile_row(i) * 128 + lane * 16) = reg[i];
+                *reinterpret_cast<vo_u32x4*>(buf + (is_x(i) ? 0 : BM * ROWB) + tile_row(i) * ROWB + lane * 16) = reg[i];
         }
     };
 
     const int wm = wave / WGN, wn = wave % WGN;
-    typename Sums<SIDE>::type acc[NT][MT] = {};
-    const int fr = lane % SIDE, fg = lane / SIDE;
-    struct Frags { vo_u32x4 w[NT][KK], x[MT][KK]; } f0, f1;          // operands of a slab's two halves
-    auto read = [&](Frags& f, const unsigned char* buf, int half) {
+    vo_f32x4 acc[NT][MT] = {};
+    const int fr = lane & 15, fg = lane >> 4;
+    struct Frags { vo_u32x4 w[NT], x[MT]; } f0, f1;                  // operands of 64 bytes of the rows
+    auto read = [&](Frags& f, const unsigned char* buf, int part) {
+        const int pos = ((part * 4 + fg) ^ swizzle<CH>(fr)) * 16;
 #pragma unroll
-        for (int q = 0; q < KK; ++q) {
-            const int pos = ((half * 4 + q * GROUPS + fg) ^ swizzle(fr)) * 16;
+        for (int i = 0; i < NT; ++i) f.w[i] = *reinterpret_cast<const vo_u32x4*>(buf + (BM + wn * TN + i * 16 + fr) * ROWB + pos);
 #pragma unroll
-            for (int i = 0; i < NT; ++i) f.w[i][q] = *reinterpret_cast<const vo_u32x4*>(buf + (BM + wn * TN + i * SIDE + fr) * 128 + pos);
-#pragma unroll
-            for (int i = 0; i < MT; ++i) f.x[i][q] = *reinterpret_cast<const vo_u32x4*>(buf + (wm * TM + i * SIDE + fr) * 128 + pos);
-        }
+        for (int i = 0; i < MT; ++i) f.x[i] = *reinterpret_cast<const vo_u32x4*>(buf + (wm * TM + i * 16 + fr) * ROWB + pos);
     };
     auto multiply = [&](const Frags& f) {
 #pragma unroll
-        for (int q = 0; q < KK; ++q)
+        for (int part = 0; part < vo_elem<T>::PARTS; ++part)
 #pragma unroll
-            for (int part = 0; part < vo_elem<T>::PARTS; ++part)
+            for (int i = 0; i < NT; ++i)
 #pragma unroll
-                for (int i = 0; i < NT; ++i)
-#pragma unroll
-                    for (int j = 0; j < MT; ++j) {
-                        if constexpr (SIDE == 32) acc[i][j] = vo_elem<T>::mma32(f.w[i][q], f.x[j][q], acc[i][j], part);
-                        else acc[i][j] = vo_elem<T>::mma16(f.w[i][q], f.x[j][q], acc[i][j], part);
-                    }
+                for (int j = 0; j < MT; ++j) acc[i][j] = vo_elem<T>::mma16(f.w[i], f.x[j], acc[i][j], part);
     };
     // one LDS read per few products, so that neither pipe waits for the other
     auto interleave = [&]() {
-        constexpr int PRODUCTS = NT * MT * KK * vo_elem<T>::PARTS, READS = (NT + MT) * KK, EACH = PRODUCTS / READS > 0 ? PRODUCTS / READS : 1;
+        constexpr int PRODUCTS = NT * MT * vo_elem<T>::PARTS, READS = NT + MT, EACH = PRODUCTS / READS > 0 ? PRODUCTS / READS : 1;
 #pragma unroll
         for (int i = 0; i < READS; ++i) {
             __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
@@ -235,33 +246,56 @@ __global__ __launch_bounds__(64 * WGM * WGN) void linear_tiles(const LinArgs a) 
         __syncthreads();
     }
     read(f0, buf, 0);
-    for (int s = 0; s + 1 < slabs; ++s) {
+    if constexpr (ROWB == 128) {
+        for (int s = 0; s + 1 < slabs; ++s) {
+            read(f1, buf, 1);
+            multiply(f0);
+            interleave();
+            if constexpr (DIRECT) {
+                vo_lds_barrier<(STAGES - 2) * LOADS>();
+                fetch(s + STAGES, buf);
+            } else {
+                __syncthreads();
+                if (s + 2 < slabs) put(buf);
+                if (s + 3 < slabs) fetch(s + 3, nullptr);
+            }
+            buf = after(buf);
+            read(f0, buf, 0);
+            multiply(f1);
+            interleave();
+        }
         read(f1, buf, 1);
         multiply(f0);
         interleave();
-        if constexpr (DIRECT) {
+        multiply(f1);
+    } else {
+        // slabs of one part: f0 and f1 take turns
+        auto step = [&](int s, Frags& now, Frags& next) {
             vo_lds_barrier<(STAGES - 2) * LOADS>();
             fetch(s + STAGES, buf);
-        } else {
-            __syncthreads();
-            if (s + 2 < slabs) put(buf);
-            if (s + 3 < slabs) fetch(s + 3, nullptr);
+            buf = after(buf);
+            read(next, buf, 0);
+            multiply(now);
+            interleave();
+        };
+        int s = 0;
+        for (; s + 2 < slabs; s += 2) {
+            step(s, f0, f1);
+            step(s + 1, f1, f0);
         }
-        buf = after(buf);
-        read(f0, buf, 0);
-        multiply(f1);
-        interleave();
+        if (s + 1 < slabs) {
+            step(s, f0, f1);
+            multiply(f1);
+        } else {
+            multiply(f0);
+        }
     }
-    read(f1, buf, 1);
-    multiply(f0);
-    interleave();
-    multiply(f1);
 
-    // store: SIDE rows at a time through a strip of LDS of the wave's own, so that rows leave in 16-byte pieces.  The
+    // store: sixteen rows at a time through a strip of LDS of the wave's own, so that rows leave in 16-byte pieces.  The
     // loop stays rolled (the epilogue's code is long) and the sums move down one place per round, because a register
     // array with a running index would live in memory.  The residual's pieces are fetched a round ahead.
-    float* strip = reinterpret_cast<float*>(lds) + wave * SIDE * STRIP;
-    constexpr int ACROSS = TN / PER, PIECES = SIDE * ACROSS >= 64 ? SIDE * ACROSS / 64 : 1;   // 16-byte pieces per row; per lane and round
+    float* strip = reinterpret_cast<float*>(lds) + wave * 16 * STRIP;
+    constexpr int ACROSS = TN / PER, PIECES = 16 * ACROSS >= 64 ? 16 * ACROSS / 64 : 1;   // 16-byte pieces per row; per lane and round
     static_assert(64 % ACROSS == 0, "a lane keeps to its columns");
     const int col = lane % ACROSS * PER, k = n0 + wn * TN + col;
     const int64_t m_first = m0 + wm * TM + lane / ACROSS;
@@ -275,16 +309,7 @@ __global__ __launch_bounds__(64 * WGM * WGN) void linear_tiles(const LinArgs a) 
 #pragma unroll 1
     for (int j = 0; j < MT; ++j) {
 #pragma unroll
-        for (int i = 0; i < NT; ++i) {
-            if constexpr (SIDE == 32) {
-#pragma unroll
-                for (int b = 0; b < 4; ++b)
-                    *reinterpret_cast<vo_f32x4*>(strip + fr * STRIP + i * 32 + b * 8 + fg * 4) =
-                        vo_f32x4{acc[i][0][4 * b], acc[i][0][4 * b + 1], acc[i][0][4 * b + 2], acc[i][0][4 * b + 3]};
-            } else {
-                *reinterpret_cast<vo_f32x4*>(strip + fr * STRIP + i * 16 + fg * 4) = acc[i][0];
-            }
-        }
+        for (int i = 0; i < NT; ++i) *reinterpret_cast<vo_f32x4*>(strip + fr * STRIP + i * 16 + fg * 4) = acc[i][0];
 #pragma unroll
         for (int i = 0; i < NT; ++i)
 #pragma unroll
@@ -293,13 +318,13 @@ __global__ __launch_bounds__(64 * WGM * WGN) void linear_tiles(const LinArgs a) 
 #pragma unroll
         for (int p = 0; p < PIECES; ++p) {
             now[p] = ahead[p];
-            if (j + 1 < MT) ahead[p].load_residual(a, m_first + (j + 1) * SIDE + p * STEP, k);
+            if (j + 1 < MT) ahead[p].load_residual(a, m_first + (j + 1) * 16 + p * STEP, k);
         }
         vo_wave_lds_fence();
 #pragma unroll
         for (int p = 0; p < PIECES; ++p) {
-            const int64_t m = m_first + j * SIDE + p * STEP;
-            if (m < a.M && k < a.K && lane / ACROSS + p * STEP < SIDE) {
+            const int64_t m = m_first + j * 16 + p * STEP;
+            if (m < a.M && k < a.K && lane / ACROSS + p * STEP < 16) {
                 float v[PER];
 #pragma unroll
                 for (int q = 0; q < PER; q += 4) {
@@ -456,10 +481,10 @@ template <typename T, bool DIRECT> int launch(const LinArgs& a, const Plan& p, h
     const dim3 grid((unsigned)(p.tiles_m * p.tiles_n * p.splits));
     constexpr int S32 = DIRECT ? 6 : 2, S64 = DIRECT ? 4 : 2;
     if (p.form == 0) linear_rows<T, DIRECT><<<grid, 512, 0, st>>>(a);
-    else if (p.form == 1) linear_tiles<T, 32, 64, 1, 4, 16, S32, DIRECT><<<grid, 256, 0, st>>>(a);
-    else if (p.form == 2) linear_tiles<T, 64, 64, 2, 2, 16, S64, DIRECT><<<grid, 256, 0, st>>>(a);
-    else if (p.form == 3) linear_tiles<T, 128, 128, 2, 2, 16, 2, DIRECT><<<grid, 256, 0, st>>>(a);
-    else if constexpr (sizeof(T) == 2 && DIRECT) linear_tiles<T, 256, 256, 2, 4, 32, 2, DIRECT><<<grid, 512, 0, st>>>(a);
+    else if (p.form == 1) linear_tiles<T, 32, 64, 1, 4, 128, S32, DIRECT><<<grid, 256, 0, st>>>(a);
+    else if (p.form == 2) linear_tiles<T, 64, 64, 2, 2, 128, S64, DIRECT><<<grid, 256, 0, st>>>(a);
+    else if (p.form == 3) linear_tiles<T, 128, 128, 2, 2, 128, 2, DIRECT><<<grid, 256, 0, st>>>(a);
+    else if constexpr (sizeof(T) == 2 && DIRECT) linear_tiles<T, 256, 256, 2, 4, 128, 2, DIRECT><<<grid, 512, 0, st>>>(a);
     VO_CHECK_LAUNCH("vo_linear");
     if (p.splits > 1) {
         const int64_t pieces = a.M * vo_ceil_div(a.K, vo_elem<T>::PER);
