@@ -62,7 +62,8 @@ def make(M, C, K, dtype, seed, bias=True, res=False):
     (65, 1, 1), (65, 8, 8), (70, 63, 65), (100, 324, 256), (129, 72, 129), (200, 130, 66), (320, 64, 64), (333, 96, 250),
     (1, 4096, 300), (3, 5001, 16), (40, 2056, 24), (70, 4100, 64), (130, 1999, 130),           # split over C
     (1500, 40, 2049), (1543, 33, 2048), (3601, 72, 4001), (3700, 9, 4096),                     # the larger tiles
-    (4800, 324, 256)])
+    (4800, 324, 256),
+    (1201, 1003, 1100), (640, 2701, 2700)])                                                    # rows padded to whole pieces first
 def test_shapes(vo, dtype, M, C, K):
     x, w, b, r = make(M, C, K, dtype, M * 7 + C * 3 + K, res=True)
     check(ops.linear(x, w), x, w)
@@ -80,7 +81,7 @@ def test_activations_over_their_whole_range(vo, dtype, act, M, K):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("M,C,K", [(9, 72, 40), (96, 72, 40), (1600, 72, 2048), (2, 4096, 24)])
+@pytest.mark.parametrize("M,C,K", [(9, 72, 40), (96, 72, 40), (1600, 72, 2048), (2, 4096, 24), (1201, 1003, 1100)])
 @pytest.mark.parametrize("lead,pad", [(0, 16), (8, 8), (1, 3), (3, 0)])
 def test_slices_of_wider_tensors(vo, dtype, M, C, K, lead, pad):
     """x, residual and out are column slices; what lies around out's columns stays as it was."""

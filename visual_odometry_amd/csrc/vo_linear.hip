@@ -22,7 +22,6 @@ struct LinArgs {
     int C, K, act;
     int splits, c_per_split;         // c_per_split: a multiple of the slab
     unsigned tiles_m, tiles_n;
-    int wide_out;                    // y, r rows allow 16-byte accesses
 };
 
 // z / (1 + e^-u): the exponential is exp2 of u log2(e), rounded once, so its relative error grows like |u| 2^-24; where |u| is
@@ -51,8 +50,8 @@ template <bool EXACT> __device__ __forceinline__ float activate(float z, int act
     }
 }
 
-// PER consecutive outputs k.. of one row (`n` of them exist): the bias and, where rows allow wide accesses, the residual are
-// fetched ahead of their use.
+// PER consecutive outputs k.. of one row: the bias and the residual are fetched ahead of their use.  A row's last, shorter
+// piece goes element by element.
 template <typename T> struct Piece {
     static constexpr int PER = vo_elem<T>::PER;
     vo_u32x4 res;
@@ -63,8 +62,7 @@ template <typename T> struct Piece {
     }
     __device__ __forceinline__ void load_residual(const LinArgs& a, int64_t m, int k) {
         res = vo_u32x4{0, 0, 0, 0};
-        if (a.res && a.wide_out && m < a.M && k + PER <= a.K)
-            res = *reinterpret_cast<const vo_u32x4*>(static_cast<const T*>(a.res) + m * a.rs + k);
+        if (a.res && m < a.M && k + PER <= a.K) res = vo_load16(static_cast<const T*>(a.res) + m * a.rs + k);
     }
     // bias, activation, residual, one rounding
     __device__ __forceinline__ void finish(const LinArgs& a, int64_t m, int k, const float* acc, const float* bias) const {
@@ -72,14 +70,14 @@ template <typename T> struct Piece {
         float v[PER];
 #pragma unroll
         for (int j = 0; j < PER; ++j) v[j] = activate<sizeof(T) == 4>(acc[j] + bias[j], a.act);
-        if (a.wide_out && k + PER <= a.K) {
+        if (k + PER <= a.K) {
             if (a.res) {
                 float r[PER];
                 vo_elem<T>::unpack(res, r);
 #pragma unroll
                 for (int j = 0; j < PER; ++j) v[j] += r[j];
             }
-            *reinterpret_cast<vo_u32x4*>(y) = vo_elem<T>::pack(v);
+            vo_store16(y, vo_elem<T>::pack(v));
         } else {
             const T* r = static_cast<const T*>(a.res) + m * a.rs + k;
 #pragma unroll
@@ -91,9 +89,9 @@ template <typename T> struct Piece {
     __device__ __forceinline__ void emit(const LinArgs& a, int split, int64_t m, int k, const float* acc, const float* bias) const {
         if (a.splits > 1) {
             float* p = a.part + ((int64_t)split * a.M + m) * a.K + k;
-            if ((a.K & 3) == 0 && k + PER <= a.K) {
+            if (k + PER <= a.K) {
 #pragma unroll
-                for (int j = 0; j < PER; j += 4) *reinterpret_cast<float4*>(p + j) = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+                for (int j = 0; j < PER; j += 4) vo_store16(p + j, __builtin_bit_cast(vo_u32x4, vo_f32x4{acc[j], acc[j + 1], acc[j + 2], acc[j + 3]}));
             } else {
 #pragma unroll
                 for (int j = 0; j < PER; ++j)
@@ -106,23 +104,22 @@ template <typename T> struct Piece {
 };
 
 // ------------------------------------------------------------------------------------------------------------ tiles
-template <int CH> __device__ __forceinline__ int swizzle(int row) { return (row / (16 / CH)) & (CH - 1); }
+__device__ __forceinline__ int swizzle(int row) { return (row >> 1) & 7; }
 
 // WGM x WGN waves; a wave owns TM rows of x times TN outputs as 16x16 products with W as the first operand, so that a lane
 // holds four consecutive outputs of one row.  LDS rows are 128 bytes (eight chunks); chunk c of row r sits at
 // c ^ (r / 2 % 8), which spreads the 16-byte reads of sixteen rows over all 64 banks (r % 8 in its place: half of the LDS cycles
 // were conflicts).  The permutation is applied to the addresses the lanes
 // fetch, because a load into LDS places lane l's bytes at position l.
-template <typename T, int BM, int BN, int WGM, int WGN, int ROWB, int STAGES, bool DIRECT>
+template <typename T, int BM, int BN, int WGM, int WGN, int STAGES, bool DIRECT>
 __global__ __launch_bounds__(64 * WGM * WGN) void linear_tiles(const LinArgs a) {
-    constexpr int PER = vo_elem<T>::PER, CH = ROWB / 16, BK = CH * PER, NW = WGM * WGN;
+    constexpr int PER = vo_elem<T>::PER, BK = 8 * PER, NW = WGM * WGN;
     constexpr int TM = BM / WGM, TN = BN / WGN, MT = TM / 16, NT = TN / 16;
-    constexpr int LR = 1024 / ROWB;                                  // rows per wave load of 1 KiB
-    constexpr int ROWS = BM + BN, LOADS = ROWS / LR / NW;            // wave loads per wave and slab
+    constexpr int ROWS = BM + BN, LOADS = ROWS / 8 / NW;             // 1 KiB wave loads (8 rows) per wave and slab
     constexpr int STRIP = TN + 4;                                    // floats per row of the store's staging strip
-    constexpr int SLAB = ROWS * ROWB, STAGE = NW * 16 * STRIP * 4;
-    static_assert(ROWS % (LR * NW) == 0 && BM % (LR * NW) == 0 && (ROWB == 64 || ROWB == 128), "a wave's loads must not straddle the operands");
-    static_assert(DIRECT || (STAGES == 2 && ROWB == 128), "registers hold one more slab");
+    constexpr int SLAB = ROWS * 128, STAGE = NW * 16 * STRIP * 4;
+    static_assert(ROWS % (8 * NW) == 0 && BM % (8 * NW) == 0, "a wave's loads must not straddle the operands");
+    static_assert(DIRECT || STAGES == 2, "registers hold one more slab");
     __shared__ __align__(16) unsigned char lds[STAGES * SLAB > STAGE ? STAGES * SLAB : STAGE];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -147,12 +144,12 @@ __global__ __launch_bounds__(64 * WGM * WGN) void linear_tiles(const LinArgs a) 
     const __amdgpu_buffer_rsrc_t wrs = vo_buffer(wt, rows_w * wb);
 
     constexpr int XL = LOADS * BM / ROWS;                            // loads 0 .. XL - 1 of a wave fetch x, the rest W
-    const int sub = lane / CH;                                       // this lane's row of a load's
+    const int sub = lane >> 3;                                       // this lane's row of a load's eight
     auto is_x = [&](int i) { return i < XL; };
-    auto tile_row = [&](int i) {                                     // first of the rows of load i, within its operand
-        return (is_x(i) ? wave * XL + i : wave * (LOADS - XL) + i - XL) * LR;
+    auto tile_row = [&](int i) {                                     // first of the eight rows of load i, within its operand
+        return (is_x(i) ? wave * XL + i : wave * (LOADS - XL) + i - XL) * 8;
     };
-    auto chunk = [&](int i) { return (lane % CH) ^ swizzle<CH>(tile_row(i) + sub); };        // the chunk it fetches
+    auto chunk = [&](int i) { return (lane & 7) ^ swizzle(tile_row(i) + sub); };             // the chunk it fetches
     // Offsets of an operand's first two loads (the chunk order repeats every 16 rows); load i lies i whole loads further.  Rows
     // behind the operand's last lie behind its descriptor and become zero by themselves.
     unsigned first[2][2];
@@ -162,7 +159,7 @@ __global__ __launch_bounds__(64 * WGM * WGN) void linear_tiles(const LinArgs a) 
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
             const int i = o == 0 ? q : XL + q;
-            first[o][q] = (unsigned)((tile_row(i) - q * LR + sub) * (o == 0 ? xb : wb)) + chunk(i) * 16;
+            first[o][q] = (unsigned)((tile_row(i) - q * 8 + sub) * (o == 0 ? xb : wb)) + chunk(i) * 16;
             ahead_of[o][q] = chunk(i) * PER;
         }
     vo_u32x4 reg[DIRECT ? 1 : LOADS];
@@ -172,8 +169,8 @@ __global__ __launch_bounds__(64 * WGM * WGN) void linear_tiles(const LinArgs a) 
 #pragma unroll
             for (int i = 0; i < LOADS; ++i) {                        // whole chunks: C is a multiple of PER
                 const int o = is_x(i) ? 0 : 1, j = is_x(i) ? i : i - XL;
-                const unsigned at = first[o][j & 1] + (unsigned)(c0 * (int)sizeof(T) + j * LR * (int)(o == 0 ? xb : wb));
-                vo_load_to_lds(o == 0 ? xrs : wrs, buf + (o == 0 ? 0 : BM * ROWB) + tile_row(i) * ROWB,
+                const unsigned at = first[o][j & 1] + (unsigned)(c0 * (int)sizeof(T) + j * 8 * (int)(o == 0 ? xb : wb));
+                vo_load_to_lds(o == 0 ? xrs : wrs, buf + (o == 0 ? 0 : BM * 128) + tile_row(i) * 128,
                                ahead_of[o][j & 1] < c_last - c0 ? at : VO_OUTSIDE);
             }
         } else {
@@ -191,7 +188,7 @@ __global__ __launch_bounds__(64 * WGM * WGN) void linear_tiles(const LinArgs a) 
         if constexpr (!DIRECT) {
 #pragma unroll
             for (int i = 0; i < LOADS; ++i)
-                *reinterpret_cast<vo_u32x4*>(buf + (is_x(i) ? 0 : BM * ROWB) + tile_row(i) * ROWB + lane * 16) = reg[i];
+                *reinterpret_cast<vo_u32x4*>(buf + (is_x(i) ? 0 : BM * 128) + tile_row(i) * 128 + lane * 16) = reg[i];
         }
     };
 
@@ -200,11 +197,11 @@ __global__ __launch_bounds__(64 * WGM * WGN) void linear_tiles(const LinArgs a) 
     const int fr = lane & 15, fg = lane >> 4;
     struct Frags { vo_u32x4 w[NT], x[MT]; } f0, f1;                  // operands of 64 bytes of the rows
     auto read = [&](Frags& f, const unsigned char* buf, int part) {
-        const int pos = ((part * 4 + fg) ^ swizzle<CH>(fr)) * 16;
+        const int pos = ((part * 4 + fg) ^ swizzle(fr)) * 16;
 #pragma unroll
-        for (int i = 0; i < NT; ++i) f.w[i] = *reinterpret_cast<const vo_u32x4*>(buf + (BM + wn * TN + i * 16 + fr) * ROWB + pos);
+        for (int i = 0; i < NT; ++i) f.w[i] = *reinterpret_cast<const vo_u32x4*>(buf + (BM + wn * TN + i * 16 + fr) * 128 + pos);
 #pragma unroll
-        for (int i = 0; i < MT; ++i) f.x[i] = *reinterpret_cast<const vo_u32x4*>(buf + (wm * TM + i * 16 + fr) * ROWB + pos);
+        for (int i = 0; i < MT; ++i) f.x[i] = *reinterpret_cast<const vo_u32x4*>(buf + (wm * TM + i * 16 + fr) * 128 + pos);
     };
     auto multiply = [&](const Frags& f) {
 #pragma unroll
@@ -246,50 +243,27 @@ __global__ __launch_bounds__(64 * WGM * WGN) void linear_tiles(const LinArgs a) 
         __syncthreads();
     }
     read(f0, buf, 0);
-    if constexpr (ROWB == 128) {
-        for (int s = 0; s + 1 < slabs; ++s) {
-            read(f1, buf, 1);
-            multiply(f0);
-            interleave();
-            if constexpr (DIRECT) {
-                vo_lds_barrier<(STAGES - 2) * LOADS>();
-                fetch(s + STAGES, buf);
-            } else {
-                __syncthreads();
-                if (s + 2 < slabs) put(buf);
-                if (s + 3 < slabs) fetch(s + 3, nullptr);
-            }
-            buf = after(buf);
-            read(f0, buf, 0);
-            multiply(f1);
-            interleave();
-        }
+    for (int s = 0; s + 1 < slabs; ++s) {
         read(f1, buf, 1);
         multiply(f0);
         interleave();
-        multiply(f1);
-    } else {
-        // slabs of one part: f0 and f1 take turns
-        auto step = [&](int s, Frags& now, Frags& next) {
+        if constexpr (DIRECT) {
             vo_lds_barrier<(STAGES - 2) * LOADS>();
             fetch(s + STAGES, buf);
-            buf = after(buf);
-            read(next, buf, 0);
-            multiply(now);
-            interleave();
-        };
-        int s = 0;
-        for (; s + 2 < slabs; s += 2) {
-            step(s, f0, f1);
-            step(s + 1, f1, f0);
-        }
-        if (s + 1 < slabs) {
-            step(s, f0, f1);
-            multiply(f1);
         } else {
-            multiply(f0);
+            __syncthreads();
+            if (s + 2 < slabs) put(buf);
+            if (s + 3 < slabs) fetch(s + 3, nullptr);
         }
+        buf = after(buf);
+        read(f0, buf, 0);
+        multiply(f1);
+        interleave();
     }
+    read(f1, buf, 1);
+    multiply(f0);
+    interleave();
+    multiply(f1);
 
     // store: sixteen rows at a time through a strip of LDS of the wave's own, so that rows leave in 16-byte pieces.  The
     // loop stays rolled (the epilogue's code is long) and the sums move down one place per round, because a register
@@ -413,13 +387,13 @@ template <typename T> __global__ __launch_bounds__(256) void linear_join(const L
     float v[PER] = {}, bias[PER];
     piece_of.load_residual(a, m, k);
     Piece<T>::load_bias(a, k, bias);
-    const bool wide = (a.K & 3) == 0 && k + PER <= a.K;
+    const bool wide = k + PER <= a.K;
     for (int s = 0; s < a.splits; ++s) {
         const float* p = a.part + ((int64_t)s * a.M + m) * a.K + k;
         if (wide) {
 #pragma unroll
             for (int j = 0; j < PER; j += 4) {
-                const vo_f32x4 t = *reinterpret_cast<const vo_f32x4*>(p + j);
+                const vo_f32x4 t = __builtin_bit_cast(vo_f32x4, vo_load16(p + j));
                 v[j] += t[0]; v[j + 1] += t[1]; v[j + 2] += t[2]; v[j + 3] += t[3];
             }
         } else {
@@ -430,31 +404,54 @@ template <typename T> __global__ __launch_bounds__(256) void linear_join(const L
     piece_of.finish(a, m, k, v, bias);
 }
 
+// Rows of C elements, any alignment, to rows of C rounded up to whole 16-byte pieces: x behind one another, then W.
+template <typename T> __global__ __launch_bounds__(256) void linear_pad(const T* x, int64_t xs, int64_t M, const T* w, int K, int C, T* out) {
+    constexpr int PER = vo_elem<T>::PER;
+    const int64_t across = (C + PER - 1) / PER, piece = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (piece >= (M + K) * across) return;
+    const int64_t row = piece / across;
+    const int c = (int)(piece % across) * PER;
+    const T* p = row < M ? x + row * xs : w + (row - M) * C;
+    *reinterpret_cast<vo_u32x4*>(out + piece * PER) = vo_load_unaligned<T>(p + c, C - c);
+}
+
 // ------------------------------------------------------------------------------------------------------------- host
 
-// Tiles: rows of x, outputs, and the rate at which a full machine works on them relative to the largest (16-bit, float32).
-struct Form { int bm, bn; float rate16, rate32; };
-constexpr Form FORMS[] = {{16, 16, 0, 0}, {32, 64, 0, 0}, {64, 64, 0.5f, 1.f}, {128, 128, 0.75f, 1.f}, {256, 256, 1.f, 0.f}};
+// Tiles: rows of x, outputs, slabs under way, resident workgroups per CU.  The estimated time of a product on a form is its rounds
+// over the CUs times a tile's work over the form's rate, which a short C does not reach (`ramp`: the C at which half of it is).
+// Measured on 16-bit products, us: 4096 x 4096 x 4096 on forms 3 / 4: 152 / 123; 2048 x 2048 x 2048 on 2 / 3 / 4: 32 / 36 / 49;
+// 38400 x 256 x 256 on 2 / 3 / 4: 19 / 25 / 26; float32 38400 x 256 x 256 on 2 / 3: 63 / 72.
+struct Form { int bm, bn; float rate16, rate32, ramp; };
+constexpr Form FORMS[] = {{16, 16, 0, 0, 0}, {32, 64, 0, 0, 0}, {64, 64, 0.55f, 1.f, 100}, {128, 128, 0.75f, 1.05f, 500}, {256, 256, 1.f, 0.f, 800}};
 
 struct Plan {
     int form;                        // of FORMS; 0: linear_rows
     int splits, c_per_split;
     int64_t tiles_m, tiles_n;
+    bool deep;                       // few 64 x 64 tiles: more slabs under way in place of more workgroups
+    int64_t padded;                  // C not in whole 16-byte pieces: elements of the padded copies of x and W (0: none are made)
 };
 
 Plan plan(int64_t M, int C, int K, int dtype) {
-    const int slab = dtype == VO_F32 ? 32 : 64;
+    const int slab = dtype == VO_F32 ? 32 : 64, per = slab / 8;
     Plan p{};
-    if (M <= 16) p.form = 0;
-    else if (M <= 32) p.form = 1;
-    else {
-        // the tile whose rounds over the 256 CUs take least
+    // Unaligned rows cannot go straight into LDS, and through registers they run at less than half the rate: where the product
+    // outweighs its operands they are copied to aligned rows first (3001 x 2777 x 3333 bfloat16: 183 us without the copies).
+    if (C % per && (double)M * K >= 512.0 * (M + K) && (double)M * K * C >= 1e9) {
+        C = (C + per - 1) / per * per;
+        p.padded = (M + K) * C;
+    }
+    if (M <= 32) {
+        // One row of 4096 x 4096 (bfloat16): 10 us by rows, 12 by split tiles and their join; 16 rows of 4096 x 16384: 39 by
+        // rows, 31 by tiles that need no split.
+        p.form = M <= 4 || (M <= 16 && vo_ceil_div(K, 64) < 192) ? 0 : 1;
+    } else {
         float best = 0.f;
         for (int f = 2; f <= 4; ++f) {
             const float rate = dtype == VO_F32 ? FORMS[f].rate32 : FORMS[f].rate16;
             if (rate == 0.f) continue;
             const int64_t tiles = vo_ceil_div(M, FORMS[f].bm) * vo_ceil_div(K, FORMS[f].bn);
-            const float cost = (float)vo_ceil_div(tiles, 256) * FORMS[f].bm * FORMS[f].bn / rate;
+            const float cost = (float)vo_ceil_div(tiles, 256) * FORMS[f].bm * FORMS[f].bn * (C + FORMS[f].ramp) / rate;
             if (p.form == 0 || cost < best) {
                 p.form = f;
                 best = cost;
@@ -474,17 +471,23 @@ Plan plan(int64_t M, int C, int K, int dtype) {
     }
     p.c_per_split = (int)vo_ceil_div(vo_ceil_div(C, slab), splits) * slab;
     p.splits = (int)vo_ceil_div(C, p.c_per_split);
+    p.deep = tiles * p.splits <= 512;                                // 512 x 2048 x 2048: 14 us against 20; 2048^3: 37 against 32
     return p;
+}
+
+int64_t needed(const Plan& p, int64_t M, int K, int dtype) {
+    return p.padded * (dtype == VO_F32 ? 4 : 2) + (p.splits > 1 ? (int64_t)p.splits * M * K * 4 : 0);
 }
 
 template <typename T, bool DIRECT> int launch(const LinArgs& a, const Plan& p, hipStream_t st) {
     const dim3 grid((unsigned)(p.tiles_m * p.tiles_n * p.splits));
-    constexpr int S32 = DIRECT ? 6 : 2, S64 = DIRECT ? 4 : 2;
+    constexpr int S32 = DIRECT ? 6 : 2, S64 = DIRECT ? 4 : 2;        // slabs under way
     if (p.form == 0) linear_rows<T, DIRECT><<<grid, 512, 0, st>>>(a);
-    else if (p.form == 1) linear_tiles<T, 32, 64, 1, 4, 128, S32, DIRECT><<<grid, 256, 0, st>>>(a);
-    else if (p.form == 2) linear_tiles<T, 64, 64, 2, 2, 128, S64, DIRECT><<<grid, 256, 0, st>>>(a);
-    else if (p.form == 3) linear_tiles<T, 128, 128, 2, 2, 128, 2, DIRECT><<<grid, 256, 0, st>>>(a);
-    else if constexpr (sizeof(T) == 2 && DIRECT) linear_tiles<T, 256, 256, 2, 4, 128, 2, DIRECT><<<grid, 512, 0, st>>>(a);
+    else if (p.form == 1) linear_tiles<T, 32, 64, 1, 4, S32, DIRECT><<<grid, 256, 0, st>>>(a);
+    else if (p.form == 2 && p.deep) linear_tiles<T, 64, 64, 2, 2, S64, DIRECT><<<grid, 256, 0, st>>>(a);
+    else if (p.form == 2) linear_tiles<T, 64, 64, 2, 2, 2, DIRECT><<<grid, 256, 0, st>>>(a);
+    else if (p.form == 3) linear_tiles<T, 128, 128, 2, 2, 2, DIRECT><<<grid, 256, 0, st>>>(a);
+    else if constexpr (sizeof(T) == 2 && DIRECT) linear_tiles<T, 256, 256, 2, 4, 2, DIRECT><<<grid, 512, 0, st>>>(a);
     VO_CHECK_LAUNCH("vo_linear");
     if (p.splits > 1) {
         const int64_t pieces = a.M * vo_ceil_div(a.K, vo_elem<T>::PER);
@@ -496,6 +499,17 @@ template <typename T, bool DIRECT> int launch(const LinArgs& a, const Plan& p, h
 
 template <typename T> int dispatch(LinArgs a, Plan p, hipStream_t st) {
     const size_t es = sizeof(T);
+    if (p.padded) {
+        T* rows = reinterpret_cast<T*>(a.part);
+        linear_pad<T><<<dim3((unsigned)vo_ceil_div(p.padded / vo_elem<T>::PER, 256)), 256, 0, st>>>(
+            static_cast<const T*>(a.x), a.xs, a.M, static_cast<const T*>(a.w), a.K, a.C, rows);
+        VO_CHECK_LAUNCH("vo_linear (padded rows)");
+        a.C = (int)(p.padded / (a.M + a.K));
+        a.x = rows;
+        a.xs = a.C;
+        a.w = rows + a.M * a.C;
+        a.part = reinterpret_cast<float*>(rows + p.padded);
+    }
     const bool direct = (a.C * es) % 16 == 0 && (a.xs * es) % 16 == 0 && reinterpret_cast<uintptr_t>(a.x) % 16 == 0 &&
                         reinterpret_cast<uintptr_t>(a.w) % 16 == 0;
     if (!direct && p.form == 4) {                                    // registers for staging leave no room for the largest tile
@@ -510,8 +524,7 @@ template <typename T> int dispatch(LinArgs a, Plan p, hipStream_t st) {
 
 extern "C" int64_t vo_linear_workspace_bytes(int64_t M, int C, int K, int dtype) {
     if (M <= 0 || C <= 0 || K <= 0) return 0;
-    const Plan p = plan(M, C, K, dtype);
-    return p.splits > 1 ? (int64_t)p.splits * M * K * 4 : 0;
+    return needed(plan(M, C, K, dtype), M, K, dtype);
 }
 
 extern "C" int vo_linear(const void* x, int64_t x_row_stride, const void* weight, const float* bias, const void* residual,
@@ -531,7 +544,7 @@ extern "C" int vo_linear(const void* x, int64_t x_row_stride, const void* weight
         return vo_fail(VO_ERR_UNSUPPORTED, "vo_linear: rows of x and weight must be under 8 MiB");
     if (p.tiles_m * p.tiles_n * p.splits * 4 >= (1ll << 31) || M * vo_ceil_div(K, 4) >= (1ll << 38))
         return vo_fail(VO_ERR_UNSUPPORTED, "vo_linear: M=%lld K=%d is too large for one launch", (long long)M, K);
-    const int64_t need = p.splits > 1 ? (int64_t)p.splits * M * K * 4 : 0;
+    const int64_t need = needed(p, M, K, dtype);
     VO_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
                "vo_linear: needs a 16-byte aligned workspace of %lld bytes", (long long)need);
     LinArgs a{};
@@ -540,8 +553,6 @@ extern "C" int vo_linear(const void* x, int64_t x_row_stride, const void* weight
     a.M = M; a.C = C; a.K = K; a.act = activation;
     a.splits = p.splits; a.c_per_split = p.c_per_split;
     a.tiles_m = (unsigned)p.tiles_m; a.tiles_n = (unsigned)p.tiles_n;
-    a.wide_out = reinterpret_cast<uintptr_t>(y) % 16 == 0 && y_row_stride * es % 16 == 0 &&
-                 (!residual || (reinterpret_cast<uintptr_t>(residual) % 16 == 0 && residual_row_stride * es % 16 == 0));
     hipStream_t st = vo_stream(stream);
     if (dtype == VO_F32) return dispatch<float>(a, p, st);
     if (dtype == VO_F16) return dispatch<_Float16>(a, p, st);

@@ -121,13 +121,21 @@ template <int PENDING = 0> static __device__ __forceinline__ void vo_lds_barrier
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(PENDING) : "memory");
 }
 
+// 16 bytes at any address: the memory pipes take unaligned accesses, the compiler just has to be told.
+static __device__ __forceinline__ vo_u32x4 vo_load16(const void* p) {
+    vo_u32x4 r;
+    __builtin_memcpy(&r, p, 16);
+    return r;
+}
+static __device__ __forceinline__ void vo_store16(void* p, vo_u32x4 v) { __builtin_memcpy(p, &v, 16); }
+
 // `n` (< PER) or all PER elements of a row from any address: a wide load that needs no alignment, or element by element at
 // a row's end.  Missing elements are zero.
 template <typename T> static __device__ __forceinline__ vo_u32x4 vo_load_unaligned(const T* p, int64_t n) {
     constexpr int PER = vo_elem<T>::PER;
     vo_u32x4 r = {0, 0, 0, 0};
     if (n >= PER) {
-        __builtin_memcpy(&r, p, 16);
+        r = vo_load16(p);
     } else {
         float v[PER];
 #pragma unroll
