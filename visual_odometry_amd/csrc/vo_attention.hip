@@ -82,38 +82,46 @@ template <typename T, int DT, int KEYS> struct Core {
             q[s] = p && c * E::PER < D ? *reinterpret_cast<const vo_u32x4*>(p + c * E::PER) : vo_u32x4{0, 0, 0, 0};
         }
     }
-    // One tile; `limit`: the lane's row sees the tile's keys below it (used when masked)
-    __device__ __forceinline__ void step(const unsigned char* kt, const unsigned char* vt, float c, bool masked, int limit, int lane) {
-        const int col = lane & 31, half = lane >> 5;
-        vo_f32x16 s[KB];
+    // s = K q of a key tile
+    __device__ __forceinline__ void scores(const unsigned char* kt, vo_f32x16* s, int lane) const {
 #pragma unroll
-        for (int b = 0; b < KB; ++b) {
-            const int r = b * 32 + col;
-            vo_f32x16 acc = {};
+        for (int b = 0; b < KB; ++b)
 #pragma unroll
-            for (int i = 0; i < QS; ++i) {
-                const vo_u32x4 kf = *reinterpret_cast<const vo_u32x4*>(kt + r * L::ROW + (((i * 2 + half) ^ L::k_swz(r)) * 16));
+            for (int j = 0; j < 16; ++j) s[b][j] = 0.f;
 #pragma unroll
-                for (int part = 0; part < E::PARTS; ++part) acc = E::mma32(kf, q[i], acc, part);
+        for (int i = 0; i < QS; ++i)
+#pragma unroll
+            for (int b = 0; b < KB; ++b) {
+                const int r = b * 32 + (lane & 31);
+                const vo_u32x4 kf = *reinterpret_cast<const vo_u32x4*>(kt + r * L::ROW + (((i * 2 + (lane >> 5)) ^ L::k_swz(r)) * 16));
+#pragma unroll
+                for (int part = 0; part < E::PARTS; ++part) s[b] = E::mma32(kf, q[i], s[b], part);
             }
-            s[b] = acc;
-        }
-        if (masked) {
+    }
+    // The lane's row sees the tile's keys below `limit`.
+    static __device__ __forceinline__ void mask(vo_f32x16* s, int limit, int lane) {
+        const int mine = limit - 4 * (lane >> 5);
 #pragma unroll
-            for (int b = 0; b < KB; ++b)
+        for (int b = 0; b < KB; ++b)
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (b * 32 + 8 * (i >> 2) + 4 * half + (i & 3) >= limit) s[b][i] = -INFINITY;
-        }
+            for (int i = 0; i < 16; ++i)
+                if (b * 32 + 8 * (i >> 2) + (i & 3) >= mine) s[b][i] = -INFINITY;
+    }
+    // The largest of this lane's scores.
+    static __device__ __forceinline__ float largest(const vo_f32x16* s) {
         float top = s[0][0];
 #pragma unroll
         for (int b = 0; b < KB; ++b)
 #pragma unroll
             for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
-        top = fmaxf(top, __shfl_xor(top, 32));
-        if (__any(top * c > m * c + 8.f || (m == -INFINITY && top > m))) {
+        return top;
+    }
+    // Lets m follow the row's largest score (`top`: this half's) where that pays (see the top of the file).
+    __device__ __forceinline__ void follow(float top, float c) {
+        top = across(top, [](float x, float y) { return fmaxf(x, y); });
+        if (__any(top * c > m * c + 8.f)) {                          // m starts at -inf
             const float next = fmaxf(m, top);
-            const float f = next == -INFINITY ? 0.f : exp2f((m - next) * c);
+            const float f = next == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - next) * c);
             l *= f;
 #pragma unroll
             for (int i = 0; i < DB; ++i)
@@ -121,50 +129,82 @@ template <typename T, int DT, int KEYS> struct Core {
                 for (int j = 0; j < 16; ++j) o[i][j] *= f;
             m = next;
         }
-        const float base = m == -INFINITY ? 0.f : -m * c;
-        float sum = 0.f;
+    }
+    // Scores 2 j and 2 j + 1 of a block of 32 keys to exponentials, rounded to the storage type where that has 16 bits; `sum` takes
+    // the unrounded ones.
+    static constexpr int PW = sizeof(T) == 2 ? 8 : 16;               // registers of a block's exponentials
+    static __device__ __forceinline__ void weigh(const vo_f32x16& s, unsigned* p, float* sum, int j, float c, float base) {
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * j], c, base));
+        const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * j + 1], c, base));
+        sum[0] += x;
+        sum[1] += y;
+        if constexpr (sizeof(T) == 2) {
+            p[j] = E::pack2(x, y);
+        } else {
+            p[2 * j] = __builtin_bit_cast(unsigned, x);
+            p[2 * j + 1] = __builtin_bit_cast(unsigned, y);
+        }
+    }
+    __device__ __forceinline__ float base_of(float c) const { return m == -INFINITY ? 0.f : -m * c; }
+    __device__ __forceinline__ void weights(const vo_f32x16* s, unsigned (*p)[PW], float c) {
+        const float base = base_of(c);
+        float sum[2] = {0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < 8 * KB; ++j) weigh(s[j / 8], p[j / 8], sum, j % 8, c, base);
+        l += sum[0] + sum[1];
+    }
+    // 16 bits: V^T of 16 keys (half `h` of block b) for every 32 features.  Keys r.. and r + 8.. : the lane supplies 8 bytes of row
+    // r + (lane % 16) / 4 and receives four rows of feature d * 32 + lane % 32.
+    // One piece is 16 keys of one block of features, the operand of one product: piece j has the features j % DB, the keys 16 (j / DB)...
+    static constexpr int VALUES = 2 * KB * DB;
+    static __device__ __forceinline__ vo_u32x4 value_piece(const unsigned char* vt, int j, int lane) {
+        const int r = 16 * (j / DB) + 4 * (lane >> 5) + ((lane & 15) >> 2), at = (lane & 1) * 8;
+        const int chunk = j % DB * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
+        const vo_u32x2 lo = transposed(vt + r * L::ROW + ((chunk ^ L::v_swz(r)) * 16) + at);
+        const vo_u32x2 hi = transposed(vt + (r + 8) * L::ROW + ((chunk ^ L::v_swz(r + 8)) * 16) + at);
+        return vo_u32x4{lo[0], lo[1], hi[0], hi[1]};
+    }
+    __device__ __forceinline__ void add_values(vo_u32x4 v, const unsigned (*p)[PW], int j) {
+        const unsigned* w = p[j / (2 * DB)] + 4 * (j / DB % 2);
+        o[j % DB] = E::mma32(v, vo_u32x4{w[0], w[1], w[2], w[3]}, o[j % DB], 0);
+    }
+    // o += V^T p
+    __device__ __forceinline__ void accumulate(const unsigned char* vt, const unsigned (*p)[PW], int lane) {
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+            for (int j = 0; j < VALUES; ++j) add_values(value_piece(vt, j, lane), p, j);
+            return;
+        }
+        const int col = lane & 31, half = lane >> 5;
 #pragma unroll
         for (int b = 0; b < KB; ++b)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                s[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], c, base));
-                sum += s[b][i];
-            }
-        l += sum;
+                const int r = b * 32 + 8 * (i >> 2) + 4 * half + (i & 3);
 #pragma unroll
-        for (int b = 0; b < KB; ++b) {
-            if constexpr (sizeof(T) == 2) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    float p[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) p[i] = s[b][8 * h + i];
-                    const vo_u32x4 pf = E::pack(p);
-#pragma unroll
-                    for (int d = 0; d < DB; ++d) {
-                        // keys r.. and r + 8.. : the lane supplies 8 bytes of row r + (lane % 16) / 4 and receives four rows of
-                        // feature d * 32 + lane % 32
-                        const int r = b * 32 + 16 * h + 4 * half + ((lane & 15) >> 2);
-                        const int chunk = d * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
-                        const int at = (lane & 1) * 8;
-                        const vo_u32x2 lo = transposed(vt + r * L::ROW + ((chunk ^ L::v_swz(r)) * 16) + at);
-                        const vo_u32x2 hi = transposed(vt + (r + 8) * L::ROW + ((chunk ^ L::v_swz(r + 8)) * 16) + at);
-                        o[d] = E::mma32(vo_u32x4{lo[0], lo[1], hi[0], hi[1]}, pf, o[d], 0);
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int r = b * 32 + 8 * (i >> 2) + 4 * half + (i & 3);
-#pragma unroll
-                    for (int d = 0; d < DB; ++d) {
-                        const int chunk = d * 8 + (col >> 2);
-                        const float vf = *reinterpret_cast<const float*>(vt + r * L::ROW + ((chunk ^ L::v_swz(r)) * 16) + (col & 3) * 4);
-                        o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf, s[b][i], o[d], 0, 0, 0);
-                    }
+                for (int d = 0; d < DB; ++d) {
+                    const int chunk = d * 8 + (col >> 2);
+                    const float vf = *reinterpret_cast<const float*>(vt + r * L::ROW + ((chunk ^ L::v_swz(r)) * 16) + (col & 3) * 4);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf, __builtin_bit_cast(float, p[b][i]), o[d], 0, 0, 0);
                 }
             }
-        }
+    }
+    // A whole tile.
+    __device__ __forceinline__ void step(const unsigned char* kt, const unsigned char* vt, float c, bool masked, int limit, int lane) {
+        vo_f32x16 s[KB];
+        unsigned p[KB][PW];
+        scores(kt, s, lane);
+        if (masked) mask(s, limit, lane);
+        follow(largest(s), c);
+        weights(s, p, c);
+        accumulate(vt, p, lane);
+    }
+    // x of this lane and of the other half's lane (l + 32) % 64, combined: both get the same
+    template <typename F> static __device__ __forceinline__ float across(float x, F f) {
+        const unsigned u = __builtin_bit_cast(unsigned, x);
+        const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+        const unsigned lo = r[0], hi = r[1];
+        return f(__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi));
     }
     static __device__ __forceinline__ vo_u32x2 transposed(const unsigned char* p) {
         typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -274,19 +314,24 @@ __global__ __launch_bounds__(256, MIN_BLOCKS) void attention_tiles(const AttArgs
     Loader<T, DT, KEYS, 4> lk, lv;
     lk.init(a.ks, a.D, false, wave, lane);
     lv.init(a.vs, a.D, true, wave, lane);
-    auto fetch = [&](int64_t t, unsigned char* buf) {
-        lk.load(kb + t * KEYS * a.ks, a.ks, p.Lk - t * KEYS, a.D, buf, wave);
-        lv.load(vb + t * KEYS * a.vs, a.vs, p.Lk - t * KEYS, a.D, buf + HALF, wave);
-    };
-    if (t0 < t1) fetch(t0, lds);
+    auto fetch_k = [&](int64_t t, unsigned char* buf) { lk.load(kb + t * KEYS * a.ks, a.ks, p.Lk - t * KEYS, a.D, buf, wave); };
+    auto fetch_v = [&](int64_t t, unsigned char* buf) { lv.load(vb + t * KEYS * a.vs, a.vs, p.Lk - t * KEYS, a.D, buf, wave); };
+    unsigned char *now = lds, *next = lds + 2 * HALF;
+    if (t0 < t1) {
+        fetch_k(t0, now);
+        fetch_v(t0, now + HALF);
+    }
     for (int64_t t = t0; t < t1; ++t) {
-        unsigned char* now = lds + ((t - t0) & 1) * 2 * HALF;
-        vo_lds_barrier();                                            // tile t has arrived, tile t - 1 has been read
-        if (t + 1 < t1) fetch(t + 1, lds + (1 - ((t - t0) & 1)) * 2 * HALF);
+        vo_lds_barrier();                                        // tile t has arrived, tile t - 1 has been read
+        if (t + 1 < t1) {
+            fetch_k(t + 1, next);
+            fetch_v(t + 1, next + HALF);
+        }
         const int64_t key = t * KEYS;
         if (key < wave_any) core.step(now, now + HALF, a.c, key + KEYS > wave_all, (int)vo_clamp64(limit - key, 0, KEYS), lane);
+        unsigned char* x = now; now = next; next = x;
     }
-    const float l = core.l + __shfl_xor(core.l, 32);
+    const float l = core.across(core.l, [](float x, float y) { return x + y; });
     if (!have) return;
     if (a.splits > 1) store_part<T, DT>(a, split, p.q0 + row, head, core.o, core.m, l, lane);
     else store_out<T, DT>(a, p.q0 + row, head, core.o, inverse(l), lane);
@@ -344,7 +389,7 @@ __global__ __launch_bounds__(64 * WAVES) void attention_rows(const AttArgs a) {
         core.step(now, now + HALF, a.c, key + KEYS > all, (int)vo_clamp64(limit - key, 0, KEYS), lane);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");           // its reads are done before it is loaded over
     }
-    core.l += __shfl_xor(core.l, 32);
+    core.l = core.across(core.l, [](float x, float y) { return x + y; });
 
     // join the waves in order: sums as (feature, row) planes of LDS, m and l behind them
     constexpr int PLANE = DT * 33 * 4;                               // 33: lanes of one row apart in banks
