@@ -655,7 +655,7 @@ int vo_linear(const void* x, int64_t x_row_stride, const void* weight, const flo
  * workspace: vo_attention_workspace_bytes(...) bytes (often 0), 16-byte aligned, contents irrelevant.  Calls that share one
  * must be ordered on one stream; two captured graphs that may replay at once need one each.
  * ------------------------------------------------------------------------- */
-int64_t vo_attention_workspace_bytes(int64_t q_tokens, int64_t k_tokens, int sequences, int q_heads, int k_heads, int D);
+int64_t vo_attention_workspace_bytes(int64_t q_tokens, int64_t k_tokens, int sequences, int q_heads, int k_heads, int D, int dtype);
 int vo_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride,
                  const void* k, int64_t k_token_stride, int64_t k_head_stride,
                  const void* v, int64_t v_token_stride, int64_t v_head_stride,

@@ -116,7 +116,7 @@ def test_groups_of_heads(vo, dtype, Hq, Hk, q_len, k_len):
     ([100], [6007], 2, 1, 64), ([40, 70], [3000, 2500], 2, 2, 128), ([129], [1500], 1, 1, 256)])      # tiles, split over the keys
 def test_long_axes_are_split_and_joined(vo, dtype, causal, q_len, k_len, Hq, Hk, D):
     from visual_odometry_amd import _lib
-    assert _lib.load().vo_attention_workspace_bytes(sum(q_len), sum(k_len), len(q_len), Hq, Hk, D) > 0
+    assert _lib.load().vo_attention_workspace_bytes(sum(q_len), sum(k_len), len(q_len), Hq, Hk, D, ops._TOKEN_DTYPES[dtype]) > 0
     run(q_len, k_len, Hq, Hk, D, dtype, causal, 5)
 
 

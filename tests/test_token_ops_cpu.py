@@ -103,10 +103,10 @@ def test_attention_entry_point_refuses():
                dict(o=ctypes.c_void_p(p.value + 2)), dict(Tq=1 << 31), dict(Tk=1 << 31), dict(dt=0, D=30)):
         assert call(**kw) == _lib.VO_ERR_UNSUPPORTED, kw
     assert call(Tq=0) == _lib.VO_OK
-    need = lib.vo_attention_workspace_bytes(1, 65536, 1, 2, 2, 32)
+    need = lib.vo_attention_workspace_bytes(1, 65536, 1, 2, 2, 32, 1)
     assert need > 0 and call(Tq=1, Tk=65536) == _lib.VO_ERR_INVALID_ARG and b"workspace" in lib.vo_last_error()
     assert call(Tq=1, Tk=65536, ws=p, wb=need - 1) == _lib.VO_ERR_INVALID_ARG
-    assert lib.vo_attention_workspace_bytes(1, 65536, 1, 3, 2, 32) == 0 and lib.vo_attention_workspace_bytes(0, 5, 1, 2, 2, 32) == 0
+    assert lib.vo_attention_workspace_bytes(1, 65536, 1, 3, 2, 32, 1) == 0 and lib.vo_attention_workspace_bytes(0, 5, 1, 2, 2, 32, 1) == 0
 
 
 def test_the_python_entry_points_refuse_cpu_tensors():

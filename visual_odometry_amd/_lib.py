@@ -95,7 +95,7 @@ SIGNATURES = {
 # entry points that return a size instead of a status
 SIZE_QUERIES = {"vo_pair_poses_workspace_bytes": [_I, _I],
                 "vo_linear_workspace_bytes": [_L, _I, _I, _I],
-                "vo_attention_workspace_bytes": [_L, _L, _I, _I, _I, _I]}
+                "vo_attention_workspace_bytes": [_L, _L, _I, _I, _I, _I, _I]}
 EXPORTS = sorted(list(SIGNATURES) + list(SIZE_QUERIES) + ["vo_version", "vo_last_error"])
 
 _lib = None

@@ -235,40 +235,41 @@ template <typename T, int DT, int KEYS, int WAVES> struct Loader {
     }
 };
 
-// A lane's column of O^T: row `row` of the output, or (split) of the workspace.
-template <typename T, int DT> __device__ __forceinline__ void store_part(const AttArgs& a, int split, int64_t token, int head,
-                                                                         const vo_f32x16* o, float m, float l, int lane) {
-    const int64_t row = ((int64_t)split * a.Tq + token) * a.Hq + head;
-    float* p = a.part + row * a.D;
-#pragma unroll
-    for (int d = 0; d < DT / 32; ++d)
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            const int f = d * 32 + 8 * b + 4 * (lane >> 5);
-            if (f < a.D) *reinterpret_cast<float4*>(p + f) = make_float4(o[d][4 * b], o[d][4 * b + 1], o[d][4 * b + 2], o[d][4 * b + 3]);
-        }
-    if (lane < 32) {
-        float* ml = a.part + (int64_t)a.splits * a.Tq * a.Hq * a.D + row * 2;
-        ml[0] = m * a.c;
-        ml[1] = l;
-    }
+// Where the results of a row go: the output, or (split) the workspace.
+__device__ __forceinline__ float* part_row(const AttArgs& a, int split, int64_t token, int head) {
+    return a.part + (((int64_t)split * a.Tq + token) * a.Hq + head) * a.D;
+}
+__device__ __forceinline__ float* part_ml(const AttArgs& a, int split, int64_t token, int head) {
+    return a.part + (int64_t)a.splits * a.Tq * a.Hq * a.D + (((int64_t)split * a.Tq + token) * a.Hq + head) * 2;
+}
+template <typename T> __device__ __forceinline__ T* out_row(const AttArgs& a, int64_t token, int head) {
+    return static_cast<T*>(a.out) + token * a.os + head * a.oh;
 }
 
-template <typename T, int DT> __device__ __forceinline__ void store_out(const AttArgs& a, int64_t token, int head, const vo_f32x16* o,
-                                                                        float inv, int lane) {
-    T* p = static_cast<T*>(a.out) + token * a.os + head * a.oh;
+// A wave's O^T (times `factor`, one number per lane = row) as rows of S: a lane holds four features of one row at a time, so
+// the rows are put together in the wave's own LDS (chunks in an order that spreads the banks) and leave in pieces of 16 bytes.
+// row(r): where row r goes, null if it does not exist.
+template <typename S, int DT, typename F>
+__device__ __forceinline__ void store_rows(const vo_f32x16* o, float factor, int D, unsigned char* lds, int lane, F row) {
+    constexpr int ES = sizeof(S), CH = DT * ES / 16, MASK = CH < 16 ? CH - 1 : 15, EACH = 16 / ES;
+    const int r = lane & 31;
 #pragma unroll
     for (int d = 0; d < DT / 32; ++d)
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
             const int f = d * 32 + 8 * b + 4 * (lane >> 5);
-            if (f >= a.D) continue;
-            const float v0 = o[d][4 * b] * inv, v1 = o[d][4 * b + 1] * inv, v2 = o[d][4 * b + 2] * inv, v3 = o[d][4 * b + 3] * inv;
-            if constexpr (sizeof(T) == 2)
-                *reinterpret_cast<vo_u32x2*>(p + f) = vo_u32x2{vo_elem<T>::pack2(v0, v1), vo_elem<T>::pack2(v2, v3)};
-            else
-                *reinterpret_cast<float4*>(p + f) = make_float4(v0, v1, v2, v3);
+            unsigned char* p = lds + r * DT * ES + (((f / EACH) ^ (r & MASK)) * 16) + f % EACH * ES;
+            const float v0 = o[d][4 * b] * factor, v1 = o[d][4 * b + 1] * factor, v2 = o[d][4 * b + 2] * factor, v3 = o[d][4 * b + 3] * factor;
+            if constexpr (ES == 2) *reinterpret_cast<vo_u32x2*>(p) = vo_u32x2{vo_elem<S>::pack2(v0, v1), vo_elem<S>::pack2(v2, v3)};
+            else *reinterpret_cast<vo_f32x4*>(p) = vo_f32x4{v0, v1, v2, v3};
         }
+    vo_wave_lds_fence();
+#pragma unroll
+    for (int i = 0; i < CH / 2; ++i) {
+        const int piece = i * 64 + lane, q = piece / CH, c = (piece % CH) ^ (q & MASK);
+        S* p = row(q);
+        if (p && c * EACH < D) *reinterpret_cast<vo_u32x4*>(p + c * EACH) = *reinterpret_cast<const vo_u32x4*>(lds + piece * 16);
+    }
 }
 
 __device__ __forceinline__ float inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }      // 0: the row saw nothing
@@ -278,6 +279,7 @@ template <typename T, int DT, int KEYS, int MIN_BLOCKS>
 __global__ __launch_bounds__(256, MIN_BLOCKS) void attention_tiles(const AttArgs a) {
     using L = Tile<T, DT>;
     constexpr int ROWS = 128, HALF = KEYS * L::ROW;
+    static_assert(HALF >= 32 * DT * 4, "a wave's rows of float32 fit a quarter of the LDS");
     __shared__ __align__(16) unsigned char lds[4 * HALF];            // two stages of K and V
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
@@ -332,9 +334,16 @@ __global__ __launch_bounds__(256, MIN_BLOCKS) void attention_tiles(const AttArgs
         unsigned char* x = now; now = next; next = x;
     }
     const float l = core.across(core.l, [](float x, float y) { return x + y; });
-    if (!have) return;
-    if (a.splits > 1) store_part<T, DT>(a, split, p.q0 + row, head, core.o, core.m, l, lane);
-    else store_out<T, DT>(a, p.q0 + row, head, core.o, inverse(l), lane);
+    vo_lds_barrier();                                                // every wave is done with the key tiles
+    const int64_t first = p.row + wave * 32;
+    if (a.splits > 1) {
+        store_rows<float, DT>(core.o, 1.f, a.D, lds + wave * HALF, lane,
+                              [&](int r) { return first + r < p.Lq ? part_row(a, split, p.q0 + first + r, head) : nullptr; });
+        if (have && lane < 32) *reinterpret_cast<float2*>(part_ml(a, split, p.q0 + row, head)) = make_float2(core.m * a.c, l);
+    } else {
+        store_rows<T, DT>(core.o, inverse(l), a.D, lds + wave * HALF, lane,
+                          [&](int r) { return first + r < p.Lq ? out_row<T>(a, p.q0 + first + r, head) : nullptr; });
+    }
 }
 
 // ------------------------------------------------------------------------------------------------------------- rows
@@ -417,7 +426,6 @@ __global__ __launch_bounds__(64 * WAVES) void attention_rows(const AttArgs a) {
             l += w[i] * x[32 + (lane & 31)];
         }
         // wave w finishes the feature blocks w, w + WAVES, ..
-        const int64_t prow = ((int64_t)split * a.Tq + p.q0 + token) * a.Hq + head;
         const float inv = inverse(l);
         for (int d = wave; d < DT / 32; d += WAVES) {
 #pragma unroll
@@ -432,54 +440,72 @@ __global__ __launch_bounds__(64 * WAVES) void attention_rows(const AttArgs a) {
                 }
                 if (!have || f >= a.D) continue;
                 if (a.splits > 1) {
-                    *reinterpret_cast<float4*>(a.part + prow * a.D + f) = make_float4(v[0], v[1], v[2], v[3]);
+                    *reinterpret_cast<vo_f32x4*>(part_row(a, split, p.q0 + token, head) + f) = vo_f32x4{v[0], v[1], v[2], v[3]};
+                } else if constexpr (sizeof(T) == 2) {
+                    *reinterpret_cast<vo_u32x2*>(out_row<T>(a, p.q0 + token, head) + f) =
+                        vo_u32x2{vo_elem<T>::pack2(v[0] * inv, v[1] * inv), vo_elem<T>::pack2(v[2] * inv, v[3] * inv)};
                 } else {
-                    T* y = static_cast<T*>(a.out) + (p.q0 + token) * a.os + head * a.oh + f;
-                    if constexpr (sizeof(T) == 2)
-                        *reinterpret_cast<vo_u32x2*>(y) = vo_u32x2{vo_elem<T>::pack2(v[0] * inv, v[1] * inv), vo_elem<T>::pack2(v[2] * inv, v[3] * inv)};
-                    else
-                        *reinterpret_cast<float4*>(y) = make_float4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+                    *reinterpret_cast<vo_f32x4*>(out_row<T>(a, p.q0 + token, head) + f) = vo_f32x4{v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv};
                 }
             }
         }
-        if (a.splits > 1 && wave == 0 && lane < 32 && have) {
-            float* x = a.part + (int64_t)a.splits * a.Tq * a.Hq * a.D + prow * 2;
-            x[0] = m * a.c;
-            x[1] = l;
-        }
     } else {
-        if (!have) return;
-        if (a.splits > 1) store_part<T, DT>(a, split, p.q0 + token, head, core.o, m, l, lane);
-        else store_out<T, DT>(a, p.q0 + token, head, core.o, inverse(l), lane);
+        auto place = [&](int r) { return p.row + r < rows ? p.row + r : -1; };
+        if (a.splits > 1) {
+            store_rows<float, DT>(core.o, 1.f, a.D, lds, lane, [&](int r) -> float* {
+                const int64_t x = place(r);
+                return x < 0 ? nullptr : part_row(a, split, p.q0 + x / a.group, kh * a.group + (int)(x % a.group));
+            });
+        } else {
+            store_rows<T, DT>(core.o, inverse(l), a.D, lds, lane, [&](int r) -> T* {
+                const int64_t x = place(r);
+                return x < 0 ? nullptr : out_row<T>(a, p.q0 + x / a.group, kh * a.group + (int)(x % a.group));
+            });
+        }
     }
+    if (a.splits > 1 && wave == 0 && lane < 32 && have)
+        *reinterpret_cast<float2*>(part_ml(a, split, p.q0 + token, head)) = make_float2(m * a.c, l);
 }
 
 // ------------------------------------------------------------------------------------------------------------- join
-// One wave per (token, head); the parts are added in their order.  Rows outside every sequence stay as they are.
-template <typename T> __global__ __launch_bounds__(256) void attention_join(const AttArgs a) {
+// One wave per (token, head): lane s takes the weight of part s; then groups of WIDTH lanes, four features a lane, each add every
+// (64 / WIDTH)-th part, and the groups' sums are added crosswise: a fixed order.  Rows outside every sequence stay as they are.
+template <typename T, int WIDTH> __global__ __launch_bounds__(256) void attention_join(const AttArgs a) {
+    constexpr int GROUPS = 64 / WIDTH;
     const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
     const int64_t token = row / a.Hq;
     if (token >= a.Tq) return;
     if (a.q_off && (token < a.q_off[0] || token >= a.q_off[a.sequences])) return;
     const int head = (int)(row % a.Hq);
-    const int64_t step = a.Tq * a.Hq;
-    const float* ml = a.part + (int64_t)a.splits * step * a.D;
-    float m = -INFINITY;
-    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, ml[(s * step + row) * 2]);
-    float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < a.splits; ++s) {
-        const float ms = ml[(s * step + row) * 2], w = ms == -INFINITY ? 0.f : exp2f(ms - m);
-        if (ms == -INFINITY) continue;                               // that part saw no key of this row
-        l += w * ml[(s * step + row) * 2 + 1];
-        if (lane * 4 < a.D) {
-            const float4 x = *reinterpret_cast<const float4*>(a.part + (s * step + row) * a.D + lane * 4);
-            o[0] += w * x.x; o[1] += w * x.y; o[2] += w * x.z; o[3] += w * x.w;
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (lane < a.splits) ml = *reinterpret_cast<const float2*>(part_ml(a, lane, token, head));
+    float m = ml.x;
+#pragma unroll
+    for (int d = 32; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+    const float w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - m);       // 0: that part saw no key of this row
+    float l = w == 0.f ? 0.f : w * ml.y;
+#pragma unroll
+    for (int d = 32; d; d >>= 1) l += __shfl_xor(l, d);
+    const int f = lane % WIDTH * 4;
+    float o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int s0 = 0; s0 < a.splits; s0 += GROUPS) {
+        const int s = s0 + lane / WIDTH;
+        const float ws = __shfl(w, s & 63);
+        if (s < a.splits && ws != 0.f && f < a.D) {
+            const vo_f32x4 x = *reinterpret_cast<const vo_f32x4*>(part_row(a, s, token, head) + f);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[j] += ws * x[j];
         }
     }
-    if (lane * 4 >= a.D) return;
+#pragma unroll
+    for (int d = 32; d >= WIDTH; d >>= 1)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] += __shfl_xor(o[j], d);
+    if (lane >= WIDTH || f >= a.D) return;
     const float inv = inverse(l);
-    T* p = static_cast<T*>(a.out) + token * a.os + head * a.oh + lane * 4;
+    T* p = out_row<T>(a, token, head) + f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) vo_elem<T>::put(p + j, o[j] * inv);
 }
@@ -492,7 +518,10 @@ struct Plan {
     int64_t tiles, blocks;
 };
 
-Plan plan(int64_t Tq, int64_t Tk, int sequences, int Hq, int Hk) {
+// Bytes of a row decide the key tiles and how many workgroups a CU holds.
+constexpr int row_bytes(int D, int es) { return (D <= 32 ? 32 : D <= 64 ? 64 : D <= 128 ? 128 : 256) * es; }
+
+Plan plan(int64_t Tq, int64_t Tk, int sequences, int Hq, int Hk, int D, int dtype) {
     const int group = Hq / Hk;
     Plan p{};
     const int64_t rows = vo_ceil_div(Tq * group, sequences);         // a sequence's rows per key head, on average
@@ -500,12 +529,34 @@ Plan plan(int64_t Tq, int64_t Tk, int sequences, int Hq, int Hk) {
     p.rows = rows <= 32;
     p.tiles = p.rows ? vo_tiles_bound(Tq, sequences, group, 32) : vo_tiles_bound(Tq, sequences, 1, 128);
     const int64_t base = p.tiles * (p.rows ? Hk : Hq);
-    int64_t want = vo_ceil_div(p.rows ? 2048 : 768, base), most = keys / (p.rows ? 128 : 256);
-    if (want > most) want = most;
-    if (want > 64) want = 64;
-    if (want < 1) want = 1;
-    p.splits = (int)want;
-    p.blocks = base * want;
+    int64_t splits = 1;
+    if (p.rows) {
+        // About eight rounds over the CUs even out sequences of different lengths (32 sequences of up to 32768 keys, 8 key heads:
+        // 495 us unsplit, 396 in 4 parts, 377 in 8, 400 in 16); a part has at least 512 keys.
+        splits = vo_ceil_div(2048, base);
+        if (splits > keys / 512) splits = keys / 512;
+    } else {
+        // Rounds over the resident workgroups times a part's key tiles and its start, plus the join's traffic.  (One sequence of
+        // 4800 float32 rows, 4 heads of 64: 352 us unsplit, 228 in 3 parts, 260 in 4, 236 in 8; 96 rows before 30001 keys, 32
+        // heads: 518 unsplit, 93 in 8, 86 in 16.)
+        const int bytes = row_bytes(D, dtype == VO_F32 ? 4 : 2), tile = bytes <= 512 ? 64 : 32;
+        const int64_t resident = 256 * (bytes <= 128 ? 4 : bytes <= 256 ? 2 : 1);
+        const double tiles = (double)vo_ceil_div(keys, tile), tile_us = D / 128.0 * (dtype == VO_F32 ? 10.0 : 2.1);
+        const double join_us = (double)Tq * Hq * D * 8 / 4e6;        // per part: written and read once
+        double best = 0.;
+        for (int s = 1; s <= 64 && s <= (keys + 255) / 256; ++s) {
+            const double blocks = (double)base * s, rounds = blocks <= resident ? 0.6 + 0.4 * blocks / resident : (double)((int64_t)((blocks + resident - 1) / resident));
+            const double us = rounds * (tiles / s + 2.) * tile_us + (s > 1 ? 4. + s * join_us : 0.);
+            if (s == 1 || us < best) {
+                best = us;
+                splits = s;
+            }
+        }
+    }
+    if (splits > 64) splits = 64;
+    if (splits < 1) splits = 1;
+    p.splits = (int)splits;
+    p.blocks = base * splits;
     return p;
 }
 
@@ -523,7 +574,7 @@ template <typename T, int DT> int launch(const AttArgs& a, const Plan& p, hipStr
     }
     VO_CHECK_LAUNCH("vo_attention");
     if (p.splits > 1) {
-        attention_join<T><<<dim3((unsigned)vo_ceil_div(a.Tq * a.Hq, 4)), 256, 0, st>>>(a);
+        attention_join<T, DT / 4><<<dim3((unsigned)vo_ceil_div(a.Tq * a.Hq, 4)), 256, 0, st>>>(a);
         VO_CHECK_LAUNCH("vo_attention (join)");
     }
     return VO_OK;
@@ -538,9 +589,9 @@ template <typename T> int dispatch(const AttArgs& a, const Plan& p, hipStream_t 
 
 }  // namespace
 
-extern "C" int64_t vo_attention_workspace_bytes(int64_t q_tokens, int64_t k_tokens, int sequences, int q_heads, int k_heads, int D) {
+extern "C" int64_t vo_attention_workspace_bytes(int64_t q_tokens, int64_t k_tokens, int sequences, int q_heads, int k_heads, int D, int dtype) {
     if (q_tokens <= 0 || k_tokens < 0 || sequences <= 0 || q_heads <= 0 || k_heads <= 0 || q_heads % k_heads || D <= 0) return 0;
-    return workspace(plan(q_tokens, k_tokens, sequences, q_heads, k_heads), q_tokens, q_heads, D);
+    return workspace(plan(q_tokens, k_tokens, sequences, q_heads, k_heads, D, dtype), q_tokens, q_heads, D);
 }
 
 extern "C" int vo_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k, int64_t k_token_stride,
@@ -567,7 +618,7 @@ extern "C" int vo_attention(const void* q, int64_t q_token_stride, int64_t q_hea
         return vo_fail(VO_ERR_UNSUPPORTED, "vo_attention: tensors must be 16-byte aligned");
     if (q_tokens >= (1ll << 31) || k_tokens >= (1ll << 31))
         return vo_fail(VO_ERR_UNSUPPORTED, "vo_attention: offsets are 32-bit: fewer than 2^31 tokens");
-    const Plan p = plan(q_tokens, k_tokens, sequences, q_heads, k_heads);
+    const Plan p = plan(q_tokens, k_tokens, sequences, q_heads, k_heads, D, dtype);
     if (p.blocks >= (1ll << 31) || q_tokens * q_heads >= (1ll << 32))
         return vo_fail(VO_ERR_UNSUPPORTED, "vo_attention: %lld tokens of %d heads are too many for one launch", (long long)q_tokens, q_heads);
     const int64_t need = workspace(p, q_tokens, q_heads, D);

@@ -1273,7 +1273,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: torc
     _call_on(q.device, "vo_attention",
              (q.data_ptr(), qs, qh, k.data_ptr(), ks, kh, v.data_ptr(), vs, vh, out.data_ptr(), os_, oh, pqo, pko, sequences, Tq, Tk, Hq, Hk,
               D, D ** -0.5 if scale is None else float(scale), 1 if causal else 0, _TOKEN_DTYPES[q.dtype]),
-             _workspace_bytes("vo_attention_workspace_bytes", Tq, Tk, sequences, Hq, Hk, D),
+             _workspace_bytes("vo_attention_workspace_bytes", Tq, Tk, sequences, Hq, Hk, D, _TOKEN_DTYPES[q.dtype]),
              q.element_size() * D * (2 * Tq * Hq + 2 * Tk * Hk))
     return out
 
