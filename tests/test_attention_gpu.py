@@ -190,6 +190,34 @@ def test_sequences_do_not_disturb_each_other(vo, dtype, q_len, k_len):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [32, 64, 128, 256])
+@pytest.mark.parametrize("q_len,k_len", [([200], [200]), ([130], [300]), ([100], [60]), ([5], [90]), ([3], [2000]), ([140], [2000])])
+def test_unbounded_keys_and_values_reach_only_the_rows_that_see_them(vo, dtype, D, q_len, k_len):
+    """Causal, with an infinity in one value, a NaN in another key and value near the diagonal: rows ahead of them are exact,
+    rows that see them have them."""
+    lq, lk = q_len[0], k_len[0]
+    q, k, v = make(q_len, k_len, 2, 1, D, dtype, 7)
+    clean = reference(q, k, v, q_len, k_len, True, D ** -0.5)
+    first = max(lk - lq // 2, lk - 90, 1)                              # a key that the later half of the rows sees
+    v[first, 0, 1] = float("inf")
+    for name, at in (("value", None), ("key", min(first + 7, lk - 1))):
+        if at is not None:
+            k[at, 0, 0] = float("nan")
+            v[at, 0, D - 1] = float("nan")
+        y = ops.attention(q, k, v, causal=True)
+        sees = torch.arange(lq, device="cuda") + lk - lq
+        ahead = sees < first
+        err = (y.double() - clean[0]).abs()
+        assert bool((err[ahead] <= clean[1][ahead]).all())
+        assert bool((y[~ahead][:, :, 1] == float("inf")).all()) or at is not None
+        others = [j for j in range(D) if j != 1]
+        if at is None:
+            assert bool((err[~ahead][:, :, others] <= clean[1][~ahead][:, :, others]).all())
+        else:
+            assert bool(y[sees >= at].isnan().all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_without_offsets_everything_is_one_sequence(vo, dtype):
     q, k, v = make([200], [333], 4, 4, 64, dtype, 1)
     assert torch.equal(ops.attention(q, k, v, causal=True), ops.attention(q, k, v, offsets([200]), offsets([333]), causal=True))

@@ -189,6 +189,61 @@ template <typename T, int DT, int KEYS> struct Core {
                 }
             }
     }
+    // Values that are infinite or NaN ("unbounded").  Where all rows see the same keys they are products like others; where a row
+    // does not see a key its weight is zero, and zero times such a value is no zero.  So a tile on a causal sequence's diagonal
+    // that holds any is multiplied with zeros in their place, and they are added at the end to the rows that see them.
+    static constexpr unsigned EXP = sizeof(T) == 4 ? 0x7f800000u : __is_same(T, _Float16) ? 0x7c00u : 0x7f80u;
+    static __device__ __forceinline__ bool unbounded(unsigned bits) { return (bits & EXP) == EXP; }
+    // Is there any in the tile?
+    static __device__ __forceinline__ bool any_unbounded(const unsigned char* vt, int lane) {
+        typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+        unsigned top[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < KEYS * L::ROW / 1024; ++i) {
+            const vo_u32x4 x = *reinterpret_cast<const vo_u32x4*>(vt + i * 1024 + lane * 16);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (sizeof(T) == 2)
+                    top[j] = __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(u16x2, top[j]), __builtin_bit_cast(u16x2, x[j] & 0x7fff7fffu)));
+                else
+                    top[j] = max(top[j], x[j] & 0x7fffffffu);
+            }
+        }
+        bool bad = false;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) bad |= unbounded(top[j]) || (sizeof(T) == 2 && unbounded(top[j] >> 16));
+        return __any(bad);
+    }
+    static __device__ __forceinline__ unsigned bounded(unsigned x) {
+        if constexpr (sizeof(T) == 4) return unbounded(x) ? 0u : x;
+        return (unbounded(x) ? 0u : x & 0xffffu) | (unbounded(x >> 16) ? 0u : x & 0xffff0000u);
+    }
+    // Part `share` of `shares` of the tile's values: unbounded ones become zero.
+    static __device__ __forceinline__ void bound(unsigned char* vt, int share, int shares, int lane) {
+#pragma unroll 1
+        for (int i = share; i < KEYS * L::ROW / 1024; i += shares) {
+            vo_u32x4* x = reinterpret_cast<vo_u32x4*>(vt + i * 1024 + lane * 16);
+            *x = vo_u32x4{bounded((*x)[0]), bounded((*x)[1]), bounded((*x)[2]), bounded((*x)[3])};
+        }
+    }
+    // The unbounded values of the keys from .. to - 1 of `v`, added as they are (any positive weight times them is them) to the sums
+    // of the rows that see them.
+    __device__ __forceinline__ void add_unbounded(const T* v, int64_t stride, int64_t from, int64_t to, int64_t limit, int D, int lane) {
+#pragma unroll 1
+        for (int64_t r = from; r < to; ++r)
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    const int f = d * 32 + 8 * b + 4 * (lane >> 5);
+                    if (f >= D || r >= limit) continue;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float x = E::get(v + r * stride + f + j);
+                        if (!(fabsf(x) < INFINITY)) o[d][4 * b + j] += x;
+                    }
+                }
+    }
     // A whole tile.
     __device__ __forceinline__ void step(const unsigned char* kt, const unsigned char* vt, float c, bool masked, int limit, int lane) {
         vo_f32x16 s[KB];
@@ -306,8 +361,11 @@ __global__ __launch_bounds__(256, MIN_BLOCKS) void attention_tiles(const AttArgs
     Core<T, DT, KEYS> core;
     core.reset();
     core.load_q(have ? static_cast<const T*>(a.q) + (p.q0 + row) * a.qs + head * a.qh : nullptr, a.D, lane);
-    // keys below `limit` are seen by this lane's row; tiles wholly below wave_all need no mask, from wave_any on no work
+    // keys below `limit` are seen by this lane's row; tiles wholly below wave_all need no mask, from wave_any on no work; tiles
+    // wholly below `all` are seen by every row of the workgroup
     const int64_t limit = a.causal ? vo_clamp64(row + shift + 1, 0, p.Lk) : p.Lk;
+    const int64_t all = a.causal ? vo_clamp64(p.row + shift + 1, 0, p.Lk) : p.Lk;
+    int64_t unbounded = p.Lk;                                        // first key of the first tile that was bounded
     const int64_t wave_all = a.causal ? vo_clamp64(p.row + wave * 32 + shift + 1, 0, p.Lk) : p.Lk;
     const int64_t wave_any = a.causal ? vo_clamp64(p.row + wave * 32 + 32 + shift, 0, p.Lk) : p.Lk;
 
@@ -330,9 +388,16 @@ __global__ __launch_bounds__(256, MIN_BLOCKS) void attention_tiles(const AttArgs
             fetch_v(t + 1, next + HALF);
         }
         const int64_t key = t * KEYS;
+        if (key + KEYS > all && all < p.Lk && core.any_unbounded(now + HALF, lane)) {        // all waves find the same
+            vo_lds_barrier();
+            core.bound(now + HALF, wave, 4, lane);
+            vo_lds_barrier();
+            unbounded = key < unbounded ? key : unbounded;
+        }
         if (key < wave_any) core.step(now, now + HALF, a.c, key + KEYS > wave_all, (int)vo_clamp64(limit - key, 0, KEYS), lane);
         unsigned char* x = now; now = next; next = x;
     }
+    if (unbounded < p.Lk) core.add_unbounded(vb, a.vs, unbounded, t1 * KEYS < p.Lk ? t1 * KEYS : p.Lk, limit, a.D, lane);
     const float l = core.across(core.l, [](float x, float y) { return x + y; });
     vo_lds_barrier();                                                // every wave is done with the key tiles
     const int64_t first = p.row + wave * 32;
@@ -395,7 +460,13 @@ __global__ __launch_bounds__(64 * WAVES) void attention_rows(const AttArgs a) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");             // tile t has arrived
         if (t + WAVES < t1) fetch(t + WAVES, mine + (stage ^ 1) * 2 * HALF);
         const int64_t key = t * KEYS;
+        const bool partial = key + KEYS > all && all < p.Lk && core.any_unbounded(now + HALF, lane);
+        if (partial) {
+            core.bound(now + HALF, 0, 1, lane);
+            vo_wave_lds_fence();
+        }
         core.step(now, now + HALF, a.c, key + KEYS > all, (int)vo_clamp64(limit - key, 0, KEYS), lane);
+        if (partial) core.add_unbounded(vb, a.vs, key, key + KEYS < p.Lk ? key + KEYS : p.Lk, limit, a.D, lane);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");           // its reads are done before it is loaded over
     }
     core.l = core.across(core.l, [](float x, float y) { return x + y; });
@@ -489,15 +560,21 @@ template <typename T, int WIDTH> __global__ __launch_bounds__(256) void attentio
     for (int d = 32; d; d >>= 1) l += __shfl_xor(l, d);
     const int f = lane % WIDTH * 4;
     float o[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int s0 = 0; s0 < a.splits; s0 += GROUPS) {
-        const int s = s0 + lane / WIDTH;
-        const float ws = __shfl(w, s & 63);
-        if (s < a.splits && ws != 0.f && f < a.D) {
-            const vo_f32x4 x = *reinterpret_cast<const vo_f32x4*>(part_row(a, s, token, head) + f);
+    for (int s0 = 0; s0 < a.splits; s0 += 4 * GROUPS) {              // four loads under way
+        float ws[4];
+        vo_f32x4 x[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) o[j] += ws * x[j];
+        for (int i = 0; i < 4; ++i) {
+            const int s = s0 + i * GROUPS + lane / WIDTH;
+            ws[i] = __shfl(w, s & 63);
+            if (s >= a.splits || f >= a.D) ws[i] = 0.f;
+            x[i] = vo_f32x4{0.f, 0.f, 0.f, 0.f};
+            if (ws[i] != 0.f) x[i] = *reinterpret_cast<const vo_f32x4*>(part_row(a, s, token, head) + f);
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[j] += ws[i] * x[i][j];
     }
 #pragma unroll
     for (int d = 32; d >= WIDTH; d >>= 1)
