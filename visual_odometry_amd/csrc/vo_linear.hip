@@ -417,10 +417,10 @@ template <typename T> __global__ __launch_bounds__(256) void linear_pad(const T*
 
 // ------------------------------------------------------------------------------------------------------------- host
 
-// Tiles: rows of x, outputs, slabs under way, resident workgroups per CU.  The estimated time of a product on a form is its rounds
-// over the CUs times a tile's work over the form's rate, which a short C does not reach (`ramp`: the C at which half of it is).
+// Tiles: rows of x, outputs; the share of the CU's rate that a tile reaches on a long C, in 16 bits and in float32; the C at which
+// half of that is reached (an eighth of it in float32, whose products take longer).
 // Measured on 16-bit products, us: 4096 x 4096 x 4096 on forms 3 / 4: 152 / 123; 2048 x 2048 x 2048 on 2 / 3 / 4: 32 / 36 / 49;
-// 38400 x 256 x 256 on 2 / 3 / 4: 19 / 25 / 26; float32 38400 x 256 x 256 on 2 / 3: 63 / 72.
+// 38400 x 256 x 256 on 2 / 3 / 4: 19 / 25 / 26; float32: 38400 x 256 x 256 on 2 / 3: 63 / 72, 4096 x 4096 x 4096: 985 / 973.
 struct Form { int bm, bn; float rate16, rate32, ramp; };
 constexpr Form FORMS[] = {{16, 16, 0, 0, 0}, {32, 64, 0, 0, 0}, {64, 64, 0.55f, 1.f, 100}, {128, 128, 0.75f, 1.05f, 500}, {256, 256, 1.f, 0.f, 800}};
 
@@ -437,7 +437,7 @@ Plan plan(int64_t M, int C, int K, int dtype) {
     Plan p{};
     // Unaligned rows cannot go straight into LDS, and through registers they run at less than half the rate: where the product
     // outweighs its operands they are copied to aligned rows first (3001 x 2777 x 3333 bfloat16: 183 us without the copies).
-    if (C % per && (double)M * K >= 512.0 * (M + K) && (double)M * K * C >= 1e9) {
+    if (C % per && (double)M * K >= (dtype == VO_F32 ? 96. : 512.) * (M + K) && (double)M * K * C >= 1e9) {
         C = (C + per - 1) / per * per;
         p.padded = (M + K) * C;
     }
@@ -445,30 +445,41 @@ Plan plan(int64_t M, int C, int K, int dtype) {
         // One row of 4096 x 4096 (bfloat16): 10 us by rows, 12 by split tiles and their join; 16 rows of 4096 x 16384: 39 by
         // rows, 31 by tiles that need no split.
         p.form = M <= 4 || (M <= 16 && vo_ceil_div(K, 64) < 192) ? 0 : 1;
+    }
+    int64_t splits = 1;
+    if (M <= 32) {
+        const int64_t tiles = vo_ceil_div(M, FORMS[p.form].bm) * vo_ceil_div(K, FORMS[p.form].bn);
+        const int64_t at_least = p.form == 0 ? 1024 : 512;           // elements of C worth a part
+        if (tiles < 192) splits = vo_ceil_div(256, tiles);
+        if (splits > C / at_least) splits = C / at_least;
+        if (splits > 16) splits = 16;
+        if (splits < 1) splits = 1;
     } else {
-        float best = 0.f;
+        // The form and the number of parts of C whose estimated time is least: rounds over the 256 CUs times a part's time, and
+        // the join's launch and traffic.  Fewer workgroups than two per CU do not hide their waits.
+        double best = 0.;
         for (int f = 2; f <= 4; ++f) {
-            const float rate = dtype == VO_F32 ? FORMS[f].rate32 : FORMS[f].rate16;
-            if (rate == 0.f) continue;
-            const int64_t tiles = vo_ceil_div(M, FORMS[f].bm) * vo_ceil_div(K, FORMS[f].bn);
-            const float cost = (float)vo_ceil_div(tiles, 256) * FORMS[f].bm * FORMS[f].bn * (C + FORMS[f].ramp) / rate;
-            if (p.form == 0 || cost < best) {
-                p.form = f;
-                best = cost;
+            const Form& form = FORMS[f];
+            const double rate = dtype == VO_F32 ? form.rate32 * 0.5e6 : form.rate16 * 4.7e6;        // operations per CU and us
+            if (rate == 0.) continue;
+            const double ramp = dtype == VO_F32 ? form.ramp / 8 : form.ramp;
+            const int64_t tiles = vo_ceil_div(M, form.bm) * vo_ceil_div(K, form.bn);
+            for (int n = 1; n <= 16 && (n == 1 || C / n >= 256); ++n) {
+                const int64_t blocks = tiles * n, rounds = vo_ceil_div(blocks, 256);
+                const double full = f == 4 ? 1. : blocks <= 256 ? 0.6 : blocks <= 512 ? 0.85 : 1.;
+                const double us = rounds * 2. * form.bm * form.bn * ((double)C / n + ramp) / (rate * full) +
+                                  (n > 1 ? 4. + n * (double)M * K * 8 / 4e6 : 0.);
+                if (p.form == 0 || us < best) {
+                    best = us;
+                    p.form = f;
+                    splits = n;
+                }
             }
         }
     }
     p.tiles_m = vo_ceil_div(M, FORMS[p.form].bm);
     p.tiles_n = vo_ceil_div(K, FORMS[p.form].bn);
     const int64_t tiles = p.tiles_m * p.tiles_n;
-    int64_t splits = 1;
-    const int64_t at_least = p.form == 0 ? 1024 : 512;               // elements of C worth a split
-    if (tiles < 192) {
-        splits = vo_ceil_div(256, tiles);
-        if (splits > C / at_least) splits = C / at_least;
-        if (splits > 16) splits = 16;
-        if (splits < 1) splits = 1;
-    }
     p.c_per_split = (int)vo_ceil_div(vo_ceil_div(C, slab), splits) * slab;
     p.splits = (int)vo_ceil_div(C, p.c_per_split);
     p.deep = tiles * p.splits <= 512;                                // 512 x 2048 x 2048: 14 us against 20; 2048^3: 37 against 32
