@@ -89,14 +89,18 @@ template <typename T, int DT, int KEYS> struct Core {
 #pragma unroll
             for (int j = 0; j < 16; ++j) s[b][j] = 0.f;
 #pragma unroll
-        for (int i = 0; i < QS; ++i)
+        for (int i = 0; i < QS; ++i) {
+            vo_u32x4 k[KB];
 #pragma unroll
             for (int b = 0; b < KB; ++b) {
                 const int r = b * 32 + (lane & 31);
-                const vo_u32x4 kf = *reinterpret_cast<const vo_u32x4*>(kt + r * L::ROW + (((i * 2 + (lane >> 5)) ^ L::k_swz(r)) * 16));
-#pragma unroll
-                for (int part = 0; part < E::PARTS; ++part) s[b] = E::mma32(kf, q[i], s[b], part);
+                k[b] = *reinterpret_cast<const vo_u32x4*>(kt + r * L::ROW + (((i * 2 + (lane >> 5)) ^ L::k_swz(r)) * 16));
             }
+#pragma unroll
+            for (int part = 0; part < E::PARTS; ++part)
+#pragma unroll
+                for (int b = 0; b < KB; ++b) s[b] = E::mma32(k[b], q[i], s[b], part);
+        }
     }
     // The lane's row sees the tile's keys below `limit`.
     static __device__ __forceinline__ void mask(vo_f32x16* s, int limit, int lane) {
