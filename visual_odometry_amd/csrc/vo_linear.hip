@@ -162,8 +162,8 @@ __global__ __launch_bounds__(64 * WGM * WGN) void linear_tiles(const LinArgs a) 
             first[o][q] = (unsigned)((tile_row(i) - q * 8 + sub) * (o == 0 ? xb : wb)) + chunk(i) * 16;
             ahead_of[o][q] = chunk(i) * PER;
         }
-    vo_u32x4 reg[DIRECT ? 1 : LOADS];
-    auto fetch = [&](int s, unsigned char* buf) {
+    struct Regs { vo_u32x4 r[DIRECT ? 1 : LOADS]; } regs;             // unaligned rows pass through registers
+    auto fetch = [&](int s, unsigned char* buf, Regs& regs) {
         const int c0 = c_first + s * BK;
         if constexpr (DIRECT) {
 #pragma unroll
@@ -173,22 +173,37 @@ __global__ __launch_bounds__(64 * WGM * WGN) void linear_tiles(const LinArgs a) 
                 vo_load_to_lds(o == 0 ? xrs : wrs, buf + (o == 0 ? 0 : BM * 128) + tile_row(i) * 128,
                                ahead_of[o][j & 1] < c_last - c0 ? at : VO_OUTSIDE);
             }
+        } else if (a.C >= PER) {
+            // a row's last, shorter piece is fetched as the row's last 16 bytes and moved down when it is put into LDS
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) {
+                const int r = tile_row(i) + sub, c = c0 + chunk(i) * PER, gone = c + PER > c_last ? c + PER - c_last : 0;
+                regs.r[i] = vo_u32x4{0, 0, 0, 0};
+                if (gone < PER && r < (is_x(i) ? rows_x : rows_w))
+                    regs.r[i] = vo_load16((is_x(i) ? xt + r * a.xs : wt + (int64_t)r * a.C) + c - gone);
+            }
         } else {
 #pragma unroll
             for (int i = 0; i < LOADS; ++i) {
-                const int r = tile_row(i) + sub;
-                const bool in = r < (is_x(i) ? rows_x : rows_w);
-                const int c = c0 + chunk(i) * PER;
+                const int r = tile_row(i) + sub, c = c0 + chunk(i) * PER;
                 const T* p = (is_x(i) ? xt + r * a.xs : wt + (int64_t)r * a.C) + c;
-                reg[i] = vo_load_unaligned<T>(p, in ? c_last - c : 0);
+                regs.r[i] = vo_load_unaligned<T>(p, r < (is_x(i) ? rows_x : rows_w) ? c_last - c : 0, c);
             }
         }
     };
-    auto put = [&](unsigned char* buf) {
+    auto put = [&](int s, unsigned char* buf, Regs& regs) {
         if constexpr (!DIRECT) {
+            const int c0 = c_first + s * BK;
+            if (c0 + BK > c_last && a.C >= PER) {
+#pragma unroll
+                for (int i = 0; i < LOADS; ++i) {
+                    const int gone = c0 + chunk(i) * PER + PER - c_last;
+                    if (gone > 0 && gone < PER) regs.r[i] = vo_move_down(regs.r[i], gone * (int)sizeof(T));
+                }
+            }
 #pragma unroll
             for (int i = 0; i < LOADS; ++i)
-                *reinterpret_cast<vo_u32x4*>(buf + (is_x(i) ? 0 : BM * 128) + tile_row(i) * 128 + lane * 16) = reg[i];
+                *reinterpret_cast<vo_u32x4*>(buf + (is_x(i) ? 0 : BM * 128) + tile_row(i) * 128 + lane * 16) = regs.r[i];
         }
     };
 
@@ -230,16 +245,15 @@ __global__ __launch_bounds__(64 * WGM * WGN) void linear_tiles(const LinArgs a) 
     auto after = [&](unsigned char* p) { return p + SLAB == lds + STAGES * SLAB ? lds : p + SLAB; };
     if constexpr (DIRECT) {
 #pragma unroll
-        for (int i = 0; i < STAGES; ++i) fetch(i, lds + i * SLAB);
+        for (int i = 0; i < STAGES; ++i) fetch(i, lds + i * SLAB, regs);
         vo_lds_barrier<(STAGES - 1) * LOADS>();
     } else {
-        fetch(0, nullptr);
-        put(lds);
-        if (slabs > 1) {
-            fetch(1, nullptr);
-            put(lds + SLAB);
-        }
-        if (slabs > 2) fetch(2, nullptr);
+        Regs second;
+        fetch(0, nullptr, regs);
+        if (slabs > 1) fetch(1, nullptr, second);
+        put(0, lds, regs);
+        if (slabs > 2) fetch(2, nullptr, regs);
+        if (slabs > 1) put(1, lds + SLAB, second);
         __syncthreads();
     }
     read(f0, buf, 0);
@@ -249,11 +263,11 @@ __global__ __launch_bounds__(64 * WGM * WGN) void linear_tiles(const LinArgs a) 
         interleave();
         if constexpr (DIRECT) {
             vo_lds_barrier<(STAGES - 2) * LOADS>();
-            fetch(s + STAGES, buf);
+            fetch(s + STAGES, buf, regs);
         } else {
             __syncthreads();
-            if (s + 2 < slabs) put(buf);
-            if (s + 3 < slabs) fetch(s + 3, nullptr);
+            if (s + 2 < slabs) put(s + 2, buf, regs);
+            if (s + 3 < slabs) fetch(s + 3, nullptr, regs);
         }
         buf = after(buf);
         read(f0, buf, 0);
@@ -351,8 +365,8 @@ __global__ __launch_bounds__(512) void linear_rows(const LinArgs a) {
                 wf[d] = __builtin_amdgcn_raw_buffer_load_b128(wrs, c < c_hi ? wo + at : VO_OUTSIDE, 0, 0);
                 xf[d] = __builtin_amdgcn_raw_buffer_load_b128(xrs, c < c_hi ? xo + at : VO_OUTSIDE, 0, 0);
             } else {
-                wf[d] = vo_load_unaligned<T>(w + (int64_t)fr * a.C + c, fr < rows_w ? c_hi - c : 0);
-                xf[d] = vo_load_unaligned<T>(x + fr * a.xs + c, fr < a.M ? c_hi - c : 0);
+                wf[d] = vo_load_unaligned<T>(w + (int64_t)fr * a.C + c, fr < rows_w ? c_hi - c : 0, c);
+                xf[d] = vo_load_unaligned<T>(x + fr * a.xs + c, fr < a.M ? c_hi - c : 0, c);
             }
         }
 #pragma unroll
@@ -412,7 +426,7 @@ template <typename T> __global__ __launch_bounds__(256) void linear_pad(const T*
     const int64_t row = piece / across;
     const int c = (int)(piece % across) * PER;
     const T* p = row < M ? x + row * xs : w + (row - M) * C;
-    *reinterpret_cast<vo_u32x4*>(out + piece * PER) = vo_load_unaligned<T>(p + c, C - c);
+    *reinterpret_cast<vo_u32x4*>(out + piece * PER) = vo_load_unaligned<T>(p + c, C - c, c);
 }
 
 // ------------------------------------------------------------------------------------------------------------- host

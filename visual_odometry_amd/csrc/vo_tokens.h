@@ -129,18 +129,34 @@ static __device__ __forceinline__ vo_u32x4 vo_load16(const void* p) {
 }
 static __device__ __forceinline__ void vo_store16(void* p, vo_u32x4 v) { __builtin_memcpy(p, &v, 16); }
 
-// `n` (< PER) or all PER elements of a row from any address: a wide load that needs no alignment, or element by element at
-// a row's end.  Missing elements are zero.
-template <typename T> static __device__ __forceinline__ vo_u32x4 vo_load_unaligned(const T* p, int64_t n) {
+// 16 bytes moved down by 0 to 15 bytes, zeros behind.
+static __device__ __forceinline__ vo_u32x4 vo_move_down(vo_u32x4 r, int bytes) {
+    const int bits = bytes * 8;
+    uint64_t lo = (uint64_t)r[1] << 32 | r[0], hi = (uint64_t)r[3] << 32 | r[2];
+    if (bits >= 64) {
+        lo = hi >> (bits - 64);
+        hi = 0;
+    } else if (bits > 0) {
+        lo = lo >> bits | hi << (64 - bits);
+        hi >>= bits;
+    }
+    return vo_u32x4{(unsigned)lo, (unsigned)(lo >> 32), (unsigned)hi, (unsigned)(hi >> 32)};
+}
+
+// PER elements of a row from p on, which may have any address; `n` of them exist (the others become zero) and `before` elements of
+// the row lie ahead of p.  A row's last, shorter piece is the row's last 16 bytes moved down.
+template <typename T> static __device__ __forceinline__ vo_u32x4 vo_load_unaligned(const T* p, int64_t n, int64_t before) {
     constexpr int PER = vo_elem<T>::PER;
     vo_u32x4 r = {0, 0, 0, 0};
     if (n >= PER) {
         r = vo_load16(p);
-    } else {
+    } else if (n > 0 && n + before >= PER) {
+        r = vo_move_down(vo_load16(p - (PER - n)), (PER - (int)n) * (int)sizeof(T));
+    } else if (n > 0) {
         float v[PER];
 #pragma unroll
         for (int j = 0; j < PER; ++j) v[j] = j < n ? vo_elem<T>::get(p + j) : 0.f;
-        r = vo_elem<T>::pack(v);                       // exact: the values come from the type itself
+        r = vo_elem<T>::pack(v);                                      // exact: the values come from the type itself
     }
     return r;
 }
