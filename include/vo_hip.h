@@ -622,7 +622,8 @@ int vo_ransac_kabsch_batch(const double* P, const double* Q, const uint8_t* weig
  *   activation  VO_ACT_*: GELU is 0.5 z (1 + erf(z/sqrt(2))), GELU_TANH its tanh form, SILU z / (1 + exp(-z)).
  *   dtype       VO_F32, VO_F16 or VO_BF16 of x, weight, residual and y.  Products and sums in float32, one rounding.
  * Any M >= 0, C >= 1, K >= 1 and any alignment; whole 16-byte pieces per row (C, strides and pointers) are read straight
- * into LDS, others through registers.  Rows of x and weight must be under 8 MiB (VO_ERR_UNSUPPORTED).
+ * into LDS, others through registers or from padded copies.  Rows of x and weight must be under 8 MiB, and a launch has
+ * fewer than 2^32 threads, which bounds M * K at some 10^10 (VO_ERR_UNSUPPORTED).
  * workspace: vo_linear_workspace_bytes(M, C, K, dtype) bytes (often 0), 16-byte aligned, contents irrelevant.  Calls that
  * share one must be ordered on one stream; two captured graphs that may replay at once need one each.
  * ------------------------------------------------------------------------- */
@@ -636,7 +637,7 @@ int vo_linear(const void* x, int64_t x_row_stride, const void* weight, const flo
 /* ---------------------------------------------------------------------------
  * Attention of packed sequences: row i of a sequence gives
  *     out[i,h,:] = sum_j p_ij v[j,h',:],   p_ij = softmax_j(scale * q[i,h,:] . k[j,h',:]),   h' = h / (q_heads / k_heads)
- * over the keys j of its sequence; with causal != 0 over those with j <= i + Lk - Lq (Lq, Lk the sequence's rows and keys:
+ * over the keys j of its sequence (scale from 1e-30 to 1e30); with causal != 0 over those with j <= i + Lk - Lq (Lq, Lk the sequence's rows and keys:
  * its last row sees every key).  A row that sees no key gives zeros.  It has NO counterpart in the reference; it is the
  * all-pairs product of vo_corr_volume_1d / _2d without the volume: along the epipolar lines of a stereo pair (one sequence
  * a line, causal: a match lies never right of its pixel), among all pixels of a frame, over packed prompts of any lengths,

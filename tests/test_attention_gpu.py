@@ -250,6 +250,52 @@ def test_equal_bits_on_another_stream_and_in_a_graph(vo, q_len, k_len):
         assert torch.equal(y, ops.attention(q, k, v, qo, ko, causal=True))
 
 
+def test_two_streams_at_once(vo):
+    """Calls that need workspaces, under way on two streams together."""
+    for q_len, k_len in (([1, 1], [5000, 3000]), ([60], [3000])):
+        sets = [make(q_len, k_len, 4, 2, 64, torch.bfloat16, 30 + i) for i in range(2)]
+        qo, ko = offsets(q_len), offsets(k_len)
+        want = [ops.attention(q, k, v, qo, ko, causal=True) for q, k, v in sets]
+        streams = [torch.cuda.Stream() for _ in sets]
+        for st in streams:
+            st.wait_stream(torch.cuda.current_stream())
+        got = [[], []]
+        for _ in range(20):
+            for i, (st, (q, k, v)) in enumerate(zip(streams, sets)):
+                with torch.cuda.stream(st):
+                    got[i].append(ops.attention(q, k, v, qo, ko, causal=True))
+        torch.cuda.synchronize()
+        assert all(torch.equal(y, want[i]) for i in range(2) for y in got[i])
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("q_len", [[40], [2]])
+def test_four_features_and_shared_heads_by_stride(vo, causal, q_len):
+    """The smallest float32 head, and key heads that are one head repeated by a stride of zero."""
+    q, k, v = make(q_len, [70], 6, 1, 4, torch.float32, 3)
+    y = ops.attention(q, k, v, causal=causal)
+    check(y, *reference(q, k, v, q_len, [70], causal, 0.5))
+    check(ops.attention(q, k.expand(70, 6, 4), v.expand(70, 6, 4), causal=causal), *reference(q, k, v, q_len, [70], causal, 0.5))
+
+
+def test_more_sequences_than_a_wave_tests_at_once(vo):
+    """Hundreds and thousands of sequences, empty ones and single tokens among them, in both forms."""
+    rng = np.random.default_rng(4)
+    for n, top in ((65, 3), (700, 2), (4500, 2), (130, 40)):
+        q_len = rng.integers(0, top + 1, n).tolist()
+        k_len = [int(x) for x in rng.integers(0, 9, n)]
+        q, k, v = make(q_len, k_len, 1, 1, 32, torch.float16, n)
+        y = ops.attention(q, k, v, offsets(q_len), offsets(k_len))
+        seq = np.repeat(np.arange(n), q_len)
+        pos = torch.tensor(np.repeat(np.arange(n), k_len)).cuda()
+        S = (q[:, 0].double() @ k[:, 0].double().t().contiguous()) * 32 ** -0.5
+        S = S.masked_fill(torch.tensor(seq).cuda()[:, None] != pos[None, :], -torch.inf)
+        P = torch.softmax(S, 1).nan_to_num(0)
+        want = P @ v[:, 0].double()
+        # a handful of keys a row: the weights' and the result's roundings, 2^-11 each of sum p |v| (<= 5 here), dominate
+        assert float((y[:, 0].double() - want).abs().max()) < 2 * 5 * 2.0 ** -11 * 1.1
+
+
 def test_a_long_cache_passes_32_bit_offsets(vo):
     """Keys and values more than 2^31 elements (and 2^32 bytes) apart: a cache of 70000 tokens at a stride of 32768."""
     n, D, stride = 70000, 64, 32768

@@ -142,6 +142,33 @@ def test_equal_inputs_give_equal_bits_also_on_another_stream(vo, M, C, K):
     assert all(torch.equal(y, want) for y in ys)
 
 
+@pytest.mark.parametrize("dtype,tiny", [(torch.float32, 2.0 ** -140), (torch.float16, 2.0 ** -24), (torch.bfloat16, 2.0 ** -130)])
+@pytest.mark.parametrize("M", [2, 40, 300])
+def test_subnormal_values_are_not_flushed(vo, dtype, tiny, M):
+    x = torch.zeros(M, 16, device="cuda", dtype=dtype)
+    x[:, 3] = tiny * torch.arange(1, M + 1, device="cuda").clamp(max=64)
+    w = torch.zeros(24, 16, device="cuda", dtype=dtype)
+    w[:, 3] = 1
+    assert float(x[0, 3]) > 0 and torch.equal(ops.linear(x, w), x[:, 3:4].expand(M, 24))
+
+
+@pytest.mark.parametrize("M,C,K", [(3, 8192, 64), (70, 4096, 64), (1201, 1003, 1100)])
+def test_two_streams_at_once(vo, M, C, K):
+    """Calls that need workspaces, under way on two streams together."""
+    sets = [make(M, C, K, torch.float16, 60 + i, res=True) for i in range(2)]
+    want = [ops.linear(x, w, b, "gelu", r) for x, w, b, r in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    for st in streams:
+        st.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(20):
+        for i, (st, (x, w, b, r)) in enumerate(zip(streams, sets)):
+            with torch.cuda.stream(st):
+                got[i].append(ops.linear(x, w, b, "gelu", r))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[i]) for i in range(2) for y in got[i])
+
+
 @pytest.mark.parametrize("M,C,K", [(1, 4096, 64), (70, 4096, 64), (300, 256, 256)])
 def test_captured_calls_replay_on_new_contents(vo, M, C, K):
     x, w, b, r = make(M, C, K, torch.float16, 4, res=True)

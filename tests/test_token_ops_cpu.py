@@ -76,6 +76,9 @@ def test_linear_entry_point_refuses():
         assert lib.vo_last_error()
     assert call(M=0) == _lib.VO_OK                                                  # nothing to do, nothing launched
     assert call(xs=1 << 22) == _lib.VO_ERR_UNSUPPORTED and call(xs=1 << 23, C=1 << 23) == _lib.VO_ERR_UNSUPPORTED
+    # more threads than a launch has
+    assert call(M=1 << 32, C=8, K=8) == _lib.VO_ERR_UNSUPPORTED and b"too large" in lib.vo_last_error()
+    assert call(M=1, C=8, K=(1 << 31) - 1, ys=1 << 31) == _lib.VO_ERR_UNSUPPORTED and b"too large" in lib.vo_last_error()
     # a shape that is split over C needs its workspace
     need = lib.vo_linear_workspace_bytes(1, 65536, 16, _lib.VO_PIECES_F16)
     assert need > 0
@@ -102,6 +105,8 @@ def test_attention_entry_point_refuses():
     for kw in (dict(D=0), dict(D=264), dict(D=12), dict(qs=60), dict(kh=4), dict(vs=-64), dict(os=1 << 23), dict(q=ctypes.c_void_p(p.value + 8)),
                dict(o=ctypes.c_void_p(p.value + 2)), dict(Tq=1 << 31), dict(Tk=1 << 31), dict(dt=0, D=30)):
         assert call(**kw) == _lib.VO_ERR_UNSUPPORTED, kw
+    assert call(Tq=(1 << 31) - 1, Hq=64, Hk=64) == _lib.VO_ERR_UNSUPPORTED and b"too many" in lib.vo_last_error()
+    assert call(scale=1e-38) == _lib.VO_ERR_INVALID_ARG and call(scale=1e38) == _lib.VO_ERR_INVALID_ARG
     assert call(Tq=0) == _lib.VO_OK
     need = lib.vo_attention_workspace_bytes(1, 65536, 1, 2, 2, 32, 1)
     assert need > 0 and call(Tq=1, Tk=65536) == _lib.VO_ERR_INVALID_ARG and b"workspace" in lib.vo_last_error()

@@ -688,7 +688,7 @@ extern "C" int vo_attention(const void* q, int64_t q_token_stride, int64_t q_hea
     VO_REQUIRE(sequences >= 1 && q_tokens >= 0 && k_tokens >= 0 && q_heads >= 1 && k_heads >= 1 && q_heads % k_heads == 0,
                "vo_attention: sequences=%d q_tokens=%lld k_tokens=%lld heads %d / %d (heads a multiple of the key heads)", sequences,
                (long long)q_tokens, (long long)k_tokens, q_heads, k_heads);
-    VO_REQUIRE(scale > 0.f && scale < INFINITY, "vo_attention: scale must be positive and finite");
+    VO_REQUIRE(scale >= 1e-30f && scale <= 1e30f, "vo_attention: scale must be positive (1e-30 to 1e30)");
     VO_REQUIRE((q_offsets && k_offsets) || (!q_offsets && !k_offsets && sequences == 1),
                "vo_attention: both offset arrays, or none and one sequence");
     const int64_t es = dtype == VO_F32 ? 4 : 2;
@@ -704,7 +704,7 @@ extern "C" int vo_attention(const void* q, int64_t q_token_stride, int64_t q_hea
     if (q_tokens >= (1ll << 31) || k_tokens >= (1ll << 31))
         return vo_fail(VO_ERR_UNSUPPORTED, "vo_attention: offsets are 32-bit: fewer than 2^31 tokens");
     const Plan p = plan(q_tokens, k_tokens, sequences, q_heads, k_heads, D, dtype);
-    if (p.blocks >= (1ll << 31) || q_tokens * q_heads >= (1ll << 32))
+    if (p.blocks * 256 >= (1ll << 32) || (p.splits > 1 && q_tokens * q_heads * 64 >= (1ll << 32)))      // threads of a launch
         return vo_fail(VO_ERR_UNSUPPORTED, "vo_attention: %lld tokens of %d heads are too many for one launch", (long long)q_tokens, q_heads);
     const int64_t need = workspace(p, q_tokens, q_heads, D);
     VO_REQUIRE(need == 0 || (workspace_ptr && workspace_bytes >= need && reinterpret_cast<uintptr_t>(workspace_ptr) % 16 == 0),

@@ -571,8 +571,11 @@ extern "C" int vo_linear(const void* x, int64_t x_row_stride, const void* weight
     // a tile's rows are addressed with 32-bit offsets
     if (x_row_stride * es * 256 >= (1ll << 31) || (int64_t)C * es * 256 >= (1ll << 31))
         return vo_fail(VO_ERR_UNSUPPORTED, "vo_linear: rows of x and weight must be under 8 MiB");
-    if (p.tiles_m * p.tiles_n * p.splits * 4 >= (1ll << 31) || M * vo_ceil_div(K, 4) >= (1ll << 38))
-        return vo_fail(VO_ERR_UNSUPPORTED, "vo_linear: M=%lld K=%d is too large for one launch", (long long)M, K);
+    // a launch has fewer than 2^32 threads (large forms may be run as tiles of half the side)
+    const int64_t limit = 1ll << 32;
+    if (p.tiles_m * p.tiles_n * p.splits * (p.form == 0 ? 512 : 1024) >= limit || M * vo_ceil_div(K, 4) >= limit * 64 ||
+        (p.splits > 1 && M * vo_ceil_div(K, 16 / es) >= limit) || p.padded / (16 / es) >= limit)
+        return vo_fail(VO_ERR_UNSUPPORTED, "vo_linear: M=%lld C=%d K=%d is too large for one launch", (long long)M, C, K);
     const int64_t need = needed(p, M, K, dtype);
     VO_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
                "vo_linear: needs a 16-byte aligned workspace of %lld bytes", (long long)need);

@@ -1172,7 +1172,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     epilogue are float32 with one rounding at the store.  ``activation``: None, "relu", "gelu" (the error function's form),
     "gelu_tanh" or "silu"; it comes before the residual is added.  Rows of x, residual and out may lie any distance apart
     (slices of wider tensors), a row's elements are consecutive; weight is contiguous.  ``out`` may be the residual itself;
-    it must not overlap anything else.  Sums are formed in a fixed order: equal inputs give equal bits."""
+    it must not overlap anything else.  Sums are formed in a fixed order: equal inputs give equal bits.  Forward only: nothing is
+    recorded for autograd."""
     _token_tensor(x, "x")
     _token_tensor(weight, "weight", x)
     if weight.dim() != 2 or not weight.is_contiguous() or weight.numel() == 0:
@@ -1233,7 +1234,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: torc
     ``scale`` defaults to 1/sqrt(D).  float32, float16 or bfloat16; scores, softmax and sums in float32.  Tokens and heads may
     lie any whole number of 16-byte pieces apart (slices of a fused projection); D is at most 256 and a multiple of 8 (4 in
     float32).  Rows outside every sequence are not written (give ``out`` to say what they hold).  The lengths stay on the
-    device: nothing synchronises, and the call can be captured.  Equal inputs give equal bits."""
+    device: nothing synchronises, and the call can be captured.  Equal inputs give equal bits.  Forward only: nothing is recorded
+    for autograd."""
     _token_tensor(q, "q")
     _token_tensor(k, "k", q)
     _token_tensor(v, "v", q)
