@@ -375,7 +375,7 @@ __global__ __launch_bounds__(256, MIN_BLOCKS) void attention_tiles(const AttArgs
     const int64_t all = a.causal ? vo_clamp64(p.row + shift + 1, 0, p.Lk) : p.Lk;
     int64_t unbounded = p.Lk;                                        // first key of the first tile that was bounded
     const int64_t wave_all = a.causal ? vo_clamp64(p.row + wave * 32 + shift + 1, 0, p.Lk) : p.Lk;
-    const int64_t wave_any = a.causal ? vo_clamp64(p.row + wave * 32 + 32 + shift, 0, p.Lk) : p.Lk;
+    const int64_t wave_any = p.row + wave * 32 >= p.Lq ? 0 : a.causal ? vo_clamp64(p.row + wave * 32 + 32 + shift, 0, p.Lk) : p.Lk;
 
     const T* kb = static_cast<const T*>(a.k) + p.k0 * a.ks + kh * a.kh;
     const T* vb = static_cast<const T*>(a.v) + p.k0 * a.vs + kh * a.vh;
