@@ -103,7 +103,7 @@ def test_lengths(vo, dtype, causal, q_len, k_len, Hq, Hk):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("Hq,Hk", [(1, 1), (7, 1), (32, 8), (40, 1), (6, 3)])
+@pytest.mark.parametrize("Hq,Hk", [(1, 1), (7, 1), (32, 8), (40, 1), (6, 3), (128, 1), (129, 1), (260, 2)])
 @pytest.mark.parametrize("q_len,k_len", [([1, 1, 1], [700, 3, 90]), ([4, 2, 7], [300, 2, 50]), ([150], [150])])
 def test_groups_of_heads(vo, dtype, Hq, Hk, q_len, k_len):
     run(q_len, k_len, Hq, Hk, 32, dtype, True, Hq)

@@ -16,8 +16,8 @@
 // then at most 256, which costs no bits in a floating-point format).
 //
 // Two forms:
-//   tiles  a workgroup of four waves takes 128 rows of one head; key tiles are shared in LDS, loaded while the previous
-//          tile is multiplied.  Matrix and vector work of a tile take about as long as each other and overlap between the two
+//   tiles  a workgroup of four waves takes 128 rows of one key head (a row is a token and one of the heads that share the key
+//          head); key tiles are shared in LDS, loaded while the previous tile is multiplied.  Matrix and vector work of a tile take about as long as each other and overlap between the two
 //          to four workgroups of a CU; the chip's power sets the clock (the same cycles are 38 % faster on zeros).  8 prompts of
 //          up to 8192 tokens, 32 / 8 heads of 128, bfloat16, causal: 2.04 ms = 1.02 PFLOP/s; 4800 float32 rows, 4 heads of 64:
 //          229 us = 103 TFLOP/s of the 151 the library's product reaches.
@@ -44,6 +44,7 @@ struct AttArgs {
     int64_t Tq, Tk;
     int sequences, Hq, Hk, group, D, causal, splits;
     unsigned tiles;                               // row tiles over all sequences (an upper bound)
+    unsigned reciprocal;                          // 2^16 / group rounded up, 0 for groups over 128
     float c;                                      // scale * log2(e)
 };
 
@@ -347,35 +348,40 @@ __global__ __launch_bounds__(256, MIN_BLOCKS) void attention_tiles(const AttArgs
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
     // numbers: key head outermost (an XCD keeps to few of them: their keys stay in its L2), then split, then row tiles from
-    // the last (the longest ones of a causal sequence come first), then the heads of the group
+    // the last (the longest ones of a causal sequence come first)
     const unsigned id = vo_xcd_contiguous(blockIdx.x, gridDim.x);
-    const int g = id % a.group;
-    unsigned rest = id / a.group;
-    const unsigned tile = a.tiles - 1 - rest % a.tiles;
-    rest /= a.tiles;
-    const int split = rest % a.splits, kh = rest / a.splits, head = kh * a.group + g;
-    const vo_place p = vo_find_tile(a.q_off, a.k_off, a.sequences, a.Tq, a.Tk, tile, 1, ROWS);
+    const unsigned tile = a.tiles - 1 - id % a.tiles;
+    const int split = id / a.tiles % a.splits, kh = id / a.tiles / a.splits;
+    const vo_place p = vo_find_tile(a.q_off, a.k_off, a.sequences, a.Tq, a.Tk, tile, a.group, ROWS);
     if (!p.any) return;
 
-    const int64_t shift = p.Lk - p.Lq;
-    const int64_t last_row = p.row + ROWS < p.Lq ? p.row + ROWS : p.Lq;                      // one past the tile's rows
-    int64_t seen = a.causal ? last_row + shift : p.Lk;                                       // keys that some row sees
+    // row r of the tile is head (r + skew) % group of token (r + skew) / group, counted from the tile's first token
+    const int64_t shift = p.Lk - p.Lq, first_token = p.row / a.group;
+    const int skew = (int)(p.row - first_token * a.group);
+    const int rows = (int)(p.Lq * a.group - p.row < ROWS ? p.Lq * a.group - p.row : ROWS);
+    // (x / group by multiplication: exact while x times the reciprocal's excess, under 256 * 128, stays below 2^16)
+    auto by_group = [&](unsigned x) { return a.reciprocal ? x * a.reciprocal >> 16 : x / (unsigned)a.group; };
+    auto token_of = [&](int r) { return first_token + by_group(r + skew); };
+    auto head_of = [&](int r) { return kh * a.group + (int)(r + skew - by_group(r + skew) * a.group); };
+    int64_t seen = a.causal ? token_of(rows - 1) + 1 + shift : p.Lk;                         // keys that some row sees
     seen = vo_clamp64(seen, 0, p.Lk);
     const int64_t key_tiles = (seen + KEYS - 1) / KEYS, per = (key_tiles + a.splits - 1) / a.splits;
     const int64_t t0 = split * per < key_tiles ? split * per : key_tiles, t1 = t0 + per < key_tiles ? t0 + per : key_tiles;
 
-    const int64_t row = p.row + wave * 32 + (lane & 31);
-    const bool have = row < p.Lq;
+    const int first = wave * 32, row = first + (lane & 31);
+    const bool have = row < rows;
+    const int64_t token = token_of(row);
+    const int head = head_of(row);
     Core<T, DT, KEYS> core;
     core.reset();
-    core.load_q(have ? static_cast<const T*>(a.q) + (p.q0 + row) * a.qs + head * a.qh : nullptr, a.D, lane);
+    core.load_q(have ? static_cast<const T*>(a.q) + (p.q0 + token) * a.qs + head * a.qh : nullptr, a.D, lane);
     // keys below `limit` are seen by this lane's row; tiles wholly below wave_all need no mask, from wave_any on no work; tiles
     // wholly below `all` are seen by every row of the workgroup
-    const int64_t limit = a.causal ? vo_clamp64(row + shift + 1, 0, p.Lk) : p.Lk;
-    const int64_t all = a.causal ? vo_clamp64(p.row + shift + 1, 0, p.Lk) : p.Lk;
+    const int64_t limit = a.causal ? vo_clamp64(token + shift + 1, 0, p.Lk) : p.Lk;
+    const int64_t all = a.causal ? vo_clamp64(first_token + shift + 1, 0, p.Lk) : p.Lk;
     int64_t unbounded = p.Lk;                                        // first key of the first tile that was bounded
-    const int64_t wave_all = a.causal ? vo_clamp64(p.row + wave * 32 + shift + 1, 0, p.Lk) : p.Lk;
-    const int64_t wave_any = p.row + wave * 32 >= p.Lq ? 0 : a.causal ? vo_clamp64(p.row + wave * 32 + 32 + shift, 0, p.Lk) : p.Lk;
+    const int64_t wave_all = a.causal ? vo_clamp64(token_of(first) + shift + 1, 0, p.Lk) : p.Lk;
+    const int64_t wave_any = first >= rows ? 0 : a.causal ? vo_clamp64(token_of(first + 31) + shift + 1, 0, p.Lk) : p.Lk;
 
     const T* kb = static_cast<const T*>(a.k) + p.k0 * a.ks + kh * a.kh;
     const T* vb = static_cast<const T*>(a.v) + p.k0 * a.vs + kh * a.vh;
@@ -408,14 +414,15 @@ __global__ __launch_bounds__(256, MIN_BLOCKS) void attention_tiles(const AttArgs
     if (unbounded < p.Lk) core.add_unbounded(vb, a.vs, unbounded, t1 * KEYS < p.Lk ? t1 * KEYS : p.Lk, limit, a.D, lane);
     const float l = core.across(core.l, [](float x, float y) { return x + y; });
     vo_lds_barrier();                                                // every wave is done with the key tiles
-    const int64_t first = p.row + wave * 32;
     if (a.splits > 1) {
-        store_rows<float, DT>(core.o, 1.f, a.D, lds + wave * HALF, lane,
-                              [&](int r) { return first + r < p.Lq ? part_row(a, split, p.q0 + first + r, head) : nullptr; });
-        if (have && lane < 32) *reinterpret_cast<float2*>(part_ml(a, split, p.q0 + row, head)) = make_float2(core.m * a.c, l);
+        store_rows<float, DT>(core.o, 1.f, a.D, lds + wave * HALF, lane, [&](int r) {
+            return first + r < rows ? part_row(a, split, p.q0 + token_of(first + r), head_of(first + r)) : nullptr;
+        });
+        if (have && lane < 32) *reinterpret_cast<float2*>(part_ml(a, split, p.q0 + token, head)) = make_float2(core.m * a.c, l);
     } else {
-        store_rows<T, DT>(core.o, inverse(l), a.D, lds + wave * HALF, lane,
-                          [&](int r) { return first + r < p.Lq ? out_row<T>(a, p.q0 + first + r, head) : nullptr; });
+        store_rows<T, DT>(core.o, inverse(l), a.D, lds + wave * HALF, lane, [&](int r) {
+            return first + r < rows ? out_row<T>(a, p.q0 + token_of(first + r), head_of(first + r)) : nullptr;
+        });
     }
 }
 
@@ -612,8 +619,8 @@ Plan plan(int64_t Tq, int64_t Tk, int sequences, int Hq, int Hk, int D, int dtyp
     const int64_t rows = vo_ceil_div(Tq * group, sequences);         // a sequence's rows per key head, on average
     const int64_t keys = vo_ceil_div(Tk, sequences);
     p.rows = rows <= 32;
-    p.tiles = p.rows ? vo_tiles_bound(Tq, sequences, group, 32) : vo_tiles_bound(Tq, sequences, 1, 128);
-    const int64_t base = p.tiles * (p.rows ? Hk : Hq);
+    p.tiles = vo_tiles_bound(Tq, sequences, group, p.rows ? 32 : 128);
+    const int64_t base = p.tiles * Hk;
     int64_t splits = 1;
     if (p.rows) {
         // About eight rounds over the CUs even out sequences of different lengths (32 sequences of up to 32768 keys, 8 key heads:
@@ -718,6 +725,7 @@ extern "C" int vo_attention(const void* q, int64_t q_token_stride, int64_t q_hea
     a.sequences = sequences; a.Hq = q_heads; a.Hk = k_heads; a.group = q_heads / k_heads;
     a.D = D; a.causal = causal != 0; a.splits = p.splits;
     a.tiles = (unsigned)p.tiles;
+    a.reciprocal = a.group <= 128 ? (65535u + a.group) / a.group : 0;
     a.c = scale * LOG2E;
     hipStream_t st = vo_stream(stream);
     if (dtype == VO_F32) return dispatch<float>(a, p, st);
