@@ -218,6 +218,32 @@ def test_unbounded_keys_and_values_reach_only_the_rows_that_see_them(vo, dtype, 
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("q_len,k_len", [([200], [200]), ([140], [4000]), ([3], [90]), ([3], [4000])])
+def test_a_row_of_nan_stays_nan(vo, dtype, q_len, k_len):
+    """A query that is not a number has no result, also where its keys are cut into parts; its neighbours do not notice."""
+    q, k, v = make(q_len, k_len, 2, 1, 64, dtype, 11)
+    want, tol = reference(q, k, v, q_len, k_len, False, 0.125)
+    q[1, 1, 5] = float("nan")
+    y = ops.attention(q, k, v)
+    assert bool(y[1, 1].isnan().all())
+    want[1, 1] = tol[1, 1] = 0
+    y[1, 1] = 0
+    check(y, want, tol)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("what", ["key", "value"])
+@pytest.mark.parametrize("q_len,k_len", [([140], [140]), ([140], [4000]), ([3], [90]), ([3], [4000])])
+def test_nan_among_keys_of_no_weight_is_not_lost(vo, dtype, what, q_len, k_len):
+    """The first keys' weights underflow to zero beside the last key's, a NaN among them (in a part of their own, where the keys
+    are cut) still reaches every row that sees it."""
+    q, k, v = make(q_len, k_len, 1, 1, 64, dtype, 12)
+    q[:], k[:], k[-1] = 8.0, -1.0, 8.0                                # scores -64 and 512: e^-576 is no float32
+    (k if what == "key" else v)[2, 0] = float("nan")
+    assert bool(ops.attention(q, k, v).isnan().all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_without_offsets_everything_is_one_sequence(vo, dtype):
     q, k, v = make([200], [333], 4, 4, 64, dtype, 1)
     assert torch.equal(ops.attention(q, k, v, causal=True), ops.attention(q, k, v, offsets([200]), offsets([333]), causal=True))

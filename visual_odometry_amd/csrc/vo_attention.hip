@@ -569,8 +569,9 @@ template <typename T, int WIDTH> __global__ __launch_bounds__(256) void attentio
     float m = ml.x;
 #pragma unroll
     for (int d = 32; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
-    const float w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - m);       // 0: that part saw no key of this row
-    float l = w == 0.f ? 0.f : w * ml.y;
+    const float w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - m);
+    const uint64_t sees = __ballot(ml.y != 0.f);                     // the other parts saw no key of this row; a NaN counts
+    float l = w * ml.y;
 #pragma unroll
     for (int d = 32; d; d >>= 1) l += __shfl_xor(l, d);
     const int f = lane % WIDTH * 4;
@@ -582,9 +583,8 @@ template <typename T, int WIDTH> __global__ __launch_bounds__(256) void attentio
         for (int i = 0; i < 4; ++i) {
             const int s = s0 + i * GROUPS + lane / WIDTH;
             ws[i] = __shfl(w, s & 63);
-            if (s >= a.splits || f >= a.D) ws[i] = 0.f;
             x[i] = vo_f32x4{0.f, 0.f, 0.f, 0.f};
-            if (ws[i] != 0.f) x[i] = *reinterpret_cast<const vo_f32x4*>(part_row(a, s, token, head) + f);
+            if (s < a.splits && f < a.D && (sees >> s & 1)) x[i] = *reinterpret_cast<const vo_f32x4*>(part_row(a, s, token, head) + f);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i)
