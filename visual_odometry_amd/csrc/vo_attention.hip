@@ -427,11 +427,16 @@ __global__ __launch_bounds__(256, MIN_BLOCKS) void attention_tiles(const AttArgs
 }
 
 // ------------------------------------------------------------------------------------------------------------- rows
+// A wave keeps one tile of K and one of V: the next K is requested as soon as the scores are formed, the next V after the sums, so
+// one of the two is always under way.  Tiles past the end are requested too (as zeros, without any traffic): the number of
+// loads under way is always the same.
 template <typename T, int DT, int KEYS, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void attention_rows(const AttArgs a) {
     using L = Tile<T, DT>;
-    constexpr int HALF = KEYS * L::ROW, MINE = 4 * HALF;             // a wave's two stages of K and V
+    constexpr int HALF = KEYS * L::ROW, MINE = 2 * HALF, PLANE = DT * 32 * 4;
+    static_assert(PLANE <= MINE, "a wave's sums must fit its tiles");
     __shared__ __align__(16) unsigned char lds[WAVES * MINE];
+    __shared__ float ml[WAVES][2][32];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const unsigned id = vo_xcd_contiguous(blockIdx.x, gridDim.x);
     const int split = id % a.splits;
@@ -464,89 +469,83 @@ __global__ __launch_bounds__(64 * WAVES) void attention_rows(const AttArgs a) {
     Loader<T, DT, KEYS, 1> lk, lv;
     lk.init(a.ks, a.D, false, 0, lane);
     lv.init(a.vs, a.D, true, 0, lane);
-    auto fetch = [&](int64_t t, unsigned char* buf) {                // 2 * N loads into the wave's own LDS
-        lk.load(kb + t * KEYS * a.ks, a.ks, p.Lk - t * KEYS, a.D, buf, 0);
-        lv.load(vb + t * KEYS * a.vs, a.vs, p.Lk - t * KEYS, a.D, buf + HALF, 0);
-    };
-    if (t0 + wave < t1) fetch(t0 + wave, mine);
-    int stage = 0;
-    for (int64_t t = t0 + wave; t < t1; t += WAVES, stage ^= 1) {
-        unsigned char* now = mine + stage * 2 * HALF;
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");             // tile t has arrived
-        if (t + WAVES < t1) fetch(t + WAVES, mine + (stage ^ 1) * 2 * HALF);
+    unsigned char *kt = mine, *vt = mine + HALF;
+    auto left = [&](int64_t t) { return t < t1 ? p.Lk - t * KEYS : 0; };
+    auto fetch_k = [&](int64_t t) { lk.load(kb + t * KEYS * a.ks, a.ks, left(t), a.D, kt, 0); };
+    auto fetch_v = [&](int64_t t) { lv.load(vb + t * KEYS * a.vs, a.vs, left(t), a.D, vt, 0); };
+    constexpr int N = Loader<T, DT, KEYS, 1>::N;
+    static_assert(N < 64, "the counter has six bits");
+    auto arrived = [] { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); };          // all but the N youngest loads
+    auto consumed = [] { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); };                // a tile's reads, before it is loaded over
+    if (t0 + wave < t1) {
+        fetch_k(t0 + wave);
+        fetch_v(t0 + wave);
+    }
+    for (int64_t t = t0 + wave; t < t1; t += WAVES) {
         const int64_t key = t * KEYS;
-        const bool partial = key + KEYS > all && all < p.Lk && core.any_unbounded(now + HALF, lane);
+        vo_f32x16 s[core.KB];
+        unsigned w[core.KB][core.PW];
+        arrived();
+        core.scores(kt, s, lane);
+        consumed();
+        fetch_k(t + WAVES);
+        if (key + KEYS > all) core.mask(s, (int)vo_clamp64(limit - key, 0, KEYS), lane);
+        core.follow(core.largest(s), a.c);
+        core.weights(s, w, a.c);
+        arrived();
+        const bool partial = key + KEYS > all && all < p.Lk && core.any_unbounded(vt, lane);
         if (partial) {
-            core.bound(now + HALF, 0, 1, lane);
+            core.bound(vt, 0, 1, lane);
             vo_wave_lds_fence();
         }
-        core.step(now, now + HALF, a.c, key + KEYS > all, (int)vo_clamp64(limit - key, 0, KEYS), lane);
+        core.accumulate(vt, w, lane);
+        consumed();
+        fetch_v(t + WAVES);
         if (partial) core.add_unbounded(vb, a.vs, key, key + KEYS < p.Lk ? key + KEYS : p.Lk, limit, a.D, lane);
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");           // its reads are done before it is loaded over
     }
     core.l = core.across(core.l, [](float x, float y) { return x + y; });
 
-    // join the waves in order: sums as (feature, row) planes of LDS, m and l behind them
-    constexpr int PLANE = DT * 33 * 4;                               // 33: lanes of one row apart in banks
-    static_assert(PLANE + 256 <= MINE || WAVES == 1, "the join must fit the wave's stages");
-    float* ml = reinterpret_cast<float*>(lds + wave * MINE + PLANE);
-    float m = core.m, l = core.l;
-    if constexpr (WAVES > 1) {
-        float* sums = reinterpret_cast<float*>(mine);
-        // every wave's own stages are free here: its loads have landed and its reads are done
+    // Join the waves in order: sums as (feature, row) planes over the wave's own tiles, where nothing is under way any more.  Features
+    // four apart (the two halves of a wave) change places with a neighbour so that they meet other banks.
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    auto at = [&](int f) { return (f ^ (f >> 2 & 1)) * 32 + (lane & 31); };
+    float* sums = reinterpret_cast<float*>(mine);
 #pragma unroll
-        for (int d = 0; d < DT / 32; ++d)
+    for (int d = 0; d < DT / 32; ++d)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) sums[(d * 32 + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3)) * 33 + (lane & 31)] = core.o[d][i];
-        if (lane < 32) { ml[lane] = core.m; ml[32 + lane] = core.l; }
-        __syncthreads();
-        float w[WAVES];
-        m = -INFINITY;
-        l = 0.f;
+        for (int i = 0; i < 16; ++i) sums[at(d * 32 + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3))] = core.o[d][i];
+    if (lane < 32) {
+        ml[wave][0][lane] = core.m;
+        ml[wave][1][lane] = core.l;
+    }
+    __syncthreads();
+    float w[WAVES], m = -INFINITY, l = 0.f;
 #pragma unroll
-        for (int i = 0; i < WAVES; ++i) m = fmaxf(m, reinterpret_cast<const float*>(lds + i * MINE + PLANE)[lane & 31]);
+    for (int i = 0; i < WAVES; ++i) m = fmaxf(m, ml[i][0][lane & 31]);
 #pragma unroll
-        for (int i = 0; i < WAVES; ++i) {
-            const float* x = reinterpret_cast<const float*>(lds + i * MINE + PLANE);
-            w[i] = m == -INFINITY ? 0.f : exp2f((x[lane & 31] - m) * a.c);
-            l += w[i] * x[32 + (lane & 31)];
+    for (int i = 0; i < WAVES; ++i) {
+        w[i] = m == -INFINITY ? 0.f : exp2f((ml[i][0][lane & 31] - m) * a.c);
+        l += w[i] * ml[i][1][lane & 31];
+    }
+    // eight features, four to each half of the wave, at a time: wave w takes the pieces w, w + WAVES, ..
+    const float inv = inverse(l);
+    for (int piece = wave; piece < DT / 8; piece += WAVES) {
+        const int f = piece * 8 + 4 * (lane >> 5);
+        float v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            v[j] = 0.f;
+#pragma unroll
+            for (int i = 0; i < WAVES; ++i) v[j] += w[i] * reinterpret_cast<const float*>(lds + i * MINE)[at(f + j)];
         }
-        // wave w finishes the feature blocks w, w + WAVES, ..
-        const float inv = inverse(l);
-        for (int d = wave; d < DT / 32; d += WAVES) {
-#pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                const int f = d * 32 + 8 * b + 4 * (lane >> 5);
-                float v[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    v[j] = 0.f;
-#pragma unroll
-                    for (int i = 0; i < WAVES; ++i) v[j] += w[i] * reinterpret_cast<const float*>(lds + i * MINE)[(f + j) * 33 + (lane & 31)];
-                }
-                if (!have || f >= a.D) continue;
-                if (a.splits > 1) {
-                    *reinterpret_cast<vo_f32x4*>(part_row(a, split, p.q0 + token, head) + f) = vo_f32x4{v[0], v[1], v[2], v[3]};
-                } else if constexpr (sizeof(T) == 2) {
-                    *reinterpret_cast<vo_u32x2*>(out_row<T>(a, p.q0 + token, head) + f) =
-                        vo_u32x2{vo_elem<T>::pack2(v[0] * inv, v[1] * inv), vo_elem<T>::pack2(v[2] * inv, v[3] * inv)};
-                } else {
-                    *reinterpret_cast<vo_f32x4*>(out_row<T>(a, p.q0 + token, head) + f) = vo_f32x4{v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv};
-                }
-            }
-        }
-    } else {
-        auto place = [&](int r) { return p.row + r < rows ? p.row + r : -1; };
+        if (!have || f >= a.D) continue;
         if (a.splits > 1) {
-            store_rows<float, DT>(core.o, 1.f, a.D, lds, lane, [&](int r) -> float* {
-                const int64_t x = place(r);
-                return x < 0 ? nullptr : part_row(a, split, p.q0 + x / a.group, kh * a.group + (int)(x % a.group));
-            });
+            *reinterpret_cast<vo_f32x4*>(part_row(a, split, p.q0 + token, head) + f) = vo_f32x4{v[0], v[1], v[2], v[3]};
+        } else if constexpr (sizeof(T) == 2) {
+            *reinterpret_cast<vo_u32x2*>(out_row<T>(a, p.q0 + token, head) + f) =
+                vo_u32x2{vo_elem<T>::pack2(v[0] * inv, v[1] * inv), vo_elem<T>::pack2(v[2] * inv, v[3] * inv)};
         } else {
-            store_rows<T, DT>(core.o, inverse(l), a.D, lds, lane, [&](int r) -> T* {
-                const int64_t x = place(r);
-                return x < 0 ? nullptr : out_row<T>(a, p.q0 + x / a.group, kh * a.group + (int)(x % a.group));
-            });
+            *reinterpret_cast<vo_f32x4*>(out_row<T>(a, p.q0 + token, head) + f) = vo_f32x4{v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv};
         }
     }
     if (a.splits > 1 && wave == 0 && lane < 32 && have)
@@ -658,7 +657,7 @@ template <typename T, int DT> int launch(const AttArgs& a, const Plan& p, hipStr
     constexpr int BYTES = DT * (int)sizeof(T);                       // of a row
     const dim3 grid((unsigned)p.blocks);
     if (p.rows) {
-        constexpr int KEYS = BYTES <= 128 ? 64 : 32, WAVES = BYTES <= 256 ? 4 : BYTES <= 512 ? 2 : 1;
+        constexpr int KEYS = BYTES <= 128 ? 64 : 32, WAVES = BYTES <= 256 ? 8 : BYTES <= 512 ? 4 : 2;
         attention_rows<T, DT, KEYS, WAVES><<<grid, 64 * WAVES, 0, st>>>(a);
     } else {
         constexpr int KEYS = BYTES <= 512 ? 64 : 32;
