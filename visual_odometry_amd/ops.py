@@ -1103,9 +1103,9 @@ def _token_tensor(t, name: str, like: torch.Tensor | None = None) -> torch.Tenso
     if like is None:
         if t.dtype not in _TOKEN_DTYPES:
             raise ValueError(f"{name}: expected float32, float16 or bfloat16, got {t.dtype}")
-    elif t.dtype != like.dtype:
+    elif t.dtype is not like.dtype:
         raise ValueError(f"{name}: dtype {t.dtype} differs from {like.dtype}")
-    elif t.device != like.device:
+    elif t.get_device() != like.get_device():
         raise ValueError(f"{name}: on {t.device}, the other tensors on {like.device}")
     return t
 
@@ -1153,15 +1153,15 @@ def _workspace_bytes(query: str, *sizes) -> int:
     return int(getattr(_lib.load(), query)(*sizes))
 
 
-def _call_on(device: torch.device, name: str, args, need: int, nbytes: int, flops: int = 0) -> None:
-    """_call on ``device`` (which need not be the current one) and its current stream, with ``need`` bytes of workspace
-    from the caching allocator; the entry point's last three arguments are workspace, its size and the stream."""
-    index = device.index
-    if index != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            return _call_on(device, name, args, need, nbytes, flops)
-    work = torch.empty((need,), device=device, dtype=torch.uint8) if need else None
-    _call(name, *args, 0 if work is None else work.data_ptr(), need, torch._C._cuda_getCurrentRawStream(index), nbytes=nbytes, flops=flops)
+def _call_on(like: torch.Tensor, name: str, args, need: int, nbytes: int, flops: int = 0) -> None:
+    """_call on the device of ``like`` (which need not be the current one) and its current stream, with ``need`` bytes of
+    workspace from the caching allocator; the entry point's last three arguments are workspace, its size and the stream."""
+    index = like.get_device()
+    if index != torch._C._cuda_getDevice():
+        with torch.cuda.device(index):
+            return _call_on(like, name, args, need, nbytes, flops)
+    work = like.new_empty(need, dtype=torch.uint8) if need else None
+    _call(name, *args, work.data_ptr() if need else 0, need, torch._C._cuda_getCurrentRawStream(index), nbytes=nbytes, flops=flops)
 
 
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, activation: str | None = None,
@@ -1181,7 +1181,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     K, C = weight.shape
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation must be one of {list(ACTIVATIONS)}, got {activation!r}")
-    if bias is not None and (bias.numel() != K or bias.device != x.device):
+    if bias is not None and (bias.numel() != K or bias.get_device() != x.get_device()):
         raise ValueError("bias must have one entry per output, on x's device")
     px, M, xs = _rows(x, "x", C)
     shape = x.shape[:-1] + (K,)
@@ -1191,7 +1191,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
             raise ValueError(f"residual must be {tuple(shape)}, got {tuple(residual.shape)}")
         pr, _, rs = _rows(residual, "residual", K)
     if out is None:
-        out = torch.empty(shape, device=x.device, dtype=x.dtype)
+        out = x.new_empty(shape)
         py, ys = out.data_ptr(), K
     else:
         if _token_tensor(out, "out", x).shape != shape:
@@ -1202,7 +1202,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
         if residual is not None and (py, ys) != (pr, rs):
             _no_overlap(out, residual, "residual (other than as the same tensor)")
     dt, es = _TOKEN_DTYPES[x.dtype], x.element_size()
-    _call_on(x.device, "vo_linear",
+    _call_on(x, "vo_linear",
              (px, xs, weight.data_ptr(), _opt(bias, "bias", torch.float32), pr, rs, py, ys, M, C, K, ACTIVATIONS[activation], dt),
              _workspace_bytes("vo_linear_workspace_bytes", M, C, K, dt),
              es * (M * C + K * C + M * K * (1 + (residual is not None))), 2 * M * C * K)
@@ -1258,11 +1258,11 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: torc
             raise ValueError("k_offsets needs q_offsets")
         pqo, pko = _dev(q_offsets, "q_offsets", torch.int32), _dev(k_offsets, "k_offsets", torch.int32)
         sequences = q_offsets.numel() - 1
-        if (sequences < 1 or q_offsets.dim() != 1 or k_offsets.shape != q_offsets.shape or q_offsets.device != q.device
-                or k_offsets.device != q.device):
+        if (sequences < 1 or q_offsets.dim() != 1 or k_offsets.shape != q_offsets.shape or q_offsets.get_device() != q.get_device()
+                or k_offsets.get_device() != q.get_device()):
             raise ValueError("q_offsets and k_offsets must both be (sequences + 1), as many as each other, on q's device")
     if out is None:
-        out = torch.empty((Tq, Hq, D), device=q.device, dtype=q.dtype)
+        out = q.new_empty(q.shape)
         os_, oh = Hq * D, D
     elif _token_tensor(out, "out", q).shape != q.shape:
         raise ValueError(f"out must be {(Tq, Hq, D)}, got {tuple(out.shape)}")
@@ -1272,7 +1272,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: torc
             raise ValueError(f"out: elements overlap or interleave (got strides {out.stride()})")
         for t, n in ((q, "q"), (k, "k"), (v, "v")):
             _no_overlap(out, t, n)
-    _call_on(q.device, "vo_attention",
+    _call_on(q, "vo_attention",
              (q.data_ptr(), qs, qh, k.data_ptr(), ks, kh, v.data_ptr(), vs, vh, out.data_ptr(), os_, oh, pqo, pko, sequences, Tq, Tk, Hq, Hk,
               D, D ** -0.5 if scale is None else float(scale), 1 if causal else 0, _TOKEN_DTYPES[q.dtype]),
              _workspace_bytes("vo_attention_workspace_bytes", Tq, Tk, sequences, Hq, Hk, D, _TOKEN_DTYPES[q.dtype]),
