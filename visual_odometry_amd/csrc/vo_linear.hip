@@ -123,7 +123,7 @@ __global__ __launch_bounds__(64 * WGM * WGN) void linear_tiles(const LinArgs a) 
     constexpr int STRIP = TN + 4;                                    // floats per row of the store's staging strip
     constexpr int SLAB = ROWS * 128, STAGE = NW * 16 * STRIP * 4;
     static_assert(ROWS % (8 * NW) == 0 && BM % (8 * NW) == 0, "a wave's loads must not straddle the operands");
-    static_assert(DIRECT || STAGES == 2, "registers hold one more slab");
+    static_assert(DIRECT || STAGES == 2, "registers hold two more slabs");
     __shared__ __align__(16) unsigned char lds[STAGES * SLAB > STAGE ? STAGES * SLAB : STAGE];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -166,7 +166,7 @@ __global__ __launch_bounds__(64 * WGM * WGN) void linear_tiles(const LinArgs a) 
             first[o][q] = (unsigned)((tile_row(i) - q * 8 + sub) * (o == 0 ? xb : wb)) + chunk(i) * 16;
             ahead_of[o][q] = chunk(i) * PER;
         }
-    struct Regs { vo_u32x4 r[DIRECT ? 1 : LOADS]; } regs;             // unaligned rows pass through registers
+    struct Regs { vo_u32x4 r[DIRECT ? 1 : LOADS]; };                 // unaligned rows pass through registers
     auto fetch = [&](int s, unsigned char* buf, Regs& regs) {
         const int c0 = c_first + s * BK;
         if constexpr (DIRECT) {
@@ -247,21 +247,8 @@ __global__ __launch_bounds__(64 * WGM * WGN) void linear_tiles(const LinArgs a) 
     // any traffic), so that the number of loads under way is always the same.
     unsigned char* buf = lds;                                        // of slab s
     auto after = [&](unsigned char* p) { return p + SLAB == lds + STAGES * SLAB ? lds : p + SLAB; };
-    if constexpr (DIRECT) {
-#pragma unroll
-        for (int i = 0; i < STAGES; ++i) fetch(i, lds + i * SLAB, regs);
-        vo_lds_barrier<(STAGES - 1) * LOADS>();
-    } else {
-        Regs second;
-        fetch(0, nullptr, regs);
-        if (slabs > 1) fetch(1, nullptr, second);
-        put(0, lds, regs);
-        if (slabs > 2) fetch(2, nullptr, regs);
-        if (slabs > 1) put(1, lds + SLAB, second);
-        __syncthreads();
-    }
-    read(f0, buf, 0);
-    for (int s = 0; s + 1 < slabs; ++s) {
+    Regs even, odd;                                                  // slabs on their way through registers
+    auto step = [&](int s, Regs& regs) {                             // regs: slab s + 2
         read(f1, buf, 1);
         multiply(f0);
         interleave();
@@ -271,12 +258,34 @@ __global__ __launch_bounds__(64 * WGM * WGN) void linear_tiles(const LinArgs a) 
         } else {
             __syncthreads();
             if (s + 2 < slabs) put(s + 2, buf, regs);
-            if (s + 3 < slabs) fetch(s + 3, nullptr, regs);
+            if (s + 4 < slabs) fetch(s + 4, nullptr, regs);
         }
         buf = after(buf);
         read(f0, buf, 0);
         multiply(f1);
         interleave();
+    };
+    if constexpr (DIRECT) {
+#pragma unroll
+        for (int i = 0; i < STAGES; ++i) fetch(i, lds + i * SLAB, even);
+        vo_lds_barrier<(STAGES - 1) * LOADS>();
+        read(f0, buf, 0);
+        for (int s = 0; s + 1 < slabs; ++s) step(s, even);
+    } else {
+        fetch(0, nullptr, even);
+        if (slabs > 1) fetch(1, nullptr, odd);
+        put(0, lds, even);
+        if (slabs > 2) fetch(2, nullptr, even);
+        if (slabs > 1) put(1, lds + SLAB, odd);
+        if (slabs > 3) fetch(3, nullptr, odd);
+        __syncthreads();
+        read(f0, buf, 0);
+        int s = 0;
+        for (; s + 2 < slabs; s += 2) {
+            step(s, even);
+            step(s + 1, odd);
+        }
+        if (s + 1 < slabs) step(s, even);
     }
     read(f1, buf, 1);
     multiply(f0);
