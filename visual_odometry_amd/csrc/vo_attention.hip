@@ -562,33 +562,36 @@ template <typename T, int WIDTH> __global__ __launch_bounds__(256) void attentio
     const int64_t token = row / a.Hq;
     if (token >= a.Tq) return;
     if (a.q_off && (token < a.q_off[0] || token >= a.q_off[a.sequences])) return;
-    const int head = (int)(row % a.Hq);
+    const int head = (int)(row % a.Hq), f = lane % WIDTH * 4;
+    // a round's sums are requested before the weights are known: a part is written for every row of a sequence
+    vo_f32x4 x[4];
+    auto fetch = [&](int s0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int s = s0 + i * GROUPS + lane / WIDTH;
+            x[i] = vo_f32x4{0.f, 0.f, 0.f, 0.f};
+            if (s < a.splits && f < a.D) x[i] = *reinterpret_cast<const vo_f32x4*>(part_row(a, s, token, head) + f);
+        }
+    };
     float2 ml = make_float2(-INFINITY, 0.f);
     if (lane < a.splits) ml = *reinterpret_cast<const float2*>(part_ml(a, lane, token, head));
+    fetch(0);
     float m = ml.x;
 #pragma unroll
     for (int d = 32; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
     const float w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - m);
-    const uint64_t sees = __ballot(ml.y != 0.f);                     // the other parts saw no key of this row; a NaN counts
-    float l = w * ml.y;
+    float l = w * ml.y;                                              // a part that saw no key of this row has neither weight nor sums
 #pragma unroll
     for (int d = 32; d; d >>= 1) l += __shfl_xor(l, d);
-    const int f = lane % WIDTH * 4;
     float o[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int s0 = 0; s0 < a.splits; s0 += 4 * GROUPS) {              // four loads under way
-        float ws[4];
-        vo_f32x4 x[4];
+    for (int s0 = 0; s0 < a.splits; s0 += 4 * GROUPS) {
+        if (s0) fetch(s0);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int s = s0 + i * GROUPS + lane / WIDTH;
-            ws[i] = __shfl(w, s & 63);
-            x[i] = vo_f32x4{0.f, 0.f, 0.f, 0.f};
-            if (s < a.splits && f < a.D && (sees >> s & 1)) x[i] = *reinterpret_cast<const vo_f32x4*>(part_row(a, s, token, head) + f);
+            const float ws = __shfl(w, s0 + i * GROUPS + lane / WIDTH & 63);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[j] += ws * x[i][j];
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) o[j] += ws[i] * x[i][j];
     }
 #pragma unroll
     for (int d = 32; d >= WIDTH; d >>= 1)
