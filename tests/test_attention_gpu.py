@@ -113,6 +113,7 @@ def test_groups_of_heads(vo, dtype, Hq, Hk, q_len, k_len):
 @pytest.mark.parametrize("causal", [False, True])
 @pytest.mark.parametrize("q_len,k_len,Hq,Hk,D", [
     ([1], [5003], 4, 1, 128), ([1, 2, 1], [4000, 1, 9001], 8, 2, 64), ([3], [2500], 2, 1, 256),       # rows, split over the keys
+    ([1], [5003], 4, 1, 96), ([100], [6007], 2, 1, 72),
     ([100], [6007], 2, 1, 64), ([40, 70], [3000, 2500], 2, 2, 128), ([129], [1500], 1, 1, 256)])      # tiles, split over the keys
 def test_long_axes_are_split_and_joined(vo, dtype, causal, q_len, k_len, Hq, Hk, D):
     from visual_odometry_amd import _lib
@@ -190,7 +191,7 @@ def test_sequences_do_not_disturb_each_other(vo, dtype, q_len, k_len):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("D", [32, 64, 128, 256])
+@pytest.mark.parametrize("D", [32, 64, 96, 128, 256])
 @pytest.mark.parametrize("q_len,k_len", [([200], [200]), ([130], [300]), ([100], [60]), ([5], [90]), ([3], [2000]), ([140], [2000])])
 def test_unbounded_keys_and_values_reach_only_the_rows_that_see_them(vo, dtype, D, q_len, k_len):
     """Causal, with an infinity in one value, a NaN in another key and value near the diagonal: rows ahead of them are exact,

@@ -48,17 +48,27 @@ struct AttArgs {
     float c;                                      // scale * log2(e)
 };
 
-// Key tiles in LDS: rows of DT elements in 16-byte chunks, chunk c of row r at c ^ swizzle(r).  K is read 16 rows of one
-// chunk at a time, V (16 bits) four rows of 64 bytes, V (float32) two rows of 128 bytes four rows apart: each permutation
-// spreads its reader's bytes over all 64 banks.
+// Key tiles in LDS: rows of DT elements in 16-byte chunks, permuted within each row.  K is read 16 rows of one chunk at a time,
+// V (16 bits) four rows of 64 bytes, V (float32) two rows of 128 bytes four rows apart: each permutation spreads its reader's
+// bytes over all 64 banks.  It is an exclusive or where the number of chunks is a power of two, else (DT = 96: two rows
+// in four, or one in two, start at another bank already) a rotation.
 template <typename T, int DT> struct Tile {
     static constexpr int ES = sizeof(T), PER = vo_elem<T>::PER, CH = DT / PER, ROW = DT * ES;
+    static constexpr bool POW2 = (CH & (CH - 1)) == 0;
     static constexpr int PER_LINE = ROW >= 256 ? 1 : 256 / ROW;      // rows in 256 bytes
     static constexpr int KMASK = CH < 16 ? CH - 1 : 15;
-    static __device__ __forceinline__ int k_swz(int r) { return (r / PER_LINE) & KMASK; }
+    static __device__ __forceinline__ int k_swz(int r) { return POW2 ? (r / PER_LINE) & KMASK : (r & 31) >> (ES == 4 ? 1 : 2); }
     static __device__ __forceinline__ int v_swz(int r) {
         if constexpr (ES == 4) return CH > 8 ? ((r >> 2) & 1) << 3 : 0;
-        return CH <= 4 ? 0 : CH == 8 ? ((r >> 1) & 1) << 2 : (r & 3) << 2;
+        return !POW2 || CH <= 4 ? 0 : CH == 8 ? ((r >> 1) & 1) << 2 : (r & 3) << 2;
+    }
+    static __device__ __forceinline__ int place(int chunk, int swz) {        // where a chunk lies
+        if constexpr (POW2) return chunk ^ swz;
+        return chunk + swz < CH ? chunk + swz : chunk + swz - CH;
+    }
+    static __device__ __forceinline__ int chunk_at(int place, int swz) {     // which chunk lies there
+        if constexpr (POW2) return place ^ swz;
+        return place < swz ? place + CH - swz : place - swz;
     }
 };
 
@@ -99,7 +109,7 @@ template <typename T, int DT, int KEYS> struct Core {
 #pragma unroll
             for (int b = 0; b < KB; ++b) {
                 const int r = b * 32 + (lane & 31);
-                k[b] = *reinterpret_cast<const vo_u32x4*>(kt + r * L::ROW + (((i * 2 + (lane >> 5)) ^ L::k_swz(r)) * 16));
+                k[b] = *reinterpret_cast<const vo_u32x4*>(kt + r * L::ROW + L::place(i * 2 + (lane >> 5), L::k_swz(r)) * 16);
             }
 #pragma unroll
             for (int part = 0; part < E::PARTS; ++part)
@@ -169,8 +179,8 @@ template <typename T, int DT, int KEYS> struct Core {
     static __device__ __forceinline__ vo_u32x4 value_piece(const unsigned char* vt, int j, int lane) {
         const int r = 16 * (j / DB) + 4 * (lane >> 5) + ((lane & 15) >> 2), at = (lane & 1) * 8;
         const int chunk = j % DB * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
-        const vo_u32x2 lo = transposed(vt + r * L::ROW + ((chunk ^ L::v_swz(r)) * 16) + at);
-        const vo_u32x2 hi = transposed(vt + (r + 8) * L::ROW + ((chunk ^ L::v_swz(r + 8)) * 16) + at);
+        const vo_u32x2 lo = transposed(vt + r * L::ROW + L::place(chunk, L::v_swz(r)) * 16 + at);
+        const vo_u32x2 hi = transposed(vt + (r + 8) * L::ROW + L::place(chunk, L::v_swz(r + 8)) * 16 + at);
         return vo_u32x4{lo[0], lo[1], hi[0], hi[1]};
     }
     __device__ __forceinline__ void add_values(vo_u32x4 v, const unsigned (*p)[PW], int j) {
@@ -193,7 +203,7 @@ template <typename T, int DT, int KEYS> struct Core {
 #pragma unroll
                 for (int d = 0; d < DB; ++d) {
                     const int chunk = d * 8 + (col >> 2);
-                    const float vf = *reinterpret_cast<const float*>(vt + r * L::ROW + ((chunk ^ L::v_swz(r)) * 16) + (col & 3) * 4);
+                    const float vf = *reinterpret_cast<const float*>(vt + r * L::ROW + L::place(chunk, L::v_swz(r)) * 16 + (col & 3) * 4);
                     o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf, __builtin_bit_cast(float, p[b][i]), o[d], 0, 0, 0);
                 }
             }
@@ -286,7 +296,7 @@ template <typename T, int DT, int KEYS, int WAVES> struct Loader {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int piece = (wave * N + i) * 64 + lane, r = piece / L::CH;
-            const int chunk = (piece % L::CH) ^ (is_v ? L::v_swz(r) : L::k_swz(r));
+            const int chunk = L::chunk_at(piece % L::CH, is_v ? L::v_swz(r) : L::k_swz(r));
             off[i] = chunk * L::PER < D ? (unsigned)(r * stride * L::ES) + chunk * 16 : VO_OUTSIDE;
         }
     }
@@ -315,14 +325,16 @@ template <typename T> __device__ __forceinline__ T* out_row(const AttArgs& a, in
 // row(r): where row r goes, null if it does not exist.
 template <typename S, int DT, typename F>
 __device__ __forceinline__ void store_rows(const vo_f32x16* o, float factor, int D, unsigned char* lds, int lane, F row) {
-    constexpr int ES = sizeof(S), CH = DT * ES / 16, MASK = CH < 16 ? CH - 1 : 15, EACH = 16 / ES;
+    using L = Tile<S, DT>;
+    constexpr int ES = sizeof(S), CH = L::CH, EACH = L::PER;
+    auto swz = [](int r) { return L::POW2 ? r & L::KMASK : L::k_swz(r); };
     const int r = lane & 31;
 #pragma unroll
     for (int d = 0; d < DT / 32; ++d)
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
             const int f = d * 32 + 8 * b + 4 * (lane >> 5);
-            unsigned char* p = lds + r * DT * ES + (((f / EACH) ^ (r & MASK)) * 16) + f % EACH * ES;
+            unsigned char* p = lds + r * DT * ES + L::place(f / EACH, swz(r)) * 16 + f % EACH * ES;
             const float v0 = o[d][4 * b] * factor, v1 = o[d][4 * b + 1] * factor, v2 = o[d][4 * b + 2] * factor, v3 = o[d][4 * b + 3] * factor;
             if constexpr (ES == 2) *reinterpret_cast<vo_u32x2*>(p) = vo_u32x2{vo_elem<S>::pack2(v0, v1), vo_elem<S>::pack2(v2, v3)};
             else *reinterpret_cast<vo_f32x4*>(p) = vo_f32x4{v0, v1, v2, v3};
@@ -330,7 +342,7 @@ __device__ __forceinline__ void store_rows(const vo_f32x16* o, float factor, int
     vo_wave_lds_fence();
 #pragma unroll
     for (int i = 0; i < CH / 2; ++i) {
-        const int piece = i * 64 + lane, q = piece / CH, c = (piece % CH) ^ (q & MASK);
+        const int piece = i * 64 + lane, q = piece / CH, c = L::chunk_at(piece % CH, swz(q));
         S* p = row(q);
         if (p && c * EACH < D) *reinterpret_cast<vo_u32x4*>(p + c * EACH) = *reinterpret_cast<const vo_u32x4*>(lds + piece * 16);
     }
@@ -613,7 +625,7 @@ struct Plan {
 };
 
 // Bytes of a row decide the key tiles and how many workgroups a CU holds.
-constexpr int row_bytes(int D, int es) { return (D <= 32 ? 32 : D <= 64 ? 64 : D <= 128 ? 128 : 256) * es; }
+constexpr int row_bytes(int D, int es) { return (D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : D <= 128 ? 128 : 256) * es; }
 
 Plan plan(int64_t Tq, int64_t Tk, int sequences, int Hq, int Hk, int D, int dtype) {
     const int group = Hq / Hk;
@@ -634,7 +646,7 @@ Plan plan(int64_t Tq, int64_t Tk, int sequences, int Hq, int Hk, int D, int dtyp
         // 4800 float32 rows, 4 heads of 64: 352 us unsplit, 228 in 3 parts, 260 in 4, 236 in 8; 96 rows before 30001 keys, 32
         // heads: 518 unsplit, 93 in 8, 86 in 16.)
         const int bytes = row_bytes(D, dtype == VO_F32 ? 4 : 2), tile = bytes <= 512 ? 64 : 32;
-        const int64_t resident = 256 * (bytes <= 128 ? 4 : bytes <= 256 ? 2 : 1);
+        const int64_t resident = 256 * (bytes <= 128 ? 4 : bytes <= 192 ? 3 : bytes <= 256 ? 2 : 1);
         const double tiles = (double)vo_ceil_div(keys, tile), tile_us = D / 128.0 * (dtype == VO_F32 ? 10.0 : 2.1);
         const double join_us = (double)Tq * Hq * D * 8 / 4e6;        // per part: written and read once
         double best = 0.;
@@ -668,7 +680,7 @@ template <typename T, int DT> int launch(const AttArgs& a, const Plan& p, hipStr
     }
     VO_CHECK_LAUNCH("vo_attention");
     if (p.splits > 1) {
-        attention_join<T, DT / 4><<<dim3((unsigned)vo_ceil_div(a.Tq * a.Hq, 4)), 256, 0, st>>>(a);
+        attention_join<T, DT == 96 ? 32 : DT / 4><<<dim3((unsigned)vo_ceil_div(a.Tq * a.Hq, 4)), 256, 0, st>>>(a);
         VO_CHECK_LAUNCH("vo_attention (join)");
     }
     return VO_OK;
@@ -677,6 +689,7 @@ template <typename T, int DT> int launch(const AttArgs& a, const Plan& p, hipStr
 template <typename T> int dispatch(const AttArgs& a, const Plan& p, hipStream_t st) {
     if (a.D <= 32) return launch<T, 32>(a, p, st);
     if (a.D <= 64) return launch<T, 64>(a, p, st);
+    if (a.D <= 96) return launch<T, 96>(a, p, st);
     if (a.D <= 128) return launch<T, 128>(a, p, st);
     return launch<T, 256>(a, p, st);
 }
