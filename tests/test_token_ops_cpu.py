@@ -63,6 +63,25 @@ def test_wrong_offsets_never_lead_outside_the_tensors():
             assert not any_ or 0 <= row < Lq
 
 
+@pytest.mark.parametrize("sequences", [62, 63, 64, 65, 66, 127, 500, 5000])
+@pytest.mark.parametrize("shape", ["equal", "rising", "one_long", "empty_but_for_some"])
+def test_tiles_of_many_sequences(sequences, shape):
+    """Lengths for which a sequence lies where equal ones would put it, and lengths for which it does not."""
+    q_len = {"equal": np.full(sequences, 40), "rising": np.arange(sequences) % 700 // 3, "one_long": np.full(sequences, 1),
+             "empty_but_for_some": np.arange(sequences) % 50 // 49 * 130}[shape].copy()
+    if shape == "one_long":
+        q_len[sequences // 3] = 20000
+    k_len = np.arange(sequences) % 7                                  # tells neighbours apart
+    q, k, tiles = _tiles(q_len, k_len, 1, 32, lead=5)
+    hits = [0] * sequences
+    for any_, row, q0, Lq, k0, Lk in tiles:
+        if any_:
+            s = int(np.flatnonzero((q[:-1] == q0) & (q_len == Lq) & (k[:-1] == k0) & (k_len == Lk))[0])
+            assert row == 32 * hits[s]
+            hits[s] += 1
+    assert hits == [-(-int(l) // 32) for l in q_len]
+
+
 def test_linear_entry_point_refuses():
     from visual_odometry_amd import _lib
     lib = _lib.load()
