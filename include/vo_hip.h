@@ -651,7 +651,8 @@ int vo_linear(const void* x, int64_t x_row_stride, const void* weight, const flo
  *   q_offsets[s+1]) and the keys [k_offsets[s], k_offsets[s+1]), any length from 0; or both NULL with sequences = 1: all
  *   rows and keys.  Rows outside every sequence are left as they were.  The offsets are read on the device and clamped to
  *   the tensors; results for offsets that do not ascend are unspecified.
- *   A key or value reaches the rows that see it and no others, whatever it holds: infinities and NaN too.
+ *   A key or value reaches the rows that see it and no others, whatever it holds: infinities and NaN too.  A key whose score is
+ *   -infinity has no weight; a row with no other key gives zeros, like one that sees none.
  * workspace: vo_attention_workspace_bytes(...) bytes (often 0), 16-byte aligned, contents irrelevant.  Calls that share one
  * must be ordered on one stream; two captured graphs that may replay at once need one each.
  * ------------------------------------------------------------------------- */

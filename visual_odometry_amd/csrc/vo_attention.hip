@@ -17,13 +17,14 @@
 //
 // Two forms:
 //   tiles  a workgroup of four waves takes 128 rows of one key head (a row is a token and one of the heads that share the key
-//          head); key tiles are shared in LDS, loaded while the previous tile is multiplied.  Matrix and vector work of a tile take about as long as each other and overlap between the two
-//          to four workgroups of a CU; the chip's power sets the clock (the same cycles are 38 % faster on zeros).  8 prompts of
-//          up to 8192 tokens, 32 / 8 heads of 128, bfloat16, causal: 2.04 ms = 1.02 PFLOP/s; 4800 float32 rows, 4 heads of 64:
-//          229 us = 103 TFLOP/s of the 151 the library's product reaches.
-//   rows   few rows per sequence (single tokens above all): the rows of all heads that share a key head are one tile of 32,
-//          every wave streams key tiles of its own into its own part of LDS, the waves' results are joined at the end.  Bound by
-//          the read of keys and values: 32 caches of up to 32768 tokens, 8 key heads of 128: 362 us = 5.4 TB/s.
+//          head); key tiles are shared in LDS, loaded while the previous tile is multiplied.  Matrix and vector work of a tile
+//          take about as long as each other and overlap between the two to four workgroups of a CU; the chip's power sets the
+//          clock (the same cycles are 38 % faster on zeros).  8 prompts of up to 8192 tokens, 32 / 8 heads of 128, bfloat16,
+//          causal: 2.04 ms = 1.02 PFLOP/s; 4800 float32 rows, 4 heads of 64: 226 us = 104 TFLOP/s of the 151 the library's
+//          product reaches.
+//   rows   few rows per sequence (single tokens above all): tiles of 32 rows, every wave streams key tiles of its own into its
+//          own part of LDS, the waves' results are joined at the end.  Bound by the read of keys and values: 32 caches of up to
+//          32768 tokens, 8 key heads of 128: 364 us = 5.4 TB/s; a single row before 777 keys 12 us, all of it waiting.
 // Either can be split over the keys; the parts (m, l, unnormalised sums) go to a workspace and are joined in a fixed order.
 #include "vo_packed.h"
 #include "vo_tokens.h"
@@ -624,7 +625,8 @@ struct Plan {
     int64_t tiles, blocks;
 };
 
-// Bytes of a row decide the key tiles and how many workgroups a CU holds.
+// Bytes of a row decide the key tiles and how many workgroups a CU holds.  (96: 16 heads of 72 or 96 over 4, 4 sequences of 3000,
+// take 143 and 146 us, padded to 128 190 and 192.)
 constexpr int row_bytes(int D, int es) { return (D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : D <= 128 ? 128 : 256) * es; }
 
 Plan plan(int64_t Tq, int64_t Tk, int sequences, int Hq, int Hk, int D, int dtype) {
@@ -643,8 +645,8 @@ Plan plan(int64_t Tq, int64_t Tk, int sequences, int Hq, int Hk, int D, int dtyp
         if (splits > keys / 512) splits = keys / 512;
     } else {
         // Rounds over the resident workgroups times a part's key tiles and its start, plus the join's traffic.  (One sequence of
-        // 4800 float32 rows, 4 heads of 64: 352 us unsplit, 228 in 3 parts, 260 in 4, 236 in 8; 96 rows before 30001 keys, 32
-        // heads: 518 unsplit, 93 in 8, 86 in 16.)
+        // 4800 float32 rows, 4 heads of 64: 352 us unsplit, 226 in 3 parts, 260 in 4, 236 in 8; 96 rows before 30001 keys, 32
+        // heads over 4: 518 unsplit, 100 in 10, 78 in 18, 85 in 32.)
         const int bytes = row_bytes(D, dtype == VO_F32 ? 4 : 2), tile = bytes <= 512 ? 64 : 32;
         const int64_t resident = 256 * (bytes <= 128 ? 4 : bytes <= 192 ? 3 : bytes <= 256 ? 2 : 1);
         const double tiles = (double)vo_ceil_div(keys, tile), tile_us = D / 128.0 * (dtype == VO_F32 ? 10.0 : 2.1);
