@@ -639,10 +639,16 @@ Plan plan(int64_t Tq, int64_t Tk, int sequences, int Hq, int Hk, int D, int dtyp
     const int64_t base = p.tiles * Hk;
     int64_t splits = 1;
     if (p.rows) {
-        // About eight rounds over the CUs even out sequences of different lengths (32 sequences of up to 32768 keys, 8 key heads:
-        // 495 us unsplit, 396 in 4 parts, 377 in 8, 400 in 16); a part has at least 512 keys.
-        splits = vo_ceil_div(2048, base);
-        if (splits > keys / 512) splits = keys / 512;
+        // Few workgroups: parts until every CU has one (and none two: that round would be as long again), of at least 256 keys, where the join's launch is worth it (one row before
+        // 777 keys, 8 key heads: 12.2 us unsplit, 12.0 in 4 parts; 1500 keys: 16.1 / 12.7; 4096: 33.0 / 18.0, 14.3 in 16).
+        if (keys >= 1024) {
+            splits = 256 / base;
+            if (splits > keys / 256) splits = keys / 256;
+        }
+        // Many: about eight rounds over the CUs even out sequences of different lengths, but parts under 2048 keys cost more than that
+        // gains (32 sequences of up to 32768 keys: 501 us unsplit, 400 in 4 parts, 383 in 8, 409 in 16; 64 of 2000: 111, 135 in 4).
+        const int64_t even = vo_ceil_div(2048, base) < keys / 2048 ? vo_ceil_div(2048, base) : keys / 2048;
+        if (splits < even) splits = even;
     } else {
         // Rounds over the resident workgroups times a part's key tiles and its start, plus the join's traffic.  (One sequence of
         // 4800 float32 rows, 4 heads of 64: 352 us unsplit, 226 in 3 parts, 260 in 4, 236 in 8; 96 rows before 30001 keys, 32
