@@ -655,12 +655,15 @@ Plan plan(int64_t Tq, int64_t Tk, int sequences, int Hq, int Hk, int D, int dtyp
         // heads over 4: 518 unsplit, 100 in 10, 78 in 18, 85 in 32.)
         const int bytes = row_bytes(D, dtype == VO_F32 ? 4 : 2), tile = bytes <= 512 ? 64 : 32;
         const int64_t resident = 256 * (bytes <= 128 ? 4 : bytes <= 192 ? 3 : bytes <= 256 ? 2 : 1);
-        const double tiles = (double)vo_ceil_div(keys, tile), tile_us = D / 128.0 * (dtype == VO_F32 ? 10.0 : 2.1);
+        // The lengths are on the device: where all workgroups run at once, the longest sequence, taken to be half as long again as the average, is what
+        // they wait for (8 sequences of 71 to 1500 keys: 26 us unsplit, 16 in 4 parts; 2 equal ones of 20000 keys lose 5 %).
+        const int64_t longest = keys + keys / 2 < Tk ? keys + keys / 2 : Tk;
+        const double tiles = (double)vo_ceil_div(keys, tile), most = (double)vo_ceil_div(longest, tile), tile_us = D / 128.0 * (dtype == VO_F32 ? 10.0 : 2.1);
         const double join_us = (double)Tq * Hq * D * 8 / 4e6;        // per part: written and read once
         double best = 0.;
-        for (int s = 1; s <= 64 && s <= (keys + 255) / 256; ++s) {
+        for (int s = 1; s <= 64 && s <= (longest + 255) / 256; ++s) {
             const double blocks = (double)base * s, rounds = blocks <= resident ? 0.6 + 0.4 * blocks / resident : (double)((int64_t)((blocks + resident - 1) / resident));
-            const double us = rounds * (tiles / s + 2.) * tile_us + (s > 1 ? 4. + s * join_us : 0.);
+            const double us = rounds * ((blocks <= resident ? most : tiles) / s + 2.) * tile_us + (s > 1 ? 4. + s * join_us : 0.);
             if (s == 1 || us < best) {
                 best = us;
                 splits = s;
