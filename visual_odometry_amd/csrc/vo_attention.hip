@@ -20,7 +20,7 @@
 //          head); key tiles are shared in LDS, loaded while the previous tile is multiplied.  Matrix and vector work of a tile
 //          take about as long as each other and overlap between the two to four workgroups of a CU; the chip's power sets the
 //          clock (the same cycles are 38 % faster on zeros).  8 prompts of up to 8192 tokens, 32 / 8 heads of 128, bfloat16,
-//          causal: 2.04 ms = 1.02 PFLOP/s; 4800 float32 rows, 4 heads of 64: 226 us = 104 TFLOP/s of the 151 the library's
+//          causal: 2.04 ms = 1.02 PFLOP/s; 4800 float32 rows, 4 heads of 64: 207 us = 114 TFLOP/s of the 151 the library's
 //          product reaches.
 //   rows   few rows per sequence (single tokens above all): tiles of 32 rows, every wave streams key tiles of its own into its
 //          own part of LDS, the waves' results are joined at the end.  Bound by the read of keys and values: 32 caches of up to
@@ -625,9 +625,13 @@ struct Plan {
     int64_t tiles, blocks;
 };
 
-// Bytes of a row decide the key tiles and how many workgroups a CU holds.  (96: 16 heads of 72 or 96 over 4, 4 sequences of 3000,
-// take 143 and 146 us, padded to 128 190 and 192.)
-constexpr int row_bytes(int D, int es) { return (D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : D <= 128 ? 128 : 256) * es; }
+// The features that a head is padded to, keys in a tile and workgroups a CU holds (LDS and registers) in the form by tiles.
+// 96 features: 16 heads of 72 or 96 over 4, 4 sequences of 3000, take 143 and 146 us, padded to 128 190 and 192.  32 keys in
+// float32, whose values take twice the registers, for more workgroups: 4800 rows, 4 heads of 64: 207 us, with 64 keys 226; 3000 rows,
+// 8 heads of 128 over 2, causal: 196, with 64 keys and one workgroup a CU 424.
+constexpr int padded(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : D <= 128 ? 128 : 256; }
+constexpr int tile_keys(int DT, int es) { return DT * es > 512 || (es == 4 && DT >= 64) ? 32 : 64; }
+constexpr int tile_blocks(int DT) { return DT <= 64 ? 4 : DT == 96 ? 3 : DT == 128 ? 2 : 1; }
 
 Plan plan(int64_t Tq, int64_t Tk, int sequences, int Hq, int Hk, int D, int dtype) {
     const int group = Hq / Hk;
@@ -651,19 +655,22 @@ Plan plan(int64_t Tq, int64_t Tk, int sequences, int Hq, int Hk, int D, int dtyp
         if (splits < even) splits = even;
     } else {
         // Rounds over the resident workgroups times a part's key tiles and its start, plus the join's traffic.  (One sequence of
-        // 4800 float32 rows, 4 heads of 64: 352 us unsplit, 226 in 3 parts, 260 in 4, 236 in 8; 96 rows before 30001 keys, 32
+        // 4800 float32 rows, 4 heads of 64: 357 us unsplit, 224 in 3 parts, 249 in 4, 213 in 5, 222 in 8; 96 rows before 30001 keys, 32
         // heads over 4: 518 unsplit, 100 in 10, 78 in 18, 85 in 32.)
-        const int bytes = row_bytes(D, dtype == VO_F32 ? 4 : 2), tile = bytes <= 512 ? 64 : 32;
-        const int64_t resident = 256 * (bytes <= 128 ? 4 : bytes <= 192 ? 3 : bytes <= 256 ? 2 : 1);
+        const int es = dtype == VO_F32 ? 4 : 2, tile = tile_keys(padded(D), es);
+        const int64_t resident = 256 * tile_blocks(padded(D));
+        // In float32 the products alone take the time, whichever workgroup of a CU they belong to: 2 x keys x features cycles a tile.
         // The lengths are on the device: where all workgroups run at once, the longest sequence, taken to be half as long again as the average, is what
         // they wait for (8 sequences of 71 to 1500 keys: 26 us unsplit, 16 in 4 parts; 2 equal ones of 20000 keys lose 5 %).
         const int64_t longest = keys + keys / 2 < Tk ? keys + keys / 2 : Tk;
-        const double tiles = (double)vo_ceil_div(keys, tile), most = (double)vo_ceil_div(longest, tile), tile_us = D / 128.0 * (dtype == VO_F32 ? 10.0 : 2.1);
+        const double tiles = (double)vo_ceil_div(keys, tile), most = (double)vo_ceil_div(longest, tile), tile_us = D / 128.0 * 2.1;
         const double join_us = (double)Tq * Hq * D * 8 / 4e6;        // per part: written and read once
         double best = 0.;
         for (int s = 1; s <= 64 && s <= (longest + 255) / 256; ++s) {
             const double blocks = (double)base * s, rounds = blocks <= resident ? 0.6 + 0.4 * blocks / resident : (double)((int64_t)((blocks + resident - 1) / resident));
-            const double us = rounds * ((blocks <= resident ? most : tiles) / s + 2.) * tile_us + (s > 1 ? 4. + s * join_us : 0.);
+            double us = rounds * ((blocks <= resident ? most : tiles) / s + 2.) * tile_us;
+            if (dtype == VO_F32) us = (double)vo_ceil_div(base * s, 256) * (most / s + 2.) * tile * padded(D) / 980.;
+            if (s > 1) us += 4. + s * join_us;
             if (s == 1 || us < best) {
                 best = us;
                 splits = s;
@@ -686,8 +693,7 @@ template <typename T, int DT> int launch(const AttArgs& a, const Plan& p, hipStr
         constexpr int KEYS = BYTES <= 128 ? 64 : 32, WAVES = BYTES <= 256 ? 8 : BYTES <= 512 ? 4 : 2;
         attention_rows<T, DT, KEYS, WAVES><<<grid, 64 * WAVES, 0, st>>>(a);
     } else {
-        constexpr int KEYS = BYTES <= 512 ? 64 : 32;
-        attention_tiles<T, DT, KEYS, BYTES <= 256 ? 2 : 1><<<grid, 256, 0, st>>>(a);
+        attention_tiles<T, DT, tile_keys(DT, sizeof(T)), tile_blocks(DT)><<<grid, 256, 0, st>>>(a);
     }
     VO_CHECK_LAUNCH("vo_attention");
     if (p.splits > 1) {
