@@ -643,8 +643,9 @@ Plan plan(int64_t Tq, int64_t Tk, int sequences, int Hq, int Hk, int D, int dtyp
     const int64_t base = p.tiles * Hk;
     int64_t splits = 1;
     if (p.rows) {
-        // Few workgroups: parts until every CU has one (and none two: that round would be as long again), of at least 256 keys, where the join's launch is worth it (one row before
-        // 777 keys, 8 key heads: 12.2 us unsplit, 12.0 in 4 parts; 1500 keys: 16.1 / 12.7; 4096: 33.0 / 18.0, 14.3 in 16).
+        // Few workgroups: parts until every CU has one (and none two: that round would be as long again), of at least 256 keys, where
+        // the join's launch is worth it (one row before 777 keys, 8 key heads: 12.2 us unsplit, 12.0 in 4 parts; 1500 keys: 16.1 /
+        // 12.7; 4096: 33.0 / 18.0, 14.3 in 16).
         if (keys >= 1024) {
             splits = 256 / base;
             if (splits > keys / 256) splits = keys / 256;
@@ -660,8 +661,9 @@ Plan plan(int64_t Tq, int64_t Tk, int sequences, int Hq, int Hk, int D, int dtyp
         const int es = dtype == VO_F32 ? 4 : 2, tile = tile_keys(padded(D), es);
         const int64_t resident = 256 * tile_blocks(padded(D));
         // In float32 the products alone take the time, whichever workgroup of a CU they belong to: 2 x keys x features cycles a tile.
-        // The lengths are on the device: where all workgroups run at once, the longest sequence, taken to be half as long again as the average, is what
-        // they wait for (8 sequences of 71 to 1500 keys: 26 us unsplit, 16 in 4 parts; 2 equal ones of 20000 keys lose 5 %).
+        // The lengths are on the device: where all workgroups run at once, the longest sequence, taken to be half as long again as the
+        // average, is what they wait for (8 sequences of 71 to 1500 keys: 26 us unsplit, 16 in 4 parts; 2 equal ones of 20000 keys
+        // lose 5 %).
         const int64_t longest = keys + keys / 2 < Tk ? keys + keys / 2 : Tk;
         const double tiles = (double)vo_ceil_div(keys, tile), most = (double)vo_ceil_div(longest, tile), tile_us = D / 128.0 * 2.1;
         const double join_us = (double)Tq * Hq * D * 8 / 4e6;        // per part: written and read once
