@@ -637,7 +637,8 @@ int vo_linear(const void* x, int64_t x_row_stride, const void* weight, const flo
 /* ---------------------------------------------------------------------------
  * Attention of packed sequences: row i of a sequence gives
  *     out[i,h,:] = sum_j p_ij v[j,h',:],   p_ij = softmax_j(scale * q[i,h,:] . k[j,h',:]),   h' = h / (q_heads / k_heads)
- * over the keys j of its sequence (scale from 1e-30 to 1e30); with causal != 0 over those with j <= i + Lk - Lq (Lq, Lk the sequence's rows and keys:
+ * over the keys j of its sequence (scale from 1e-30 to 1e30; scores of any size that float32 holds); with causal != 0 over
+ * those with j <= i + Lk - Lq (Lq, Lk the sequence's rows and keys:
  * its last row sees every key).  A row that sees no key gives zeros.  It has NO counterpart in the reference; it is the
  * all-pairs product of vo_corr_volume_1d / _2d without the volume: along the epipolar lines of a stereo pair (one sequence
  * a line, causal: a match lies never right of its pixel), among all pixels of a frame, over packed prompts of any lengths,

@@ -397,3 +397,62 @@ def test_refusals(vo):
     w = torch.zeros(8, 4, 300, device="cuda", dtype=torch.float16)
     with pytest.raises(VoHipError, match="at most 256"):
         ops.attention(w, w, w)
+
+
+def in_hull(y, v, dtype):
+    """Every result is a mean of the values: no further out than their extremes, but for the roundings of the weights (half a step
+    each, of 16-bit storage) and of the result, and 2 (n + 64) 2^-24 for the float32 sums of n terms, numerator and denominator."""
+    half = torch.finfo(dtype).eps / 2
+    slack = 1 + (2 * half + 4 * (len(v) + 64) * U32) * 1.05
+    top = v.double().abs().amax(0)
+    return bool((y.double().abs() <= top * slack).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("scale", [0.125, 1.0, 1e9, 1e30])
+@pytest.mark.parametrize("q_len,k_len", [([140], [300]), ([3], [300]), ([1], [31]), ([140], [4000]), ([3], [4000])])
+def test_scores_of_any_size_with_one_key_ahead_give_its_value(vo, dtype, causal, scale, q_len, k_len):
+    """Scores up to 4e9, times scales up to 1e30: products of two stored numbers, exact in float32.  The key that is furthest ahead has
+    the weight 1, the others' are under e^-100, so the result is its value, bit for bit."""
+    lq, lk, D = q_len[0], k_len[0], 64
+    q, k, v = make(q_len, k_len, 2, 1, D, dtype, 31)
+    q[:], k[:] = 0, 0
+    q[..., 7] = 3e4
+    g = torch.Generator(device="cuda").manual_seed(8)
+    # 256 to 32768 with eight bits each, so that equal ones are equal and different ones 2^-8 of themselves apart (products: 2^13 at least)
+    mant = torch.randint(128, 256, (lk,), generator=g, device="cuda").double()
+    power = torch.randint(1, 8, (lk,), generator=g, device="cuda").double()
+    sign = torch.randint(0, 2, (lk,), generator=g, device="cuda").double() * 2 - 1
+    k[:, 0, 7] = (sign * mant * 2 ** power).to(dtype)
+    y = ops.attention(q, k, v, causal=causal, scale=scale)
+    s = q[0, 0, 7].double() * k[:, 0, 7].double() * scale
+    for i in range(lq):
+        n = max(0, min(lk, i + 1 + lk - lq)) if causal else lk
+        best = s[:n] == s[:n].max()
+        others = s[:n][~best]
+        assert len(others) == 0 or float(s[:n].max() - others.max()) > 100
+        if int(best.sum()) == 1:
+            assert torch.equal(y[i], v[int(best.nonzero()[0])].expand(2, D)), i
+        else:                                                          # equal keys share the weight
+            assert in_hull(y[i], v[:n][best][:, 0], dtype), i
+
+
+@pytest.mark.parametrize("dtype,spread", [(torch.float32, 6e4), (torch.float32, 1e9), (torch.float16, 1.6e4), (torch.bfloat16, 6e4), (torch.bfloat16, 1e9)])
+@pytest.mark.parametrize("q_len,k_len", [([140], [300]), ([3], [300]), ([140], [4000]), ([3], [4000])])
+def test_large_random_scores_give_means_of_the_values(vo, dtype, spread, q_len, k_len):
+    """Normally distributed queries and keys of a spread near float16's largest numbers, and far over it."""
+    g = torch.Generator(device="cuda").manual_seed(9)
+    n = lambda *s: (torch.randn(*s, generator=g, device="cuda") * spread).clamp(-6e4 if dtype == torch.float16 else -1e30, 6e4 if dtype == torch.float16 else 1e30)
+    q, k = n(q_len[0], 2, 64).to(dtype), n(k_len[0], 1, 64).to(dtype)
+    v = (torch.randn(k_len[0], 1, 64, generator=g, device="cuda").abs() + 1).to(dtype)
+    y = ops.attention(q, k, v)
+    assert in_hull(y, v, dtype) and bool((y.double() >= 0.95).all())        # a row whose weights vanish would give zeros
+    # where one key is ahead by more than the scores can be off, its value is the result
+    for h in range(2):
+        s = q[:, h].double() @ k[:, 0].double().t().contiguous() * 0.125
+        b = q[:, h].double().abs() @ k[:, 0].double().abs().t().contiguous() * 0.125
+        top = s.topk(2, 1)
+        clear = top.values[:, 0] - top.values[:, 1] > 150 + 4 * 66 * U32 * b.amax(1) + 8 * U32 * s.abs().amax(1)
+        assert bool(clear.any())
+        assert torch.equal(y[clear, h], v[top.indices[clear, 0], 0])

@@ -11,9 +11,11 @@
 //                 at all) and no value crosses lanes.  m, l and the rescaling factor are one number per lane.
 // V^T in 16 bits comes out of LDS by the transposing read: four keys of one feature per lane.
 //
-// The exponent's argument is (s - m) * scale * log2(e), formed in one fused multiply-add; m follows the true maximum only
-// when it has grown by more than 2^8 in the exponentials, so most tiles need no rescaling of the sums (the exponentials are
-// then at most 256, which costs no bits in a floating-point format).
+// The exponent's argument is (s - m) * scale * log2(e), with the difference formed first: s c - m c in one fused multiply-add would
+// leave the rounding of m c in it, which is 16 and more where scores times c pass 2^28 (no weight would be near 1, sums would vanish or
+// overflow).  The instruction more costs the prompts below 1.5 %, heads of 32 features 8 %; both forms under a test of |m c| spill.
+// m follows the true maximum only when it has grown by more than 2^8 in the exponentials, so most tiles need no
+// rescaling of the sums (the exponentials are then at most 256, which costs no bits in a floating-point format).
 //
 // Two forms:
 //   tiles  a workgroup of four waves takes 128 rows of one key head (a row is a token and one of the heads that share the key
@@ -139,7 +141,7 @@ template <typename T, int DT, int KEYS> struct Core {
     // Lets m follow the row's largest score (`top`: this half's) where that pays (see the top of the file).
     __device__ __forceinline__ void follow(float top, float c) {
         top = across(top, [](float x, float y) { return fmaxf(x, y); });
-        if (__any(top * c > m * c + 8.f)) {                          // m starts at -inf
+        if (__any((top - m) * c > 8.f)) {                            // m starts at -inf; -inf - -inf is no reason either
             const float next = fmaxf(m, top);
             const float f = next == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - next) * c);
             l *= f;
@@ -153,9 +155,9 @@ template <typename T, int DT, int KEYS> struct Core {
     // Scores 2 j and 2 j + 1 of a block of 32 keys to exponentials, rounded to the storage type where that has 16 bits; `sum` takes
     // the unrounded ones.
     static constexpr int PW = sizeof(T) == 2 ? 8 : 16;               // registers of a block's exponentials
-    static __device__ __forceinline__ void weigh(const vo_f32x16& s, unsigned* p, float* sum, int j, float c, float base) {
-        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * j], c, base));
-        const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * j + 1], c, base));
+    static __device__ __forceinline__ void weigh(const vo_f32x16& s, unsigned* p, float* sum, int j, float c, float ref) {
+        const float x = __builtin_amdgcn_exp2f((s[2 * j] - ref) * c);
+        const float y = __builtin_amdgcn_exp2f((s[2 * j + 1] - ref) * c);
         sum[0] += x;
         sum[1] += y;
         if constexpr (sizeof(T) == 2) {
@@ -165,12 +167,11 @@ template <typename T, int DT, int KEYS> struct Core {
             p[2 * j + 1] = __builtin_bit_cast(unsigned, y);
         }
     }
-    __device__ __forceinline__ float base_of(float c) const { return m == -INFINITY ? 0.f : -m * c; }
     __device__ __forceinline__ void weights(const vo_f32x16* s, unsigned (*p)[PW], float c) {
-        const float base = base_of(c);
+        const float ref = m == -INFINITY ? 0.f : m;
         float sum[2] = {0.f, 0.f};
 #pragma unroll
-        for (int j = 0; j < 8 * KB; ++j) weigh(s[j / 8], p[j / 8], sum, j % 8, c, base);
+        for (int j = 0; j < 8 * KB; ++j) weigh(s[j / 8], p[j / 8], sum, j % 8, c, ref);
         l += sum[0] + sum[1];
     }
     // 16 bits: V^T of 16 keys (half `h` of block b) for every 32 features.  Keys r.. and r + 8.. : the lane supplies 8 bytes of row
@@ -431,7 +432,7 @@ __global__ __launch_bounds__(256, MIN_BLOCKS) void attention_tiles(const AttArgs
         store_rows<float, DT>(core.o, 1.f, a.D, lds + wave * HALF, lane, [&](int r) {
             return first + r < rows ? part_row(a, split, p.q0 + token_of(first + r), head_of(first + r)) : nullptr;
         });
-        if (have && lane < 32) *reinterpret_cast<float2*>(part_ml(a, split, p.q0 + token, head)) = make_float2(core.m * a.c, l);
+        if (have && lane < 32) *reinterpret_cast<float2*>(part_ml(a, split, p.q0 + token, head)) = make_float2(core.m, l);
     } else {
         store_rows<T, DT>(core.o, inverse(l), a.D, lds + wave * HALF, lane, [&](int r) {
             return first + r < rows ? out_row<T>(a, p.q0 + token_of(first + r), head_of(first + r)) : nullptr;
@@ -562,7 +563,7 @@ __global__ __launch_bounds__(64 * WAVES) void attention_rows(const AttArgs a) {
         }
     }
     if (a.splits > 1 && wave == 0 && lane < 32 && have)
-        *reinterpret_cast<float2*>(part_ml(a, split, p.q0 + token, head)) = make_float2(m * a.c, l);
+        *reinterpret_cast<float2*>(part_ml(a, split, p.q0 + token, head)) = make_float2(m, l);
 }
 
 // ------------------------------------------------------------------------------------------------------------- join
@@ -592,7 +593,7 @@ template <typename T, int WIDTH> __global__ __launch_bounds__(256) void attentio
     float m = ml.x;
 #pragma unroll
     for (int d = 32; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
-    const float w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - m);
+    const float w = ml.x == -INFINITY ? 0.f : exp2f((ml.x - m) * a.c);
     float l = w * ml.y;                                              // a part that saw no key of this row has neither weight nor sums
 #pragma unroll
     for (int d = 32; d; d >>= 1) l += __shfl_xor(l, d);
