@@ -653,7 +653,8 @@ int vo_linear(const void* x, int64_t x_row_stride, const void* weight, const flo
  *   rows and keys.  Rows outside every sequence are left as they were.  The offsets are read on the device and clamped to
  *   the tensors; results for offsets that do not ascend are unspecified.
  *   A key or value reaches the rows that see it and no others, whatever it holds: infinities and NaN too.  A key whose score is
- *   -infinity has no weight; a row with no other key gives zeros, like one that sees none.
+ *   -infinity has the weight zero; a row with no other key gives zeros, like one that sees none.  The product of a weight of zero
+ *   (also one that has underflown, in the storage type, beside the largest met up to there) and an infinite value is NaN.
  * workspace: vo_attention_workspace_bytes(...) bytes (often 0), 16-byte aligned, contents irrelevant.  Calls that share one
  * must be ordered on one stream; two captured graphs that may replay at once need one each.
  * ------------------------------------------------------------------------- */

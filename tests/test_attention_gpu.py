@@ -456,3 +456,52 @@ def test_large_random_scores_give_means_of_the_values(vo, dtype, spread, q_len, 
         clear = top.values[:, 0] - top.values[:, 1] > 150 + 4 * 66 * U32 * b.amax(1) + 8 * U32 * s.abs().amax(1)
         assert bool(clear.any())
         assert torch.equal(y[clear, h], v[top.indices[clear, 0], 0])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [32, 64, 96, 128, 256])
+@pytest.mark.parametrize("score", ["minus infinity", "underflows"])
+@pytest.mark.parametrize("q_len,k_len", [([200], [200]), ([130], [300]), ([140], [2000]), ([5], [90]), ([3], [300]), ([3], [2000])])
+def test_an_infinite_value_without_weight_gives_nan_wherever_its_tile_lies(vo, dtype, D, score, q_len, k_len):
+    """Zero times infinity, in a tile that every row sees whole, in one on the diagonal and in any part of a split axis: rows that see the
+    key have a NaN in that feature and nothing else, the others have nothing of it."""
+    lq, lk = q_len[0], k_len[0]
+    g = torch.Generator(device="cuda").manual_seed(13)
+    for at in sorted({0, 1, lk // 2, max(lk - lq, 0) + lq // 2, lk - 2}):
+        q, k, v = make(q_len, k_len, 2, 1, D, dtype, 14 + at)
+        q[..., 0] = 4
+        k[at, 0] = 0
+        k[at, 0, 0] = float("-inf") if score == "minus infinity" else -1000.0        # e^-500 is no float32
+        clean = reference(q, torch.cat([k[:at], k[at + 1:]]), torch.cat([v[:at], v[at + 1:]]), [lq], [lk - 1], False, D ** -0.5 if D < 64 else 0.125)
+        for causal in (False, True):
+            v2 = v.clone()
+            v2[at, 0, 3] = float("inf")
+            y = ops.attention(q, k, v2, causal=causal, scale=D ** -0.5 if D < 64 else 0.125)
+            without = ops.attention(q, k, v, causal=causal, scale=D ** -0.5 if D < 64 else 0.125)
+            last = torch.arange(lq, device="cuda") + (lk - lq) if causal else torch.full((lq,), lk - 1, device="cuda")
+            sees = last >= at
+            alone = (last == 0) & sees                                  # a row's only key: finite scores have the weight 1 there
+            want = y[..., 3].isinf() & (alone & (score == "underflows"))[:, None] | y[..., 3].isnan()
+            assert bool(want[sees].all()), (at, causal)
+            assert torch.equal(y[~sees], without[~sees]), (at, causal)
+            y[..., 3] = without[..., 3]                                 # the other features have the same bits, whatever the tile went through
+            assert bool(y.isfinite().all()) and torch.equal(y, without), (at, causal)
+            if not causal:
+                check(without, *clean)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("q_len,k_len", [([140], [140]), ([140], [2000]), ([4], [4]), ([3], [2000])])
+def test_rows_whose_only_scores_are_minus_infinity(vo, dtype, q_len, k_len):
+    """Zeros under finite values; NaN in the features of values that are not finite."""
+    q, k, v = make(q_len, k_len, 1, 1, 32, dtype, 15)
+    q[..., 0], k[:] = 4, 0
+    k[..., 0] = float("-inf")
+    for causal in (False, True):
+        assert bool((ops.attention(q, k, v, causal=causal) == 0).all())
+    v[0, 0, 3], v[0, 0, 9] = float("inf"), float("nan")
+    for causal in (False, True):
+        y = ops.attention(q, k, v, causal=causal)
+        assert bool(y[..., [3, 9]].isnan().all())
+        y[..., [3, 9]] = 0
+        assert bool((y == 0).all())

@@ -212,7 +212,8 @@ template <typename T, int DT, int KEYS> struct Core {
     }
     // Values that are infinite or NaN ("unbounded").  Where all rows see the same keys they are products like others; where a row
     // does not see a key its weight is zero, and zero times such a value is no zero.  So a tile on a causal sequence's diagonal
-    // that holds any is multiplied with zeros in their place, and they are added at the end to the rows that see them.
+    // that holds any is multiplied with zeros in their place, and their products are added at the end to the rows that see them: the
+    // value itself (any positive weight times it is it), or NaN where the weight beside the row's largest is zero all the same.
     static constexpr unsigned EXP = sizeof(T) == 4 ? 0x7f800000u : __is_same(T, _Float16) ? 0x7c00u : 0x7f80u;
     static __device__ __forceinline__ bool unbounded(unsigned bits) { return (bits & EXP) == EXP; }
     // Is there any in the tile?
@@ -247,11 +248,32 @@ template <typename T, int DT, int KEYS> struct Core {
             *x = vo_u32x4{bounded((*x)[0]), bounded((*x)[1]), bounded((*x)[2]), bounded((*x)[3])};
         }
     }
-    // The unbounded values of the keys from .. to - 1 of `v`, added as they are (any positive weight times them is them) to the sums
-    // of the rows that see them.
-    __device__ __forceinline__ void add_unbounded(const T* v, int64_t stride, int64_t from, int64_t to, int64_t limit, int D, int lane) {
+    // The products of the unbounded values of the tile's `keys` keys, in memory from `v` on, added to the sums; kt: the keys.  The scores
+    // are formed once more: to keep the weights' zeros from the loop would cost its kernels registers that they spill.
+    __device__ __forceinline__ void add_unbounded(const unsigned char* kt, const T* v, int64_t stride, int keys, int limit, float c, int D, int lane) {
+        vo_f32x16 s[KB];
+        unsigned none[KB];                                           // the row's keys of weight zero: a bit for each of a block's 32
+        scores(kt, s, lane);
+        const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int b = 0; b < KB; ++b) {
+            unsigned u = 0;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float w = __builtin_amdgcn_exp2f((s[b][i] - ref) * c);
+                bool zero = w == 0.f;
+                if constexpr (sizeof(T) == 2) zero = (E::pack2(w, 0.f) & 0x7fffu) == 0;
+                u |= (unsigned)zero << (8 * (i >> 2) + (i & 3));
+            }
+            const auto both = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+            none[b] = both[0] | both[1] << 4;                        // the upper half of the wave holds the keys four further
+        }
 #pragma unroll 1
-        for (int64_t r = from; r < to; ++r)
+        for (int r = 0; r < keys; ++r) {
+            unsigned u = none[0];
+#pragma unroll
+            for (int b = 1; b < KB; ++b) u = r >> 5 == b ? none[b] : u;
+            const bool zero = u >> (r & 31) & 1;
 #pragma unroll
             for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -261,9 +283,10 @@ template <typename T, int DT, int KEYS> struct Core {
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const float x = E::get(v + r * stride + f + j);
-                        if (!(fabsf(x) < INFINITY)) o[d][4 * b + j] += x;
+                        if (!(fabsf(x) < INFINITY)) o[d][4 * b + j] += zero ? NAN : x;
                     }
                 }
+        }
     }
     // A whole tile.
     __device__ __forceinline__ void step(const unsigned char* kt, const unsigned char* vt, float c, bool masked, int limit, int lane) {
@@ -393,7 +416,7 @@ __global__ __launch_bounds__(256, MIN_BLOCKS) void attention_tiles(const AttArgs
     // wholly below `all` are seen by every row of the workgroup
     const int64_t limit = a.causal ? vo_clamp64(token + shift + 1, 0, p.Lk) : p.Lk;
     const int64_t all = a.causal ? vo_clamp64(first_token + shift + 1, 0, p.Lk) : p.Lk;
-    int64_t unbounded = p.Lk;                                        // first key of the first tile that was bounded
+    int64_t unbounded = t1;                                          // the first tile that was bounded
     const int64_t wave_all = a.causal ? vo_clamp64(token_of(first) + shift + 1, 0, p.Lk) : p.Lk;
     const int64_t wave_any = first >= rows ? 0 : a.causal ? vo_clamp64(token_of(first + 31) + shift + 1, 0, p.Lk) : p.Lk;
 
@@ -420,12 +443,18 @@ __global__ __launch_bounds__(256, MIN_BLOCKS) void attention_tiles(const AttArgs
             vo_lds_barrier();
             core.bound(now + HALF, wave, 4, lane);
             vo_lds_barrier();
-            unbounded = key < unbounded ? key : unbounded;
+            unbounded = t < unbounded ? t : unbounded;
         }
         if (key < wave_any) core.step(now, now + HALF, a.c, key + KEYS > wave_all, (int)vo_clamp64(limit - key, 0, KEYS), lane);
         unsigned char* x = now; now = next; next = x;
     }
-    if (unbounded < p.Lk) core.add_unbounded(vb, a.vs, unbounded, t1 * KEYS < p.Lk ? t1 * KEYS : p.Lk, limit, a.D, lane);
+    for (int64_t t = unbounded; t < t1; ++t) {
+        vo_lds_barrier();
+        fetch_k(t, now);
+        vo_lds_barrier();
+        const int64_t key = t * KEYS;
+        if (key < wave_any) core.add_unbounded(now, vb + key * a.vs, a.vs, (int)vo_clamp64(p.Lk - key, 0, KEYS), (int)vo_clamp64(limit - key, 0, KEYS), a.c, a.D, lane);
+    }
     const float l = core.across(core.l, [](float x, float y) { return x + y; });
     vo_lds_barrier();                                                // every wave is done with the key tiles
     if (a.splits > 1) {
@@ -495,6 +524,7 @@ __global__ __launch_bounds__(64 * WAVES) void attention_rows(const AttArgs a) {
         fetch_k(t0 + wave);
         fetch_v(t0 + wave);
     }
+    int64_t unbounded = t1;                                          // the wave's first tile that was bounded
     for (int64_t t = t0 + wave; t < t1; t += WAVES) {
         const int64_t key = t * KEYS;
         vo_f32x16 s[core.KB];
@@ -507,15 +537,21 @@ __global__ __launch_bounds__(64 * WAVES) void attention_rows(const AttArgs a) {
         core.follow(core.largest(s), a.c);
         core.weights(s, w, a.c);
         arrived();
-        const bool partial = key + KEYS > all && all < p.Lk && core.any_unbounded(vt, lane);
-        if (partial) {
+        if (key + KEYS > all && all < p.Lk && core.any_unbounded(vt, lane)) {
             core.bound(vt, 0, 1, lane);
             vo_wave_lds_fence();
+            unbounded = t < unbounded ? t : unbounded;
         }
         core.accumulate(vt, w, lane);
         consumed();
         fetch_v(t + WAVES);
-        if (partial) core.add_unbounded(vb, a.vs, key, key + KEYS < p.Lk ? key + KEYS : p.Lk, limit, a.D, lane);
+    }
+    for (int64_t t = unbounded; t < t1; t += WAVES) {
+        const int64_t key = t * KEYS;
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // nothing is under way into the tile or read from it
+        fetch_k(t);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        core.add_unbounded(kt, vb + key * a.vs, a.vs, (int)vo_clamp64(p.Lk - key, 0, KEYS), (int)vo_clamp64(limit - key, 0, KEYS), a.c, a.D, lane);
     }
     core.l = core.across(core.l, [](float x, float y) { return x + y; });
 
