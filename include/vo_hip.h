@@ -646,8 +646,8 @@ int vo_linear(const void* x, int64_t x_row_stride, const void* weight, const flo
  *   q, out (q_tokens, q_heads, D), k, v (k_tokens, k_heads, D): D consecutive elements per token and head, token and head
  *   strides in ELEMENTS, so slices of one fused projection are fine.  Storage VO_F32, VO_F16 or VO_BF16; products, softmax
  *   and sums in float32; with 16-bit storage the exponentials are rounded to it (relative to the row's largest) before they
- *   meet v, and the result is rounded once.  D at most 256; D, strides and pointers whole 16-byte pieces, strides under
- *   16 MiB (VO_ERR_UNSUPPORTED otherwise).  out overlaps none of the inputs.
+ *   meet v, and the result is rounded once.  D at most 256; D, strides and pointers whole 16-byte pieces, tokens under
+ *   16 MiB apart (VO_ERR_UNSUPPORTED otherwise); heads may lie any distance apart.  out overlaps none of the inputs.
  *   q_offsets, k_offsets: device arrays of sequences + 1 ascending int32: sequence s owns the rows [q_offsets[s],
  *   q_offsets[s+1]) and the keys [k_offsets[s], k_offsets[s+1]), any length from 0; or both NULL with sequences = 1: all
  *   rows and keys.  Rows outside every sequence are left as they were.  The offsets are read on the device and clamped to

@@ -505,3 +505,32 @@ def test_rows_whose_only_scores_are_minus_infinity(vo, dtype, q_len, k_len):
         assert bool(y[..., [3, 9]].isnan().all())
         y[..., [3, 9]] = 0
         assert bool((y == 0).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lq", [1, 40, 200])
+def test_heads_more_than_16_mib_apart(vo, dtype, lq):
+    """A cache with its heads outermost, as a transposed view: 70000 tokens of 128 features lie 17 MiB (float32: 34) apart."""
+    n, D = 70000, 128
+    g = torch.Generator(device="cuda").manual_seed(17)
+    cache = torch.randn(2, 2, n, D, generator=g, device="cuda").to(dtype)
+    k, v = cache[0].transpose(0, 1), cache[1].transpose(0, 1)
+    assert k.stride(1) * k.element_size() >= 1 << 24
+    hold = torch.empty(4, n, D, device="cuda", dtype=dtype)             # queries and results likewise
+    hold[:, :lq] = torch.randn(4, lq, D, generator=g, device="cuda").to(dtype)
+    q = hold.transpose(0, 1)[:lq]
+    out = torch.full((4, n, D), 7.0, device="cuda", dtype=dtype)
+    y = ops.attention(q, k, v, causal=True, out=out.transpose(0, 1)[:lq])
+    want = ops.attention(q.contiguous(), k.contiguous(), v.contiguous(), causal=True)
+    assert torch.equal(y, want) and bool((out[:, lq:] == 7).all())
+    check(want[:1], *reference(q[:1], k[:n - lq + 1], v[:n - lq + 1], [1], [n - lq + 1], True, D ** -0.5))
+
+
+def test_tokens_16_mib_apart_are_refused(vo):
+    from visual_odometry_amd._lib import VoHipError
+    hold = torch.zeros(3 << 23, device="cuda", dtype=torch.float16)
+    far = hold.as_strided((2, 1, 32), (1 << 23, 32, 1))
+    near = torch.zeros(2, 1, 32, device="cuda", dtype=torch.float16)
+    for args in ((far, near, near), (near, far, near), (near, near, far)):
+        with pytest.raises(VoHipError, match="under 16 MiB"):
+            ops.attention(*args)

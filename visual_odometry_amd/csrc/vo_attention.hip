@@ -773,10 +773,14 @@ extern "C" int vo_attention(const void* q, int64_t q_token_stride, int64_t q_hea
     if (D < 1 || D > 256 || D * es % 16) return vo_fail(VO_ERR_UNSUPPORTED, "vo_attention: D=%d must be at most 256 and whole 16-byte pieces", D);
     if (q_tokens == 0) return VO_OK;
     VO_REQUIRE(q && out && (k_tokens == 0 || (k && v)), "vo_attention: null pointer");
-    const int64_t strides[] = {q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride, out_token_stride, out_head_stride};
-    for (int64_t s : strides)
-        if (s < 0 || s * es % 16 || s * es >= (1ll << 24))
-            return vo_fail(VO_ERR_UNSUPPORTED, "vo_attention: strides must be whole 16-byte pieces under 16 MiB (got %lld elements)", (long long)s);
+    // a key tile is addressed with 32-bit offsets from its first token; heads are 64-bit products
+    const int64_t strides[] = {q_token_stride, k_token_stride, v_token_stride, out_token_stride, q_head_stride, k_head_stride, v_head_stride, out_head_stride};
+    for (int i = 0; i < 8; ++i) {
+        const int64_t s = strides[i];
+        if (s < 0 || s % (16 / es) || (i < 4 && s >= (1ll << 24) / es))
+            return vo_fail(VO_ERR_UNSUPPORTED, "vo_attention: strides must be whole 16-byte pieces, tokens' under 16 MiB (got %lld elements between %s)",
+                           (long long)s, i < 4 ? "tokens" : "heads");
+    }
     if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(out)) % 16)
         return vo_fail(VO_ERR_UNSUPPORTED, "vo_attention: tensors must be 16-byte aligned");
     if (q_tokens >= (1ll << 31) || k_tokens >= (1ll << 31))

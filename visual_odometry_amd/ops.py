@@ -1232,8 +1232,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: torc
     serves for both when Tq = Tk).  Every row takes softmax(scale * q.k) over its sequence's keys, ``causal``: over the keys
     j <= i + Lk - Lq (aligned at the ends, so a single new row sees the whole history); a row that sees no key gives zeros.
     ``scale`` defaults to 1/sqrt(D).  float32, float16 or bfloat16; scores, softmax and sums in float32.  Tokens and heads may
-    lie any whole number of 16-byte pieces apart (slices of a fused projection); D is at most 256 and a multiple of 8 (4 in
-    float32).  Rows outside every sequence are not written (give ``out`` to say what they hold).  The lengths stay on the
+    lie any whole number of 16-byte pieces apart, tokens under 16 MiB (slices of a fused projection, a cache with its heads
+    outermost); D is at most 256 and a multiple of 8 (4 in float32).  Rows outside every sequence are not written (give ``out`` to say what they hold).  The lengths stay on the
     device: nothing synchronises, and the call can be captured.  Equal inputs give equal bits.  Forward only: nothing is recorded
     for autograd."""
     _token_tensor(q, "q")
