@@ -213,3 +213,46 @@ def test_refusals(vo):
         ops.linear(buf[:, :16], w, out=buf[:, 8:32])
     with pytest.raises(ValueError, match="overlaps residual"):
         ops.linear(x, w, residual=buf[:, :24], out=buf[:, 8:32])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("M,C,K", [(3, 8, 40), (24, 8, 40), (300, 8, 256), (2, 4096, 40), (70, 4100, 64)])
+def test_activations_keep_their_digits_on_the_negative_side(vo, dtype, act, M, C, K):
+    """z from -12 (gelu_tanh: -9) to 0, one product of two numbers of eight bits, so exact: the result is right relative to itself, however
+    near to zero it is.  An exponential's argument e (z^2 / 2 for gelu, up to 144 / 2) takes at most eight roundings of itself -- gelu:
+    |z| / sqrt 2 two, each twice in its square, the square and the change of base one or two each; gelu_tanh: a cube, a sum and
+    three factors; silu: two -- and an error of an exponent is a relative one of the result.  2^-20 for the functions themselves and the
+    few products around them (16 bits: 2^-19, GELU's polynomial is off by 8e-7); the store's half step, of a subnormal where the result is one."""
+    x = torch.zeros(M, C, device="cuda", dtype=dtype)
+    w = torch.zeros(K, C, device="cuda", dtype=dtype)
+    lo = -12.0 if act != "gelu_tanh" else -9.0
+    x[:, 3] = torch.linspace(lo, -0.01, M, device="cuda").bfloat16().to(dtype)                # eight bits each, in every type
+    w[:, 3] = (1 - torch.arange(K, device="cuda") / (2.0 * K)).bfloat16().to(dtype)
+    z = x[:, 3].double()[:, None] * w[:, 3].double()[None, :]
+    if act == "gelu":
+        want, e = 0.5 * z * torch.erfc(z * -math.sqrt(0.5)), z * z / 2          # torch's ndtr is (1 + erf) / 2: no digits left at -8
+    elif act == "silu":
+        want, e = z * torch.sigmoid(z), z.abs()
+    else:
+        u = 2 * math.sqrt(2 / math.pi) * (z + 0.044715 * z ** 3)
+        want, e = z * torch.sigmoid(u), u.abs()
+    got = ops.linear(x, w, activation=act).double()
+    rel = 8 * U32 * (e + 1) + (2.0 ** -20 if dtype == torch.float32 else 2.0 ** -19)
+    smallest = {torch.float32: 2.0 ** -126, torch.float16: 2.0 ** -14, torch.bfloat16: 2.0 ** -126}[dtype]
+    half = torch.finfo(dtype).eps / 2
+    tol = want.abs() * (rel + half) * 1.01 + smallest * half * 1.01
+    worst = ((got - want).abs() / tol).max().item()
+    assert worst <= 1.0, f"error {worst:.3g} times the bound"
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", ["relu", "gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("M", [3, 40, 300])
+def test_activations_of_the_largest_numbers(vo, dtype, act, M):
+    """Large numbers and infinity above zero stay as they are, large ones below become zero, NaN stays NaN."""
+    big = torch.finfo(dtype).max
+    x = torch.tensor([big, float("inf"), -big, float("nan"), 50.0, -300.0], device="cuda").to(dtype).repeat(M // 6 + 1)[:M, None]
+    y = ops.linear(x, torch.ones(24, 1, device="cuda", dtype=dtype), activation=act)
+    above, below = (x > 0).expand(M, 24), (x < 0).expand(M, 24)
+    assert torch.equal(y[above], x.expand(M, 24)[above]) and bool((y[below] == 0).all()) and bool(y[x.isnan().expand(M, 24)].isnan().all())
