@@ -534,3 +534,24 @@ def test_tokens_16_mib_apart_are_refused(vo):
     for args in ((far, near, near), (near, far, near), (near, near, far)):
         with pytest.raises(VoHipError, match="under 16 MiB"):
             ops.attention(*args)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lens", [[150, 33, 0, 260], [1, 2, 1]])
+@pytest.mark.parametrize("order", ["token", "head"])
+def test_result_beside_its_inputs_in_one_buffer(vo, dtype, lens, order):
+    """The result takes heads of the buffer that holds q, k and v: no element is shared."""
+    Hq, Hk, D, T = 4, 2, 64, sum(lens)
+    g = torch.Generator(device="cuda").manual_seed(2)
+    n = 2 * Hq + 2 * Hk
+    hold = torch.randn(T, n, D, generator=g, device="cuda").to(dtype)
+    if order == "head":
+        hold = hold.transpose(0, 1).contiguous().transpose(0, 1)
+    keep = hold.clone()
+    q, k, v, out = hold[:, :Hq], hold[:, Hq:Hq + Hk], hold[:, Hq + Hk:Hq + 2 * Hk], hold[:, Hq + 2 * Hk:]
+    ops.attention(q, k, v, offsets(lens), causal=True, out=out)
+    assert torch.equal(hold[:, :Hq + 2 * Hk], keep[:, :Hq + 2 * Hk])
+    check(out, *reference(keep[:, :Hq], keep[:, Hq:Hq + Hk], keep[:, Hq + Hk:Hq + 2 * Hk], lens, lens, True, D ** -0.5))
+    for first in (1, Hq - 1, Hq, Hq + Hk, Hq + 2 * Hk - 1):
+        with pytest.raises(ValueError, match="overlaps"):
+            ops.attention(q, k, v, offsets(lens), causal=True, out=hold[:, first:first + Hq])

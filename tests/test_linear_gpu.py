@@ -256,3 +256,37 @@ def test_activations_of_the_largest_numbers(vo, dtype, act, M):
     y = ops.linear(x, torch.ones(24, 1, device="cuda", dtype=dtype), activation=act)
     above, below = (x > 0).expand(M, 24), (x < 0).expand(M, 24)
     assert torch.equal(y[above], x.expand(M, 24)[above]) and bool((y[below] == 0).all()) and bool(y[x.isnan().expand(M, 24)].isnan().all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,C,K", [(1, 40, 24), (9, 72, 40), (96, 71, 33), (1600, 72, 2048), (3, 4096, 64), (1201, 1003, 1100)])
+def test_x_residual_and_result_side_by_side_in_one_buffer(vo, dtype, M, C, K):
+    """Column ranges of one buffer share no element."""
+    x, w, b, r = make(M, C, K, dtype, 13, res=True)
+    buf = torch.full((M, C + 2 * K + 3), 7.0, device="cuda", dtype=dtype)
+    buf[:, :C], buf[:, C:C + K] = x, r
+    ops.linear(buf[:, :C], w, b, "relu", buf[:, C:C + K], out=buf[:, C + K:C + 2 * K])
+    check(buf[:, C + K:C + 2 * K], x, w, b, "relu", r)
+    assert torch.equal(buf[:, :C], x) and torch.equal(buf[:, C:C + K], r) and bool((buf[:, C + 2 * K:] == 7).all())
+
+
+def test_columns_that_meet_are_refused(vo):
+    """One shared column at either end, across the buffer's line end, or between rows of different strides."""
+    x, w, b, r = make(8, 16, 24, torch.float16, 1, res=True)
+    buf = torch.zeros(9, 64, device="cuda", dtype=torch.float16)
+    flat = buf.view(-1)
+    for at in (0, 1, 15, -23, -1):                                      # x in columns 24 .. 39, the result 24 wide at 24 + at
+        with pytest.raises(ValueError, match="overlaps x"):
+            ops.linear(buf[:8, 24:40], w, out=buf[:8, 24 + at:48 + at])
+    ops.linear(buf[:8, 24:40], w, out=buf[:8, 40:64])
+    ops.linear(buf[:8, 24:40], w, out=buf[:8, 0:24])
+    late = flat[56:56 + 8 * 64].view(8, 64)[:, :16]                     # columns 56 .. 63 and the next row's 0 .. 7
+    with pytest.raises(ValueError, match="overlaps x"):
+        ops.linear(late, w, out=buf[:8, 0:24])
+    with pytest.raises(ValueError, match="overlaps x"):
+        ops.linear(late, w, out=buf[:8, 40:64])
+    ops.linear(late, w, out=buf[:8, 8:32])
+    with pytest.raises(ValueError, match="overlaps x"):
+        ops.linear(buf[0:8:2, 0:16], w, out=flat[16:16 + 4 * 40].view(4, 40)[:, :24])
+    with pytest.raises(ValueError, match="overlaps weight"):
+        ops.linear(x[:2], buf[:6].view(24, 16), out=buf[2:4, :24])

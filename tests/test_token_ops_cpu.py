@@ -140,3 +140,35 @@ def test_the_python_entry_points_refuse_cpu_tensors():
         ops.linear(torch.zeros(2, 8), torch.zeros(4, 8))
     with pytest.raises(ValueError, match="GPU tensor"):
         ops.attention(torch.zeros(2, 1, 8), torch.zeros(2, 1, 8), torch.zeros(2, 1, 8))
+
+
+def test_overlaps_are_found_and_column_ranges_are_none():
+    """Against the elements themselves: two random strided views of one buffer that share an element are always refused, and rows the same
+    distance apart never where they share no column."""
+    import random
+    import torch
+    from visual_odometry_amd import ops
+    rng, base, ids = random.Random(0), torch.zeros(2000, dtype=torch.float16), torch.arange(2000)
+
+    def view(step=0):
+        if step or rng.random() < 0.6:
+            n = (rng.randint(2 if step else 1, 6), rng.randint(1, 12))
+            return n, (step or rng.choice([n[1], n[1] + rng.randint(0, 30), 48, 24]), 1), rng.randint(0, 200)
+        n = (rng.randint(1, 5), rng.randint(1, 3), rng.randint(1, 8))
+        return n, rng.choice([(n[1] * n[2] + rng.randint(0, 30), n[2], 1), (48, n[2] + rng.randint(0, 4), 1),
+                              (n[2], n[0] * n[2] + rng.randint(0, 9), 1), (96, 0, 1)]), rng.randint(0, 200)
+
+    def refused(a, b):
+        try:
+            ops._no_overlap(a, b, "x")
+        except ValueError:
+            return True
+        return False
+    for step in [0] * 3000 + [40] * 3000:
+        a, b = view(step), view(step)
+        shared = bool(set(ids.as_strided(*a).flatten().tolist()) & set(ids.as_strided(*b).flatten().tolist()))
+        says = refused(base.as_strided(*a), base.as_strided(*b))
+        assert says or not shared, (a, b)
+        if step:
+            columns = [{(v[2] + i) % step for i in range(v[0][1])} for v in (a, b)]
+            assert not says or columns[0] & columns[1], (a, b)

@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import math
 
 import numpy as np
 import torch
@@ -1139,12 +1140,29 @@ def _span(t: torch.Tensor):
     return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
 
 
+def _lines(t: torch.Tensor):
+    """The lines a tensor lies in: (bytes from one to the next, bytes a line reaches); 0 from one to the next where it is one line."""
+    axes = sorted((s * t.element_size(), n) for n, s in zip(t.shape, t.stride()) if n > 1)
+    reach = t.element_size()
+    for i, (step, n) in enumerate(axes):
+        if i == len(axes) - 1 and step > reach:
+            return step, reach
+        reach += (n - 1) * step
+    return 0, reach
+
+
 def _no_overlap(out: torch.Tensor, t: torch.Tensor | None, name: str) -> None:
     if t is None or t.numel() == 0 or out.numel() == 0:
         return
     (a, b), (c, d) = _span(out), _span(t)
-    if a < d and c < b:
-        raise ValueError(f"out overlaps {name} in memory")
+    if b <= c or d <= a:
+        return
+    # column ranges of one buffer: counted modulo the lines' common distance, t's line lies behind out's and ends before out's next
+    (out_step, out_reach), (step, reach) = _lines(out), _lines(t)
+    common = math.gcd(out_step, step)
+    if common and out_reach <= (c - a) % common <= common - reach:
+        return
+    raise ValueError(f"out overlaps {name} in memory")
 
 
 @functools.lru_cache(maxsize=4096)
@@ -1172,7 +1190,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     epilogue are float32 with one rounding at the store.  ``activation``: None, "relu", "gelu" (the error function's form),
     "gelu_tanh" or "silu"; it comes before the residual is added.  Rows of x, residual and out may lie any distance apart
     (slices of wider tensors), a row's elements are consecutive; weight is contiguous.  ``out`` may be the residual itself;
-    it must not overlap anything else.  Sums are formed in a fixed order: equal inputs give equal bits.  Forward only: nothing is
+    it must not overlap anything else (columns of one buffer that x, residual and out share out among them are fine).  Sums are
+    formed in a fixed order: equal inputs give equal bits.  Forward only: nothing is
     recorded for autograd."""
     _token_tensor(x, "x")
     _token_tensor(weight, "weight", x)
