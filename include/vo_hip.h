@@ -616,7 +616,8 @@ int vo_ransac_kabsch_batch(const double* P, const double* Q, const uint8_t* weig
  *     y[m,k] = act( sum_c x[m,c] * weight[k,c] + bias[k] ) + residual[m,k]
  * It has NO counterpart in the reference; it is vo_conv1x1 for tensors whose rows are pixels or tokens (the layout of
  * vo_conv1x1_pixel_major's output and of vo_attention below), in three storage types.
- *   x (M,C), y and residual (M,K): rows of consecutive elements, row strides in ELEMENTS (at least the row's length).
+ *   x (M,C), y and residual (M,K): rows of consecutive elements, row strides in ELEMENTS (at least the row's length; the
+ *   residual's may be 0: one row for all).
  *   weight (K,C) dense, bias (K) float32 or NULL, residual NULL or of x's type.  y may be the residual itself (same
  *   pointer and stride); otherwise it must not overlap any input.
  *   activation  VO_ACT_*: GELU is 0.5 z (1 + erf(z/sqrt(2))), GELU_TANH its tanh form, SILU z / (1 + exp(-z)).

@@ -290,3 +290,19 @@ def test_columns_that_meet_are_refused(vo):
         ops.linear(buf[0:8:2, 0:16], w, out=flat[16:16 + 4 * 40].view(4, 40)[:, :24])
     with pytest.raises(ValueError, match="overlaps weight"):
         ops.linear(x[:2], buf[:6].view(24, 16), out=buf[2:4, :24])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,C,K", [(1, 40, 24), (9, 72, 40), (96, 71, 33), (1600, 72, 2048), (3, 4096, 64), (70, 4100, 64), (1201, 1003, 1100)])
+def test_one_residual_row_for_all(vo, dtype, M, C, K):
+    """A residual expanded over the rows (their stride is 0)."""
+    x, w, b, r = make(M, C, K, dtype, 14, res=True)
+    y = ops.linear(x, w, b, "gelu", r[:1].expand(M, K))
+    check(y, x, w, b, "gelu", r[:1].expand(M, K))
+    assert torch.equal(y, ops.linear(x, w, b, "gelu", r[:1].expand(M, K).contiguous()))
+    if M == 96:
+        assert torch.equal(ops.linear(x.view(2, 48, C), w, b, "gelu", r[0].expand(2, 48, K)).view(M, K), y)
+        with pytest.raises(ValueError, match="out: rows overlap"):
+            ops.linear(x, w, out=r[:1].expand(M, K))
+        with pytest.raises(ValueError, match="rows overlap"):
+            ops.linear(x, w, residual=r.view(-1).as_strided((M, K), (1, 1)))

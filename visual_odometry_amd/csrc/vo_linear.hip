@@ -577,8 +577,8 @@ extern "C" int vo_linear(const void* x, int64_t x_row_stride, const void* weight
     VO_REQUIRE(M >= 0 && C >= 1 && K >= 1, "vo_linear: M=%lld C=%d K=%d (M >= 0, C >= 1, K >= 1 required)", (long long)M, C, K);
     if (M == 0) return VO_OK;
     VO_REQUIRE(x && weight && y, "vo_linear: null pointer");
-    VO_REQUIRE(x_row_stride >= C && y_row_stride >= K && (!residual || residual_row_stride >= K),
-               "vo_linear: row strides must be at least the rows' lengths");
+    VO_REQUIRE(x_row_stride >= C && y_row_stride >= K && (!residual || residual_row_stride >= K || residual_row_stride == 0),
+               "vo_linear: row strides must be at least the rows' lengths (the residual's may be 0)");
     const int64_t es = dtype == VO_F32 ? 4 : 2;
     const Plan p = plan(M, C, K, dtype);
     // a tile's rows are addressed with 32-bit offsets

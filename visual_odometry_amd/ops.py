@@ -1111,8 +1111,9 @@ def _token_tensor(t, name: str, like: torch.Tensor | None = None) -> torch.Tenso
     return t
 
 
-def _rows(t: torch.Tensor, name: str, width: int):
-    """(..., width) whose leading axes collapse to rows one stride apart -> (ptr, rows, row stride in elements)."""
+def _rows(t: torch.Tensor, name: str, width: int, one_row: bool = False):
+    """(..., width) whose leading axes collapse to rows one stride apart -> (ptr, rows, row stride in elements).  ``one_row``: the
+    stride may be 0 (one row expanded over all)."""
     shape, st = t.shape, t.stride()
     if not shape or shape[-1] != width:
         raise ValueError(f"{name}: expected rows of {width}, got shape {tuple(shape)}")
@@ -1129,7 +1130,7 @@ def _rows(t: torch.Tensor, name: str, width: int):
         raise ValueError(f"{name}: a row's elements must be consecutive (got strides {st})")
     if m == 1:
         return t.data_ptr(), 1, width
-    if st[0] < width:
+    if st[0] < width and not (one_row and st[0] == 0):
         raise ValueError(f"{name}: rows overlap (got strides {st})")
     return t.data_ptr(), m, st[0]
 
@@ -1189,7 +1190,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     x, weight, residual and out are float32, float16 or bfloat16 alike, bias (K) is float32; products, sums and the
     epilogue are float32 with one rounding at the store.  ``activation``: None, "relu", "gelu" (the error function's form),
     "gelu_tanh" or "silu"; it comes before the residual is added.  Rows of x, residual and out may lie any distance apart
-    (slices of wider tensors), a row's elements are consecutive; weight is contiguous.  ``out`` may be the residual itself;
+    (slices of wider tensors), a row's elements are consecutive; weight is contiguous.  residual may be one row expanded over all.  ``out`` may be the residual itself;
     it must not overlap anything else (columns of one buffer that x, residual and out share out among them are fine).  Sums are
     formed in a fixed order: equal inputs give equal bits.  Forward only: nothing is
     recorded for autograd."""
@@ -1208,7 +1209,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     if residual is not None:
         if _token_tensor(residual, "residual", x).shape != shape:
             raise ValueError(f"residual must be {tuple(shape)}, got {tuple(residual.shape)}")
-        pr, _, rs = _rows(residual, "residual", K)
+        pr, _, rs = _rows(residual, "residual", K, one_row=True)
     if out is None:
         out = x.new_empty(shape)
         py, ys = out.data_ptr(), K
