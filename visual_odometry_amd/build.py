@@ -8,6 +8,7 @@ to the GPU box with the source tree.
 from __future__ import annotations
 
 import os
+import shlex
 import shutil
 import subprocess
 import sys
@@ -32,11 +33,36 @@ def hipcc() -> str:
     return exe
 
 
-def _newer(target: str, deps) -> bool:
-    if not os.path.exists(target):
+def _line(cmd) -> str:
+    """A command line as it is kept beside its target, the same wherever the tree lies."""
+    return shlex.join(cmd).replace(os.path.dirname(PKG) + os.sep, "")
+
+
+def _current(target: str, deps, cmd) -> bool:
+    """``target`` is newer than what it is made from and was made by this command line."""
+    try:
+        with open(target + ".cmd") as f:
+            if f.read() != _line(cmd):
+                return False
+        t = os.path.getmtime(target)
+        return all(os.path.getmtime(d) <= t for d in deps)
+    except FileNotFoundError:
         return False
-    t = os.path.getmtime(target)
-    return all(os.path.getmtime(d) <= t for d in deps)
+
+
+def _make(target: str, cmd, what: str) -> None:
+    """Runs ``cmd``, which makes ``target``; it takes its place when it is whole (another process may have the old one loaded)."""
+    part = f"{target}.{os.getpid()}.part"
+    r = subprocess.run([part if c == target else c for c in cmd], capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{what}:\n{r.stdout}\n{r.stderr}")
+    if r.stderr.strip():
+        sys.stderr.write(r.stderr)
+    if os.path.exists(target + ".cmd"):
+        os.remove(target + ".cmd")
+    os.replace(part, target)
+    with open(target + ".cmd", "w") as f:
+        f.write(_line(cmd))
 
 
 def sources():
@@ -49,31 +75,24 @@ def headers():
     return hs
 
 
-def _compile(src: str, extra=()) -> str:
+def _compile(src: str, force: bool = False) -> str:
     obj = os.path.join(OBJDIR, os.path.basename(src)[:-4] + ".o")
-    if _newer(obj, [src] + headers()):
-        return obj
-    cmd = [hipcc(), *CFLAGS, *extra, "-c", src, "-o", obj]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError(f"hipcc failed for {src}:\n{r.stdout}\n{r.stderr}")
-    if r.stderr.strip():
-        sys.stderr.write(r.stderr)
+    cmd = [hipcc(), *CFLAGS, "-c", src, "-o", obj]
+    if force or not _current(obj, [src] + headers(), cmd):
+        _make(obj, cmd, f"hipcc failed for {src}")
     return obj
 
 
 def build_library(force: bool = False, jobs: int = 8) -> str:
+    """The library, from what has changed (``force``: from every source)."""
     os.makedirs(LIBDIR, exist_ok=True)
     os.makedirs(OBJDIR, exist_ok=True)
     srcs = sources()
-    if not force and _newer(LIB, srcs + headers()):
-        return LIB
     with ThreadPoolExecutor(max_workers=min(jobs, len(srcs))) as ex:
-        objs = list(ex.map(_compile, srcs))
+        objs = list(ex.map(lambda src: _compile(src, force), srcs))
     cmd = [hipcc(), "-shared", "-fPIC", f"--offload-arch={ARCH}", "-o", LIB, *objs]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
+    if force or not _current(LIB, objs, cmd):
+        _make(LIB, cmd, "link failed")
     return LIB
 
 
@@ -82,12 +101,9 @@ def build_host_checks() -> str:
     root = os.path.dirname(PKG)
     src = os.path.join(root, "tests", "host_checks.hip")
     out = os.path.join(root, "tests", "_host_checks.so")
-    if _newer(out, [src] + headers()):
-        return out
     cmd = [hipcc(), "-O2", "-std=c++17", "-fPIC", "-shared", f"--offload-arch={ARCH}", src, "-o", out]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError(f"hipcc failed for {src}:\n{r.stdout}\n{r.stderr}")
+    if not _current(out, [src] + headers(), cmd):
+        _make(out, cmd, f"hipcc failed for {src}")
     return out
 
 
