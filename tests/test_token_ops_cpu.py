@@ -172,3 +172,25 @@ def test_overlaps_are_found_and_column_ranges_are_none():
         if step:
             columns = [{(v[2] + i) % step for i in range(v[0][1])} for v in (a, b)]
             assert not says or columns[0] & columns[1], (a, b)
+
+
+def test_more_threads_than_a_launch_has_are_refused_also_where_the_count_passes_64_bits():
+    from visual_odometry_amd import _lib
+    lib = _lib.load()
+    p = ctypes.cast((ctypes.c_char * 4096)(), ctypes.c_void_p)
+    p = ctypes.c_void_p((p.value + 15) // 16 * 16)
+
+    def attention(S, T, H, D=32, dt=1):
+        return lib.vo_attention(p, H * D, D, p, H * D, D, p, H * D, D, p, H * D, D, p, p, S, T, T, H, H, D, 1.0, 0, dt, p, 1 << 60, None)
+
+    def linear(M, C, K):
+        return lib.vo_linear(p, C, p, None, None, 0, p, K, M, C, K, 0, 1, p, 1 << 60, None)
+    # ten million single tokens: as many workgroups of up to 512 threads
+    for D, dt in ((32, 1), (128, 2), (32, 0), (64, 0)):
+        assert attention(10_000_000, 10_000_000, 1, D, dt) == _lib.VO_ERR_UNSUPPORTED and b"too many" in lib.vo_last_error()
+    big = (1 << 31) - 1
+    assert lib.vo_attention(p, 0, 0, p, 0, 0, p, 0, 0, p, 32, 0, p, p, big, 1, 1, big, big, 32, 1.0, 0, 1, p, 1 << 60, None) == _lib.VO_ERR_UNSUPPORTED
+    assert lib.vo_attention_workspace_bytes(1, 1, big, big, big, 32, 1) == 0
+    for M, K in ((1 << 55, 1 << 17), (1 << 62, 1 << 20), ((1 << 63) - 1, 64), (1 << 45, 1 << 30)):
+        assert linear(M, 8, K) == _lib.VO_ERR_UNSUPPORTED and b"too large" in lib.vo_last_error(), (M, K)
+        assert lib.vo_linear_workspace_bytes(M, 8, K, 1) == 0

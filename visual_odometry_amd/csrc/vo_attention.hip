@@ -668,6 +668,7 @@ struct Plan {
 // 8 heads of 128 over 2, causal: 196, with 64 keys and one workgroup a CU 424.
 constexpr int padded(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : D <= 128 ? 128 : 256; }
 constexpr int tile_keys(int DT, int es) { return DT * es > 512 || (es == 4 && DT >= 64) ? 32 : 64; }
+constexpr int rows_waves(int DT, int es) { return DT * es <= 256 ? 8 : DT * es <= 512 ? 4 : 2; }
 constexpr int tile_blocks(int DT) { return DT <= 64 ? 4 : DT == 96 ? 3 : DT == 128 ? 2 : 1; }
 
 Plan plan(int64_t Tq, int64_t Tk, int sequences, int Hq, int Hk, int D, int dtype) {
@@ -723,13 +724,21 @@ Plan plan(int64_t Tq, int64_t Tk, int sequences, int Hq, int Hk, int D, int dtyp
     return p;
 }
 
+// A launch has fewer than 2^32 threads.  Sizes that pass this by far (2^25 workgroups of the fewest threads, by a bound from below) are
+// told first: the products in plan() could pass 64 bits.
+bool too_many(int64_t Tq, int sequences, int Hq, int Hk) { return (double)Tq * Hq / 128 + (sequences - 1.) * Hk >= (double)(1 << 25); }
+bool too_many(const Plan& p, int64_t Tq, int Hq, int D, int dtype) {
+    const int threads = p.rows ? 64 * rows_waves(padded(D), dtype == VO_F32 ? 4 : 2) : 256;
+    return p.blocks * threads >= (1ll << 32) || (p.splits > 1 && Tq * Hq * 64 >= (1ll << 32));
+}
+
 int64_t workspace(const Plan& p, int64_t Tq, int Hq, int D) { return p.splits > 1 ? (int64_t)p.splits * Tq * Hq * (D + 2) * 4 : 0; }
 
 template <typename T, int DT> int launch(const AttArgs& a, const Plan& p, hipStream_t st) {
     constexpr int BYTES = DT * (int)sizeof(T);                       // of a row
     const dim3 grid((unsigned)p.blocks);
     if (p.rows) {
-        constexpr int KEYS = BYTES <= 128 ? 64 : 32, WAVES = BYTES <= 256 ? 8 : BYTES <= 512 ? 4 : 2;
+        constexpr int KEYS = BYTES <= 128 ? 64 : 32, WAVES = rows_waves(DT, sizeof(T));
         attention_rows<T, DT, KEYS, WAVES><<<grid, 64 * WAVES, 0, st>>>(a);
     } else {
         attention_tiles<T, DT, tile_keys(DT, sizeof(T)), tile_blocks(DT)><<<grid, 256, 0, st>>>(a);
@@ -754,6 +763,7 @@ template <typename T> int dispatch(const AttArgs& a, const Plan& p, hipStream_t 
 
 extern "C" int64_t vo_attention_workspace_bytes(int64_t q_tokens, int64_t k_tokens, int sequences, int q_heads, int k_heads, int D, int dtype) {
     if (q_tokens <= 0 || k_tokens < 0 || sequences <= 0 || q_heads <= 0 || k_heads <= 0 || q_heads % k_heads || D <= 0) return 0;
+    if (too_many(q_tokens, sequences, q_heads, k_heads)) return 0;
     return workspace(plan(q_tokens, k_tokens, sequences, q_heads, k_heads, D, dtype), q_tokens, q_heads, D);
 }
 
@@ -785,8 +795,9 @@ extern "C" int vo_attention(const void* q, int64_t q_token_stride, int64_t q_hea
         return vo_fail(VO_ERR_UNSUPPORTED, "vo_attention: tensors must be 16-byte aligned");
     if (q_tokens >= (1ll << 31) || k_tokens >= (1ll << 31))
         return vo_fail(VO_ERR_UNSUPPORTED, "vo_attention: offsets are 32-bit: fewer than 2^31 tokens");
-    const Plan p = plan(q_tokens, k_tokens, sequences, q_heads, k_heads, D, dtype);
-    if (p.blocks * 256 >= (1ll << 32) || (p.splits > 1 && q_tokens * q_heads * 64 >= (1ll << 32)))      // threads of a launch
+    const bool many = too_many(q_tokens, sequences, q_heads, k_heads);
+    const Plan p = many ? Plan{} : plan(q_tokens, k_tokens, sequences, q_heads, k_heads, D, dtype);
+    if (many || too_many(p, q_tokens, q_heads, D, dtype))
         return vo_fail(VO_ERR_UNSUPPORTED, "vo_attention: %lld tokens of %d heads are too many for one launch", (long long)q_tokens, q_heads);
     const int64_t need = workspace(p, q_tokens, q_heads, D);
     VO_REQUIRE(need == 0 || (workspace_ptr && workspace_bytes >= need && reinterpret_cast<uintptr_t>(workspace_ptr) % 16 == 0),

@@ -517,6 +517,10 @@ Plan plan(int64_t M, int C, int K, int dtype) {
     return p;
 }
 
+// A launch has fewer than 2^32 threads.  Sizes that pass this by far (2^23 tiles of the largest size) are told first: the products in
+// plan() could pass 64 bits.
+bool too_large(int64_t M, int K) { return (double)M * K >= (double)(1ll << 39); }
+
 int64_t needed(const Plan& p, int64_t M, int K, int dtype) {
     return p.padded * (dtype == VO_F32 ? 4 : 2) + (p.splits > 1 ? (int64_t)p.splits * M * K * 4 : 0);
 }
@@ -565,7 +569,7 @@ template <typename T> int dispatch(LinArgs a, Plan p, hipStream_t st) {
 }  // namespace
 
 extern "C" int64_t vo_linear_workspace_bytes(int64_t M, int C, int K, int dtype) {
-    if (M <= 0 || C <= 0 || K <= 0) return 0;
+    if (M <= 0 || C <= 0 || K <= 0 || too_large(M, K)) return 0;
     return needed(plan(M, C, K, dtype), M, K, dtype);
 }
 
@@ -580,13 +584,13 @@ extern "C" int vo_linear(const void* x, int64_t x_row_stride, const void* weight
     VO_REQUIRE(x_row_stride >= C && y_row_stride >= K && (!residual || residual_row_stride >= K || residual_row_stride == 0),
                "vo_linear: row strides must be at least the rows' lengths (the residual's may be 0)");
     const int64_t es = dtype == VO_F32 ? 4 : 2;
-    const Plan p = plan(M, C, K, dtype);
     // a tile's rows are addressed with 32-bit offsets
     if (x_row_stride * es * 256 >= (1ll << 31) || (int64_t)C * es * 256 >= (1ll << 31))
         return vo_fail(VO_ERR_UNSUPPORTED, "vo_linear: rows of x and weight must be under 8 MiB");
-    // a launch has fewer than 2^32 threads (large forms may be run as tiles of half the side)
-    const int64_t limit = 1ll << 32;
-    if (p.tiles_m * p.tiles_n * p.splits * (p.form == 0 ? 512 : 1024) >= limit || M * vo_ceil_div(K, 4) >= limit * 64 ||
+    const bool large = too_large(M, K);
+    const Plan p = large ? Plan{} : plan(M, C, K, dtype);
+    const int64_t limit = 1ll << 32;                                 // (large forms may be run as tiles of half the side)
+    if (large || p.tiles_m * p.tiles_n * p.splits * (p.form == 0 ? 512 : 1024) >= limit || M * vo_ceil_div(K, 4) >= limit * 64 ||
         (p.splits > 1 && M * vo_ceil_div(K, 16 / es) >= limit) || p.padded / (16 / es) >= limit)
         return vo_fail(VO_ERR_UNSUPPORTED, "vo_linear: M=%lld C=%d K=%d is too large for one launch", (long long)M, C, K);
     const int64_t need = needed(p, M, K, dtype);
