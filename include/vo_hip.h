@@ -639,16 +639,16 @@ int vo_linear(const void* x, int64_t x_row_stride, const void* weight, const flo
  * Attention of packed sequences: row i of a sequence gives
  *     out[i,h,:] = sum_j p_ij v[j,h',:],   p_ij = softmax_j(scale * q[i,h,:] . k[j,h',:]),   h' = h / (q_heads / k_heads)
  * over the keys j of its sequence (scale from 1e-30 to 1e30; scores of any size that float32 holds); with causal != 0 over
- * those with j <= i + Lk - Lq (Lq, Lk the sequence's rows and keys:
- * its last row sees every key).  A row that sees no key gives zeros.  It has NO counterpart in the reference; it is the
- * all-pairs product of vo_corr_volume_1d / _2d without the volume: along the epipolar lines of a stereo pair (one sequence
- * a line, causal: a match lies never right of its pixel), among all pixels of a frame, over packed prompts of any lengths,
- * or for one new token over a long cache.
+ * those with j <= i + Lk - Lq (Lq, Lk the sequence's rows and keys: its last row sees every key).  A row that sees no key gives
+ * zeros.  It has NO counterpart in the reference; it is the all-pairs product of vo_corr_volume_1d / _2d without the volume:
+ * along the epipolar lines of a stereo pair (one sequence a line, causal: a match lies never right of its pixel), among all
+ * pixels of a frame, over packed prompts of any lengths, or for one new token over a long cache.
  *   q, out (q_tokens, q_heads, D), k, v (k_tokens, k_heads, D): D consecutive elements per token and head, token and head
  *   strides in ELEMENTS, so slices of one fused projection are fine.  Storage VO_F32, VO_F16 or VO_BF16; products, softmax
- *   and sums in float32; with 16-bit storage the exponentials are rounded to it (relative to the row's largest) before they
- *   meet v, and the result is rounded once.  D at most 256; D, strides and pointers whole 16-byte pieces, tokens under
- *   16 MiB apart (VO_ERR_UNSUPPORTED otherwise); heads may lie any distance apart.  out overlaps none of the inputs.
+ *   and sums in float32; with 16-bit storage the exponentials are rounded to it (relative to the row's largest; float16: to
+ *   steps of 2^-31 and up) before they meet v, and the result is rounded once.  D at most 256; D, strides and pointers whole
+ *   16-byte pieces, tokens under 16 MiB apart (VO_ERR_UNSUPPORTED otherwise); heads may lie any distance apart.  out overlaps
+ *   none of the inputs.
  *   q_offsets, k_offsets: device arrays of sequences + 1 ascending int32: sequence s owns the rows [q_offsets[s],
  *   q_offsets[s+1]) and the keys [k_offsets[s], k_offsets[s+1]), any length from 0; or both NULL with sequences = 1: all
  *   rows and keys.  Rows outside every sequence are left as they were.  The offsets are read on the device and clamped to

@@ -555,3 +555,19 @@ def test_result_beside_its_inputs_in_one_buffer(vo, dtype, lens, order):
     for first in (1, Hq - 1, Hq, Hq + Hk, Hq + 2 * Hk - 1):
         with pytest.raises(ValueError, match="overlaps"):
             ops.attention(q, k, v, offsets(lens), causal=True, out=hold[:, first:first + Hq])
+
+
+@pytest.mark.parametrize("rows,keys,heads", [(1, 3000, 1), (1, 200000, 1), (130, 100000, 1), (1000, 30000, 128), (1, 900, 64)])
+def test_float16_keys_far_below_the_first_count_together(vo, rows, keys, heads):
+    """One key 18 ahead of all others (e^-18 = 2^-26): one of the others weighs less than float16's smallest number, all of them
+    together do not."""
+    D = 64
+    q = torch.zeros(rows, heads, D, device="cuda", dtype=torch.float16)
+    k, v = torch.zeros(keys, 1, D, device="cuda", dtype=torch.float16), torch.zeros(keys, 1, D, device="cuda", dtype=torch.float16)
+    q[..., 0], k[0, 0, 0], v[1:] = 1, 18, 1
+    y = ops.attention(q, k.expand(keys, heads, D), v.expand(keys, heads, D), scale=1.0).double()
+    rest = (keys - 1) * np.exp(-18.0)
+    want = rest / (1 + rest)
+    # a weight of 2^-26, stored 2^7 up in steps of 2^-24: off by at most half a step, 2^-6 of itself; the float32 sums of n terms; the
+    # result's own rounding (2^-25 where it is subnormal)
+    assert float((y - want).abs().max()) <= want * (2.0 ** -6 + 2.0 ** -11 + 4 * (keys + 64) * U32) + 2.0 ** -25

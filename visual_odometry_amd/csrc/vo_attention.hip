@@ -15,7 +15,8 @@
 // leave the rounding of m c in it, which is 16 and more where scores times c pass 2^28 (no weight would be near 1, sums would vanish or
 // overflow).  The instruction more costs the prompts below 1.5 %, heads of 32 features 8 %; both forms under a test of |m c| spill.
 // m follows the true maximum only when it has grown by more than 2^8 in the exponentials, so most tiles need no
-// rescaling of the sums (the exponentials are then at most 256, which costs no bits in a floating-point format).
+// rescaling of the sums (the exponentials are then at most 256, which costs no bits in a floating-point format).  In float16 they are
+// kept 2^7 up, sums included: its smallest number is 2^-24, and thousands of keys below that beside one large one weigh something together.
 //
 // Two forms:
 //   tiles  a workgroup of four waves takes 128 rows of one key head (a row is a token and one of the heads that share the key
@@ -152,12 +153,14 @@ template <typename T, int DT, int KEYS> struct Core {
             m = next;
         }
     }
+    static __device__ __forceinline__ float weight(float s, float c, float ref) {
+        return __builtin_amdgcn_exp2f(__is_same(T, _Float16) ? __builtin_fmaf(s - ref, c, 7.f) : (s - ref) * c);
+    }
     // Scores 2 j and 2 j + 1 of a block of 32 keys to exponentials, rounded to the storage type where that has 16 bits; `sum` takes
     // the unrounded ones.
     static constexpr int PW = sizeof(T) == 2 ? 8 : 16;               // registers of a block's exponentials
     static __device__ __forceinline__ void weigh(const vo_f32x16& s, unsigned* p, float* sum, int j, float c, float ref) {
-        const float x = __builtin_amdgcn_exp2f((s[2 * j] - ref) * c);
-        const float y = __builtin_amdgcn_exp2f((s[2 * j + 1] - ref) * c);
+        const float x = weight(s[2 * j], c, ref), y = weight(s[2 * j + 1], c, ref);
         sum[0] += x;
         sum[1] += y;
         if constexpr (sizeof(T) == 2) {
@@ -260,7 +263,7 @@ template <typename T, int DT, int KEYS> struct Core {
             unsigned u = 0;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const float w = __builtin_amdgcn_exp2f((s[b][i] - ref) * c);
+                const float w = weight(s[b][i], c, ref);
                 bool zero = w == 0.f;
                 if constexpr (sizeof(T) == 2) zero = (E::pack2(w, 0.f) & 0x7fffu) == 0;
                 u |= (unsigned)zero << (8 * (i >> 2) + (i & 3));
