@@ -571,3 +571,26 @@ def test_float16_keys_far_below_the_first_count_together(vo, rows, keys, heads):
     # a weight of 2^-26, stored 2^7 up in steps of 2^-24: off by at most half a step, 2^-6 of itself; the float32 sums of n terms; the
     # result's own rounding (2^-25 where it is subnormal)
     assert float((y - want).abs().max()) <= want * (2.0 ** -6 + 2.0 ** -11 + 4 * (keys + 64) * U32) + 2.0 ** -25
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("step", [0, 8, 40])
+@pytest.mark.parametrize("q_len,n", [([10], 10), ([3], 10), ([140], 150), ([3], 70)])
+def test_tokens_that_overlap_in_memory(vo, dtype, causal, step, q_len, n):
+    """Keys and values that are windows of one array; an infinity in it reaches the features in whose place it stands, no others."""
+    D, lq = 64, q_len[0]
+    q, _, _ = make(q_len, [1], 1, 1, D, dtype, 19)
+    g = torch.Generator(device="cuda").manual_seed(20)
+    hold = [torch.randn(n * step + 2 * D, generator=g, device="cuda").to(dtype) for _ in range(2)]
+    k, v = (h.as_strided((n, 1, D), (step, D, 1)) for h in hold)
+    want, tol = reference(q, k, v, q_len, [n], causal, 0.125)
+    check(ops.attention(q, k, v, causal=causal), want, tol)
+    hold[1][(n - 1) * step + 30] = float("inf")
+    y = ops.attention(q, k, v, causal=causal)
+    at = torch.isinf(v[:, 0])                                          # (n, D)
+    last = torch.arange(lq, device="cuda") + (n - lq) if causal else torch.full((lq,), n - 1, device="cuda")
+    hit = (torch.arange(n, device="cuda")[None, :] <= last[:, None]).float() @ at.float() > 0
+    assert bool((y[:, 0][hit] == float("inf")).all())
+    ok = (y.double() - want).abs()[:, 0] <= tol[:, 0]
+    assert bool(ok[~hit].all())

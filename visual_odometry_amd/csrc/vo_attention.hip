@@ -214,9 +214,10 @@ template <typename T, int DT, int KEYS> struct Core {
             }
     }
     // Values that are infinite or NaN ("unbounded").  Where all rows see the same keys they are products like others; where a row
-    // does not see a key its weight is zero, and zero times such a value is no zero.  So a tile on a causal sequence's diagonal
-    // that holds any is multiplied with zeros in their place, and their products are added at the end to the rows that see them: the
-    // value itself (any positive weight times it is it), or NaN where the weight beside the row's largest is zero all the same.
+    // does not see a key its weight is zero, and zero times such a value is no zero.  So a tile on a causal sequence's diagonal (or
+    // at the end of tokens that overlap in memory) that holds any is multiplied with zeros in their place, and their products are
+    // added at the end to the rows that see them: the value itself (any positive weight times it is it), or NaN where the weight
+    // beside the row's largest is zero all the same.
     static constexpr unsigned EXP = sizeof(T) == 4 ? 0x7f800000u : __is_same(T, _Float16) ? 0x7c00u : 0x7f80u;
     static __device__ __forceinline__ bool unbounded(unsigned bits) { return (bits & EXP) == EXP; }
     // Is there any in the tile?
@@ -418,7 +419,8 @@ __global__ __launch_bounds__(256, MIN_BLOCKS) void attention_tiles(const AttArgs
     // keys below `limit` are seen by this lane's row; tiles wholly below wave_all need no mask, from wave_any on no work; tiles
     // wholly below `all` are seen by every row of the workgroup
     const int64_t limit = a.causal ? vo_clamp64(token + shift + 1, 0, p.Lk) : p.Lk;
-    const int64_t all = a.causal ? vo_clamp64(first_token + shift + 1, 0, p.Lk) : p.Lk;
+    int64_t all = a.causal ? vo_clamp64(first_token + shift + 1, 0, p.Lk) : p.Lk;
+    if (a.vs < a.D && all == p.Lk) --all;                            // tokens overlap: a tile at their end holds parts of tokens behind the last
     int64_t unbounded = t1;                                          // the first tile that was bounded
     const int64_t wave_all = a.causal ? vo_clamp64(token_of(first) + shift + 1, 0, p.Lk) : p.Lk;
     const int64_t wave_any = first >= rows ? 0 : a.causal ? vo_clamp64(token_of(first + 31) + shift + 1, 0, p.Lk) : p.Lk;
@@ -507,7 +509,8 @@ __global__ __launch_bounds__(64 * WAVES) void attention_rows(const AttArgs a) {
     core.reset();
     core.load_q(have ? static_cast<const T*>(a.q) + (p.q0 + token) * a.qs + head * a.qh : nullptr, a.D, lane);
     const int64_t limit = a.causal ? vo_clamp64(token + shift + 1, 0, p.Lk) : p.Lk;
-    const int64_t all = a.causal ? vo_clamp64(p.row / a.group + shift + 1, 0, p.Lk) : p.Lk;
+    int64_t all = a.causal ? vo_clamp64(p.row / a.group + shift + 1, 0, p.Lk) : p.Lk;
+    if (a.vs < a.D && all == p.Lk) --all;                            // see attention_tiles
 
     const T* kb = static_cast<const T*>(a.k) + p.k0 * a.ks + kh * a.kh;
     const T* vb = static_cast<const T*>(a.v) + p.k0 * a.vs + kh * a.vh;
