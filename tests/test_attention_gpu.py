@@ -594,3 +594,21 @@ def test_tokens_that_overlap_in_memory(vo, dtype, causal, step, q_len, n):
     assert bool((y[:, 0][hit] == float("inf")).all())
     ok = (y.double() - want).abs()[:, 0] <= tol[:, 0]
     assert bool(ok[~hit].all())
+
+
+@pytest.mark.parametrize("rows,keys,heads", [(1, 300, 1), (300, 300, 1), (3, 5000, 1), (300, 5000, 1), (1000, 500, 128)])
+def test_means_of_float16s_largest_number_stay_finite(vo, rows, keys, heads):
+    """One key ahead of many equal ones whose weight, a little over (1 + 2^-11) / 2, rounds up by nearly half a step of float16, while
+    the sum that divides them is not rounded: the mean of equal values must not pass them, into infinity where they are the largest."""
+    q = torch.zeros(rows, heads, 32, device="cuda", dtype=torch.float16)
+    k, v = torch.zeros(keys, 1, 32, device="cuda", dtype=torch.float16), torch.empty(keys, 1, 32, device="cuda", dtype=torch.float16)
+    q[..., :2] = 1
+    k[1:, 0, 0] = float(np.log(0.5 * (1 + 2.0 ** -11 + 2.0 ** -15)))
+    k[1:, 0, 1] = float(np.log(0.5 * (1 + 2.0 ** -11 + 2.0 ** -15))) - float(k[1, 0, 0])
+    v[..., :16], v[..., 16:] = 65504, -65504
+    y = ops.attention(q, k.expand(keys, heads, 32), v.expand(keys, heads, 32), scale=1.0)
+    assert bool(y.isfinite().all())
+    assert float((y.double().abs() / 65504 - 1).abs().max()) <= 2.0 ** -10 + 4 * (keys + 64) * U32
+    v[0, 0, 5] = float("inf")
+    y = ops.attention(q, k.expand(keys, heads, 32), v.expand(keys, heads, 32), scale=1.0)
+    assert bool((y[..., 5] == float("inf")).all()) and bool(y[..., 6:].isfinite().all())

@@ -338,6 +338,14 @@ template <typename T, int DT, int KEYS, int WAVES> struct Loader {
     }
 };
 
+// A result in 16 bits.  The weights of the sum are rounded, the sum of weights that divides it is not: a mean of numbers near the
+// type's largest may pass it by a rounding, but is finite like them.
+template <typename T> constexpr float LARGEST = __is_same(T, _Float16) ? 65504.f : __is_same(T, __bf16) ? 0x1.fep127f : INFINITY;
+template <typename T> __device__ __forceinline__ float in_range(float x) {
+    if constexpr (sizeof(T) == 4) return x;
+    return fabsf(x) < INFINITY ? fminf(fmaxf(x, -LARGEST<T>), LARGEST<T>) : x;
+}
+
 // Where the results of a row go: the output, or (split) the workspace.
 __device__ __forceinline__ float* part_row(const AttArgs& a, int split, int64_t token, int head) {
     return a.part + (((int64_t)split * a.Tq + token) * a.Hq + head) * a.D;
@@ -358,16 +366,27 @@ __device__ __forceinline__ void store_rows(const vo_f32x16* o, float factor, int
     constexpr int ES = sizeof(S), CH = L::CH, EACH = L::PER;
     auto swz = [](int r) { return L::POW2 ? r & L::KMASK : L::k_swz(r); };
     const int r = lane & 31;
+    auto put = [&](auto result) {
 #pragma unroll
-    for (int d = 0; d < DT / 32; ++d)
+        for (int d = 0; d < DT / 32; ++d)
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            const int f = d * 32 + 8 * b + 4 * (lane >> 5);
-            unsigned char* p = lds + r * DT * ES + L::place(f / EACH, swz(r)) * 16 + f % EACH * ES;
-            const float v0 = o[d][4 * b] * factor, v1 = o[d][4 * b + 1] * factor, v2 = o[d][4 * b + 2] * factor, v3 = o[d][4 * b + 3] * factor;
-            if constexpr (ES == 2) *reinterpret_cast<vo_u32x2*>(p) = vo_u32x2{vo_elem<S>::pack2(v0, v1), vo_elem<S>::pack2(v2, v3)};
-            else *reinterpret_cast<vo_f32x4*>(p) = vo_f32x4{v0, v1, v2, v3};
-        }
+            for (int b = 0; b < 4; ++b) {
+                const int f = d * 32 + 8 * b + 4 * (lane >> 5);
+                unsigned char* p = lds + r * DT * ES + L::place(f / EACH, swz(r)) * 16 + f % EACH * ES;
+                const float v0 = result(o[d][4 * b]), v1 = result(o[d][4 * b + 1]), v2 = result(o[d][4 * b + 2]), v3 = result(o[d][4 * b + 3]);
+                if constexpr (ES == 2) *reinterpret_cast<vo_u32x2*>(p) = vo_u32x2{vo_elem<S>::pack2(v0, v1), vo_elem<S>::pack2(v2, v3)};
+                else *reinterpret_cast<vo_f32x4*>(p) = vo_f32x4{v0, v1, v2, v3};
+            }
+    };
+    float top = 0.f;                                                 // of the numbers: one test for all of a lane's
+    if constexpr (ES == 2) {
+#pragma unroll
+        for (int d = 0; d < DT / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(o[d][i]));
+    }
+    if (ES == 2 && __any(top * factor > LARGEST<S>)) put([&](float x) { return in_range<S>(x * factor); });
+    else put([&](float x) { return x * factor; });
     vo_wave_lds_fence();
 #pragma unroll
     for (int i = 0; i < CH / 2; ++i) {
@@ -599,7 +618,7 @@ __global__ __launch_bounds__(64 * WAVES) void attention_rows(const AttArgs a) {
             *reinterpret_cast<vo_f32x4*>(part_row(a, split, p.q0 + token, head) + f) = vo_f32x4{v[0], v[1], v[2], v[3]};
         } else if constexpr (sizeof(T) == 2) {
             *reinterpret_cast<vo_u32x2*>(out_row<T>(a, p.q0 + token, head) + f) =
-                vo_u32x2{vo_elem<T>::pack2(v[0] * inv, v[1] * inv), vo_elem<T>::pack2(v[2] * inv, v[3] * inv)};
+                vo_u32x2{vo_elem<T>::pack2(in_range<T>(v[0] * inv), in_range<T>(v[1] * inv)), vo_elem<T>::pack2(in_range<T>(v[2] * inv), in_range<T>(v[3] * inv))};
         } else {
             *reinterpret_cast<vo_f32x4*>(out_row<T>(a, p.q0 + token, head) + f) = vo_f32x4{v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv};
         }
@@ -657,7 +676,7 @@ template <typename T, int WIDTH> __global__ __launch_bounds__(256) void attentio
     const float inv = inverse(l);
     T* p = out_row<T>(a, token, head) + f;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) vo_elem<T>::put(p + j, o[j] * inv);
+    for (int j = 0; j < 4; ++j) vo_elem<T>::put(p + j, in_range<T>(o[j] * inv));
 }
 
 // ------------------------------------------------------------------------------------------------------------- host
