@@ -656,6 +656,8 @@ int vo_linear(const void* x, int64_t x_row_stride, const void* weight, const flo
  *   A key or value reaches the rows that see it and no others, whatever it holds: infinities and NaN too.  A key whose score is
  *   -infinity has the weight zero; a row with no other key gives zeros, like one that sees none.  The product of a weight of zero
  *   (also one that has underflown, in the storage type, beside the largest met up to there) and an infinite value is NaN.
+ * The form and the parts of the key axis are chosen for the average lengths, the only ones known to the host: sequences many
+ * times longer than the rest are better off in a call of their own.
  * workspace: vo_attention_workspace_bytes(...) bytes (often 0), 16-byte aligned, contents irrelevant.  Calls that share one
  * must be ordered on one stream; two captured graphs that may replay at once need one each.
  * ------------------------------------------------------------------------- */

@@ -9,6 +9,8 @@
 //                 keys that is, the sum over keys is the same as long as V^T is read in the same order.  So the exponentials
 //                 are already where the second product needs them: they are rounded to the 16-bit type in place (float32: not
 //                 at all) and no value crosses lanes.  m, l and the rescaling factor are one number per lane.
+// The rounding is what the 16-bit product takes; it carries the result's error from its own rounding's 0.0017 (bfloat16, relative to
+// 64 bits) to 0.0022, in float16 from 0.00021 to 0.00029.  To multiply the remainder too would be half as many products again.
 // V^T in 16 bits comes out of LDS by the transposing read: four keys of one feature per lane.
 //
 // The exponent's argument is (s - m) * scale * log2(e), with the difference formed first: s c - m c in one fused multiply-add would
@@ -23,11 +25,11 @@
 //          head); key tiles are shared in LDS, loaded while the previous tile is multiplied.  Matrix and vector work of a tile
 //          take about as long as each other and overlap between the two to four workgroups of a CU; the chip's power sets the
 //          clock (the same cycles are 38 % faster on zeros).  8 prompts of up to 8192 tokens, 32 / 8 heads of 128, bfloat16,
-//          causal: 2.04 ms = 1.02 PFLOP/s; 4800 float32 rows, 4 heads of 64: 207 us = 114 TFLOP/s of the 151 the library's
+//          causal: 2.09 ms = 1.00 PFLOP/s; 4800 float32 rows, 4 heads of 64: 204 us = 116 TFLOP/s of the 153 the library's
 //          product reaches.
 //   rows   few rows per sequence (single tokens above all): tiles of 32 rows, every wave streams key tiles of its own into its
 //          own part of LDS, the waves' results are joined at the end.  Bound by the read of keys and values: 32 caches of up to
-//          32768 tokens, 8 key heads of 128: 364 us = 5.4 TB/s; a single row before 777 keys 12 us, all of it waiting.
+//          32768 tokens, 8 key heads of 128: 363 us = 5.4 TB/s; a single row before 777 keys 12 us, all of it waiting.
 // Either can be split over the keys; the parts (m, l, unnormalised sums) go to a workspace and are joined in a fixed order.
 #include "vo_packed.h"
 #include "vo_tokens.h"
@@ -688,14 +690,17 @@ struct Plan {
 };
 
 // The features that a head is padded to, keys in a tile and workgroups a CU holds (LDS and registers) in the form by tiles.
-// 96 features: 16 heads of 72 or 96 over 4, 4 sequences of 3000, take 143 and 146 us, padded to 128 190 and 192.  32 keys in
-// float32, whose values take twice the registers, for more workgroups: 4800 rows, 4 heads of 64: 207 us, with 64 keys 226; 3000 rows,
+// 96 features: 16 heads of 72 or 96 over 4, 4 sequences of 3000, take 144 and 148 us, padded to 128 186 and 192.  32 keys in
+// float32, whose values take twice the registers, for more workgroups: 4800 rows, 4 heads of 64: 204 us, with 64 keys 226; 3000 rows,
 // 8 heads of 128 over 2, causal: 196, with 64 keys and one workgroup a CU 424.
 constexpr int padded(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : D <= 128 ? 128 : 256; }
 constexpr int tile_keys(int DT, int es) { return DT * es > 512 || (es == 4 && DT >= 64) ? 32 : 64; }
 constexpr int rows_waves(int DT, int es) { return DT * es <= 256 ? 8 : DT * es <= 512 ? 4 : 2; }
 constexpr int tile_blocks(int DT) { return DT <= 64 ? 4 : DT == 96 ? 3 : DT == 128 ? 2 : 1; }
 
+// The lengths are on the device, so the averages decide.  What that costs where they differ much (bfloat16, 32 heads over 8 of 128, causal):
+// single rows, a history of 32768 keys among 63 of 100: 186 us, in two calls 47; a prompt of 4096 among 600 tokens before 100 keys: 408
+// and 296; among 20 tokens before 2000 keys: 158 and 182.
 Plan plan(int64_t Tq, int64_t Tk, int sequences, int Hq, int Hk, int D, int dtype) {
     const int group = Hq / Hk;
     Plan p{};

